@@ -350,6 +350,26 @@ int ml_dice_loss_backward(const ml_dense_shape* s, int dtype, const float* grad_
                           float scale, void* grad, void* workspace, size_t workspace_bytes,
                           ml_stream_t stream);
 
+/* ---- layer norm (no counterpart in the reference) ----------------------------
+ * Over the last dimension of x (rows, width) in `dtype`: y = (x - m) r w + b with
+ * m = mean x and r = 1 / sqrt(mean (x - m)^2 + eps), the norm of a decoder's queries
+ * in front of the mask and class logits.  weight and bias (width,) in param_dtype
+ * (`dtype` or ML_F32), each NULL for ones / zeros.  mean and rstd: (rows,) float for
+ * the backward, both NULL where none follows.  Statistics are float32, summed about
+ * the mean.  Any width; eps >= 0.
+ * Backward: grad_input (rows, width) in `dtype`, grad_weight and grad_bias (width,)
+ * in param_dtype, each NULL where it is not wanted; sums over the rows are float32
+ * in a fixed order.  workspace (ml_layer_norm_backward_workspace_size bytes, 0 for an
+ * invalid shape) is needed for grad_weight and grad_bias. */
+int ml_layer_norm_forward(int dtype, int param_dtype, const void* x, const void* weight, const void* bias,
+                          int64_t rows, int64_t width, float eps, void* y, float* mean, float* rstd,
+                          ml_stream_t stream);
+size_t ml_layer_norm_backward_workspace_size(int64_t rows, int64_t width);
+int ml_layer_norm_backward(int dtype, int param_dtype, const void* grad_out, const void* x,
+                           const void* weight, const float* mean, const float* rstd, int64_t rows,
+                           int64_t width, void* grad_input, void* grad_weight, void* grad_bias,
+                           void* workspace, size_t workspace_bytes, ml_stream_t stream);
+
 /* ---- input validation helper ------------------------------------------------
  * flag[0] = 1 if any of x[0..n) equals `value`, else 0 (one small kernel, no
  * synchronisation).  Replaces the device-wide comparison + reduction behind

@@ -8,6 +8,7 @@
 // src/cpu/matching.cpp:618).
 #include <ATen/hip/HIPContext.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <chrono>
@@ -843,6 +844,141 @@ torch::Tensor backward_dice_loss(const torch::Tensor& grad_out, const torch::Ten
   return grad;
 }
 
+// --------------------------------------------------------------------------
+// layer norm over the last dimension (no counterpart in the reference)
+// --------------------------------------------------------------------------
+// (rows, width) of a layer norm's input; weight and bias as given to it.
+struct NormArgs {
+  int64_t rows, width;
+  int dt, pdt;
+};
+NormArgs norm_args(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
+                   const c10::optional<torch::Tensor>& bias) {
+  ML_CHECK_INPUT(x);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "layer_norm: input must have a last dimension of at least 1");
+  NormArgs a;
+  a.width = x.size(-1);
+  a.rows = x.numel() / a.width;
+  a.dt = a.pdt = dtype_code(x, "input");
+  bool first = true;
+  for (const auto* p : {&weight, &bias}) {
+    if (!p->has_value()) continue;
+    const torch::Tensor& t = **p;
+    ML_CHECK_INPUT(t);
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == a.width, "layer_norm: weight and bias must have shape (",
+                a.width, ",), the input's last dimension");
+    TORCH_CHECK(t.device() == x.device(), "all tensors must be on the same device");
+    const int d = dtype_code(t, "weight and bias");
+    TORCH_CHECK(d == a.dt || d == ML_F32,
+                "layer_norm: weight and bias must have the input's dtype or be float32");
+    TORCH_CHECK(first || d == a.pdt, "layer_norm: weight and bias must have the same dtype");
+    a.pdt = d;
+    first = false;
+  }
+  return a;
+}
+
+const void* ptr_or_null(const c10::optional<torch::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+// y[, mean, rstd]
+std::vector<torch::Tensor> layer_norm_forward(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
+                                              const c10::optional<torch::Tensor>& bias, double eps,
+                                              bool want_stats) {
+  const NormArgs a = norm_args(x, weight, bias);
+  TORCH_CHECK_VALUE(eps >= 0.0, "layer_norm: eps must not be negative");
+  const c10::DeviceGuard guard(x.device());
+  std::vector<torch::Tensor> r = {torch::empty_like(x)};
+  if (want_stats)
+    for (int i = 0; i < 2; ++i) r.push_back(torch::empty({a.rows}, x.options().dtype(torch::kFloat32)));
+  ml_ok(ml_layer_norm_forward(a.dt, a.pdt, x.data_ptr(), ptr_or_null(weight), ptr_or_null(bias), a.rows, a.width,
+                              (float)eps, r[0].data_ptr(), want_stats ? r[1].data_ptr<float>() : nullptr,
+                              want_stats ? r[2].data_ptr<float>() : nullptr, cur_stream()));
+  return r;
+}
+
+// gradients of the input, the weight and the bias, those asked for (the others undefined)
+std::vector<torch::Tensor> layer_norm_backward(const torch::Tensor& grad_out, const torch::Tensor& x,
+                                               const c10::optional<torch::Tensor>& weight,
+                                               const torch::Tensor& mean, const torch::Tensor& rstd,
+                                               bool need_input, bool need_weight, bool need_bias,
+                                               bool params_f32) {
+  NormArgs a = norm_args(x, weight, c10::nullopt);
+  if (params_f32) a.pdt = ML_F32;
+  ML_CHECK_INPUT(grad_out);
+  ML_CHECK_INPUT(mean);
+  ML_CHECK_INPUT(rstd);
+  TORCH_CHECK(grad_out.sizes() == x.sizes() && grad_out.scalar_type() == x.scalar_type(),
+              "layer_norm: grad_out must match the input in shape and dtype");
+  TORCH_CHECK(mean.scalar_type() == torch::kFloat32 && rstd.scalar_type() == torch::kFloat32 &&
+                  mean.numel() == a.rows && rstd.numel() == a.rows,
+              "layer_norm: mean and rstd must be float32, one value per row");
+  TORCH_CHECK(grad_out.device() == x.device() && mean.device() == x.device() && rstd.device() == x.device(),
+              "all tensors must be on the same device");
+  const c10::DeviceGuard guard(x.device());
+  const auto popt = a.pdt == ML_F32 ? x.options().dtype(torch::kFloat32) : x.options();
+  torch::Tensor dx, dw, db, ws;
+  if (need_input) dx = torch::empty_like(x);
+  if (need_weight) dw = torch::empty({a.width}, popt);
+  if (need_bias) db = torch::empty({a.width}, popt);
+  if (need_weight || need_bias) ws = workspace(ml_layer_norm_backward_workspace_size(a.rows, a.width), x);
+  auto p = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  ml_ok(ml_layer_norm_backward(a.dt, a.pdt, grad_out.data_ptr(), x.data_ptr(), ptr_or_null(weight),
+                               mean.data_ptr<float>(), rstd.data_ptr<float>(), a.rows, a.width, p(dx), p(dw), p(db),
+                               p(ws), ws.defined() ? ws.numel() : 0, cur_stream()));
+  return {dx, dw, db};
+}
+
+// Gradients of a backward that has none of its own: under create_graph they carry a
+// node that raises when something differentiates them.
+torch::autograd::variable_list once(torch::autograd::variable_list g, const char* msg) {
+  if (!torch::GradMode::is_enabled()) return g;
+  torch::autograd::variable_list vars;
+  for (auto& x : g)
+    if (x.defined()) vars.push_back(x.detach().set_requires_grad(true));
+  auto node = std::make_shared<torch::autograd::DelayedError>(msg, (int64_t)vars.size());
+  const auto out = (*node)(std::move(vars));
+  size_t i = 0;
+  for (auto& x : g)
+    if (x.defined()) x = out[i++];
+  return g;
+}
+
+struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input,
+                               const c10::optional<torch::Tensor>& weight,
+                               const c10::optional<torch::Tensor>& bias, double eps) {
+    auto cont = [](const c10::optional<torch::Tensor>& t) {
+      return t.has_value() ? c10::optional<torch::Tensor>(t->contiguous()) : t;
+    };
+    const auto x = input.contiguous();
+    const auto w = cont(weight), b = cont(bias);
+    auto r = layer_norm_forward(x, w, b, eps, true);
+    ctx->save_for_backward({x, w.has_value() ? *w : torch::Tensor(), r[1], r[2]});
+    // the weight's and the bias's gradients have their common dtype
+    const auto& p = w.has_value() ? w : b;
+    ctx->saved_data["params_f32"] = p.has_value() && p->scalar_type() == torch::kFloat32;
+    ctx->saved_data["bias"] = b.has_value();
+    return r[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto sv = ctx->get_saved_variables();
+    c10::optional<torch::Tensor> w;
+    if (sv[1].defined()) w = sv[1];
+    // only tensors that were given count as inputs of the node
+    const bool need_w = w.has_value() && ctx->needs_input_grad(1);
+    const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.has_value() ? 2 : 1);
+    const auto r = layer_norm_backward(g[0].detach().contiguous(), sv[0], w, sv[2], sv[3], ctx->needs_input_grad(0),
+                                       need_w, need_b, ctx->saved_data["params_f32"].toBool());
+    return once({r[0], r[1], r[2], torch::Tensor()}, "the backward of layer_norm cannot be differentiated");
+  }
+};
+
+torch::Tensor layer_norm_autograd(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
+                                  const c10::optional<torch::Tensor>& bias, double eps) {
+  return LayerNormNode::apply(input, weight, bias, eps);
+}
+
 // Device flag (int32, shape (1,)): 1 if any element of `x` equals `value`.
 torch::Tensor any_equal(const torch::Tensor& x, int64_t value) {
   ML_CHECK_INPUT(x);
@@ -920,6 +1056,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Pairwise sigmoid CE over sampled points (HIP)");
   m.def("forward_pw_dice_loss_sampling", &forward_pw_dice_loss_sampling,
         "Pairwise dice loss over sampled points (HIP)");
+  m.def("layer_norm_forward", &layer_norm_forward,
+        "Layer norm over the last dimension: output, and per row mean and 1/deviation if asked for (HIP)",
+        py::arg("input"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("want_stats") = false);
+  m.def("layer_norm_backward", &layer_norm_backward,
+        "Gradients of layer_norm_forward with respect to input, weight and bias (HIP)", py::arg("grad_out"),
+        py::arg("input"), py::arg("weight"), py::arg("mean"), py::arg("rstd"), py::arg("need_input") = true,
+        py::arg("need_weight") = true, py::arg("need_bias") = true, py::arg("params_f32") = false);
+  m.def("layer_norm_autograd", &layer_norm_autograd,
+        "Layer norm as a C++ autograd node, differentiable in input, weight and bias (HIP)", py::arg("input"),
+        py::arg("weight"), py::arg("bias"), py::arg("eps"));
   m.def("any_equal", &any_equal, "Device flag: any element equal to value (HIP)");
   m.attr("__backend__") = "hip-gfx950";
 }

@@ -19,6 +19,7 @@ from .label.pw_sigmoid_label_loss import PairwiseSigmoidLabelLossFunction
 from .label.pw_softmax_label_loss import PairwiseSoftmaxLabelLossFunction, pairwise_softmax_label_loss
 from .mask.pw_mask import PairwiseMaskLossFunction
 from .mask.matching import MaskMatchingFunction
+from .head.layer_norm import LayerNormFunction, layer_norm
 from .losses import sigmoid_cross_entropy_loss, dice_loss
 
 __all__ = [
@@ -38,4 +39,6 @@ __all__ = [
     "point_sample",
     "calculate_uncertainty",
     "get_uncertain_point_coords_with_randomness",
+    "LayerNormFunction",
+    "layer_norm",
 ]
