@@ -370,6 +370,37 @@ int ml_layer_norm_backward(int dtype, int param_dtype, const void* grad_out, con
                            int64_t width, void* grad_input, void* grad_weight, void* grad_bias,
                            void* workspace, size_t workspace_bytes, ml_stream_t stream);
 
+/* ---- products of ragged groups of rows with one matrix per group ---------------
+ * No counterpart in the reference: what makes the mask logits of its operators (an
+ * image's queries times its feature map), for query sets of any size per image.
+ * Rows offsets[g] .. offsets[g + 1] of x (rows, K) form group g of `groups` and take
+ * matrix g % matrices of weight (matrices, K, N), or (matrices, N, K) with
+ * `transposed`: y_r = x_r W.  So L * B query sets (layer major) share B feature
+ * maps.  groups is a positive multiple of matrices, at most 4,000; K, N <= 2^22.
+ * offsets: (groups + 1) int64 on the device, not decreasing; each is held to
+ * 0 .. rows and to at least the one before.  NULL: groups of rows / groups rows.  Rows in no group (before the first or
+ * behind the last) take zeros in y and grad_input and count for no grad_weight.
+ * All tensors in `dtype`; sums are float32, rounded once, in an order that the
+ * shape fixes.  grad_weight has weight's layout.
+ * Workspace: ml_grouped_matmul_workspace_size bytes for the product, 0 for a
+ * shape that is refused. */
+typedef struct ml_grouped_shape {
+  int64_t rows, K, N, groups, matrices;
+} ml_grouped_shape;
+enum { ML_GROUPED_FORWARD = 0, ML_GROUPED_BACKWARD_INPUT = 1, ML_GROUPED_BACKWARD_WEIGHT = 2 };
+size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, int dtype, int product);
+int ml_grouped_matmul_forward(const ml_grouped_shape* s, int dtype, const void* x, const void* weight,
+                              int transposed, const int64_t* offsets, void* y, void* workspace,
+                              size_t workspace_bytes, ml_stream_t stream);
+int ml_grouped_matmul_backward_input(const ml_grouped_shape* s, int dtype, const void* grad_out,
+                                     const void* weight, int transposed, const int64_t* offsets,
+                                     void* grad_input, void* workspace, size_t workspace_bytes,
+                                     ml_stream_t stream);
+int ml_grouped_matmul_backward_weight(const ml_grouped_shape* s, int dtype, const void* x,
+                                      const void* grad_out, int transposed, const int64_t* offsets,
+                                      void* grad_weight, void* workspace, size_t workspace_bytes,
+                                      ml_stream_t stream);
+
 /* ---- input validation helper ------------------------------------------------
  * flag[0] = 1 if any of x[0..n) equals `value`, else 0 (one small kernel, no
  * synchronisation).  Replaces the device-wide comparison + reduction behind

@@ -979,6 +979,143 @@ torch::Tensor layer_norm_autograd(const torch::Tensor& input, const c10::optiona
   return LayerNormNode::apply(input, weight, bias, eps);
 }
 
+// --------------------------------------------------------------------------
+// products of ragged groups of rows with one matrix per group (no counterpart
+// in the reference)
+// --------------------------------------------------------------------------
+// x (R, K) with offsets (groups + 1,), or (groups, n, K) without; weight
+// (matrices, K, N), or (matrices, N, K) with `transposed`.
+ml_grouped_shape grouped_shape(const torch::Tensor& x, const torch::Tensor& weight,
+                               const c10::optional<torch::Tensor>& offsets, bool transposed, bool out_rows) {
+  TORCH_CHECK(weight.dim() == 3, "grouped_matmul: weight must be (matrices, K, N), or (matrices, N, K) if transposed");
+  ml_grouped_shape s;
+  s.matrices = weight.size(0);
+  s.K = weight.size(transposed ? 2 : 1);
+  s.N = weight.size(transposed ? 1 : 2);
+  const int64_t width = out_rows ? s.N : s.K;
+  const char* what = out_rows ? "grad_out" : "input";
+  if (offsets.has_value()) {
+    const torch::Tensor& o = *offsets;
+    ML_CHECK_INPUT(o);
+    TORCH_CHECK(o.scalar_type() == torch::kLong, "offsets must be int64");
+    TORCH_CHECK(o.dim() == 1 && o.size(0) >= 2, "grouped_matmul: offsets must have shape (groups + 1,)");
+    TORCH_CHECK(o.device() == x.device(), "all tensors must be on the same device");
+    TORCH_CHECK(x.dim() == 2, "grouped_matmul: ", what, " must be (rows, ", width, ") with offsets");
+    s.groups = o.size(0) - 1;
+    s.rows = x.size(0);
+  } else {
+    TORCH_CHECK(x.dim() == 3, "grouped_matmul: ", what, " must be (groups, rows, ", width, ") without offsets");
+    s.groups = x.size(0);
+    s.rows = s.groups * x.size(1);
+  }
+  TORCH_CHECK(x.size(-1) == width, "grouped_matmul: ", what, " must have ", width, " columns, got ", x.size(-1));
+  TORCH_CHECK(s.matrices >= 1 && s.groups >= 1 && s.groups % s.matrices == 0,
+              "grouped_matmul: the number of groups must be a positive multiple of the number of matrices");
+  TORCH_CHECK(x.scalar_type() == weight.scalar_type(), "grouped_matmul: input and weight must have the same dtype");
+  TORCH_CHECK(x.device() == weight.device(), "all tensors must be on the same device");
+  return s;
+}
+
+const int64_t* offsets_ptr(const c10::optional<torch::Tensor>& o) {
+  return o.has_value() ? o->data_ptr<int64_t>() : nullptr;
+}
+
+torch::Tensor grouped_ws(const ml_grouped_shape& s, int dt, int product, const torch::Tensor& like) {
+  const size_t bytes = ml_grouped_matmul_workspace_size(&s, dt, product);
+  TORCH_CHECK(bytes > 0, ml_last_error());
+  return workspace(bytes, like);
+}
+
+std::vector<int64_t> with_width(const torch::Tensor& x, int64_t width) {
+  auto v = x.sizes().vec();
+  v.back() = width;
+  return v;
+}
+
+torch::Tensor grouped_matmul_forward(const torch::Tensor& x, const torch::Tensor& weight,
+                                     const c10::optional<torch::Tensor>& offsets, bool transposed) {
+  ML_CHECK_INPUT(x);
+  ML_CHECK_INPUT(weight);
+  const ml_grouped_shape s = grouped_shape(x, weight, offsets, transposed, false);
+  const int dt = dtype_code(x, "input");
+  const c10::DeviceGuard guard(x.device());
+  auto y = torch::empty(with_width(x, s.N), x.options());
+  auto ws = grouped_ws(s, dt, ML_GROUPED_FORWARD, x);
+  ml_ok(ml_grouped_matmul_forward(&s, dt, x.data_ptr(), weight.data_ptr(), transposed, offsets_ptr(offsets),
+                                  y.data_ptr(), ws.data_ptr(), ws.numel(), cur_stream()));
+  return y;
+}
+
+torch::Tensor grouped_matmul_backward_input(const torch::Tensor& grad_out, const torch::Tensor& weight,
+                                            const c10::optional<torch::Tensor>& offsets, bool transposed) {
+  ML_CHECK_INPUT(grad_out);
+  ML_CHECK_INPUT(weight);
+  const ml_grouped_shape s = grouped_shape(grad_out, weight, offsets, transposed, true);
+  const int dt = dtype_code(grad_out, "grad_out");
+  const c10::DeviceGuard guard(grad_out.device());
+  auto dx = torch::empty(with_width(grad_out, s.K), grad_out.options());
+  auto ws = grouped_ws(s, dt, ML_GROUPED_BACKWARD_INPUT, grad_out);
+  ml_ok(ml_grouped_matmul_backward_input(&s, dt, grad_out.data_ptr(), weight.data_ptr(), transposed,
+                                         offsets_ptr(offsets), dx.data_ptr(), ws.data_ptr(), ws.numel(),
+                                         cur_stream()));
+  return dx;
+}
+
+// gradient of a weight of `matrices` matrices, in its layout
+torch::Tensor grouped_matmul_backward_weight(const torch::Tensor& x, const torch::Tensor& grad_out,
+                                             const c10::optional<torch::Tensor>& offsets, int64_t matrices,
+                                             bool transposed) {
+  ML_CHECK_INPUT(x);
+  ML_CHECK_INPUT(grad_out);
+  TORCH_CHECK(matrices >= 1, "grouped_matmul: at least one matrix");
+  TORCH_CHECK(x.dim() >= 2 && x.dim() == grad_out.dim(), "grouped_matmul: input and grad_out must have the same rows");
+  for (int64_t i = 0; i + 1 < x.dim(); ++i)
+    TORCH_CHECK(x.size(i) == grad_out.size(i), "grouped_matmul: input and grad_out must have the same rows");
+  const int64_t K = x.size(-1), N = grad_out.size(-1);
+  const c10::DeviceGuard guard(x.device());
+  auto dw = torch::empty({matrices, transposed ? N : K, transposed ? K : N}, x.options());
+  const ml_grouped_shape s = grouped_shape(x, dw, offsets, transposed, false);
+  TORCH_CHECK(grad_out.scalar_type() == x.scalar_type() && grad_out.device() == x.device(),
+              "grouped_matmul: input and grad_out must have the same dtype and device");
+  const int dt = dtype_code(x, "input");
+  auto ws = grouped_ws(s, dt, ML_GROUPED_BACKWARD_WEIGHT, x);
+  ml_ok(ml_grouped_matmul_backward_weight(&s, dt, x.data_ptr(), grad_out.data_ptr(), transposed, offsets_ptr(offsets),
+                                          dw.data_ptr(), ws.data_ptr(), ws.numel(), cur_stream()));
+  return dw;
+}
+
+struct GroupedNode : public torch::autograd::Function<GroupedNode> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input,
+                               const torch::Tensor& weight, const c10::optional<torch::Tensor>& offsets,
+                               bool transposed) {
+    const auto x = input.contiguous(), w = weight.contiguous();
+    c10::optional<torch::Tensor> o;
+    if (offsets.has_value()) o = offsets->contiguous();
+    auto y = grouped_matmul_forward(x, w, o, transposed);
+    ctx->save_for_backward({x, w, o.has_value() ? *o : torch::Tensor()});
+    ctx->saved_data["transposed"] = transposed;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto sv = ctx->get_saved_variables();
+    c10::optional<torch::Tensor> o;
+    if (sv[2].defined()) o = sv[2];
+    const bool transposed = ctx->saved_data["transposed"].toBool();
+    const auto gy = g[0].detach().contiguous();
+    torch::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = grouped_matmul_backward_input(gy, sv[1], o, transposed);
+    if (ctx->needs_input_grad(1))
+      dw = grouped_matmul_backward_weight(sv[0], gy, o, sv[1].size(0), transposed);
+    return once({dx, dw, torch::Tensor(), torch::Tensor()}, "the backward of grouped_matmul cannot be differentiated");
+  }
+};
+
+torch::Tensor grouped_matmul_autograd(const torch::Tensor& input, const torch::Tensor& weight,
+                                      const c10::optional<torch::Tensor>& offsets, bool transposed) {
+  return GroupedNode::apply(input, weight, offsets, transposed);
+}
+
 // Device flag (int32, shape (1,)): 1 if any element of `x` equals `value`.
 torch::Tensor any_equal(const torch::Tensor& x, int64_t value) {
   ML_CHECK_INPUT(x);
@@ -1066,6 +1203,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_autograd", &layer_norm_autograd,
         "Layer norm as a C++ autograd node, differentiable in input, weight and bias (HIP)", py::arg("input"),
         py::arg("weight"), py::arg("bias"), py::arg("eps"));
+  m.def("grouped_matmul_forward", &grouped_matmul_forward,
+        "Rows in ragged groups times one matrix per group (HIP)", py::arg("input"), py::arg("weight"),
+        py::arg("offsets"), py::arg("transposed") = false);
+  m.def("grouped_matmul_backward_input", &grouped_matmul_backward_input,
+        "Gradient of grouped_matmul_forward with respect to its rows (HIP)", py::arg("grad_out"), py::arg("weight"),
+        py::arg("offsets"), py::arg("transposed") = false);
+  m.def("grouped_matmul_backward_weight", &grouped_matmul_backward_weight,
+        "Gradient of grouped_matmul_forward with respect to its matrices (HIP)", py::arg("input"),
+        py::arg("grad_out"), py::arg("offsets"), py::arg("matrices"), py::arg("transposed") = false);
+  m.def("grouped_matmul_autograd", &grouped_matmul_autograd,
+        "Grouped product as a C++ autograd node, differentiable in input and weight (HIP)", py::arg("input"),
+        py::arg("weight"), py::arg("offsets"), py::arg("transposed") = false);
   m.def("any_equal", &any_equal, "Device flag: any element equal to value (HIP)");
   m.attr("__backend__") = "hip-gfx950";
 }

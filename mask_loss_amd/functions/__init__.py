@@ -19,6 +19,8 @@ from .label.pw_sigmoid_label_loss import PairwiseSigmoidLabelLossFunction
 from .label.pw_softmax_label_loss import PairwiseSoftmaxLabelLossFunction, pairwise_softmax_label_loss
 from .mask.pw_mask import PairwiseMaskLossFunction
 from .mask.matching import MaskMatchingFunction
+from .mask.mask_logits import mask_logits
+from .head.grouped_matmul import GroupedMatmulFunction, grouped_matmul
 from .head.layer_norm import LayerNormFunction, layer_norm
 from .losses import sigmoid_cross_entropy_loss, dice_loss
 
@@ -39,6 +41,9 @@ __all__ = [
     "point_sample",
     "calculate_uncertainty",
     "get_uncertain_point_coords_with_randomness",
+    "mask_logits",
+    "GroupedMatmulFunction",
+    "grouped_matmul",
     "LayerNormFunction",
     "layer_norm",
 ]
