@@ -22,8 +22,8 @@
 // index past its end is zero in both operands (a NaN beyond it never counts).
 //
 // LDS images are XOR-swizzled so that the reads below meet every bank once:
-//   KC      rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 % 8): a read of
-//           16 rows at one chunk covers 256 bytes
+//   KC      rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 % 8); rows of 64
+//           bytes, at c ^ swizzle64(r)
 //   not KC  rows of the tile's width, one per reduced index k.  16-bit: 32-byte unit u
 //           at u ^ (k % 4 + 4 (k / 8 % 2)), read by ds_read_b64_tr_b16, which hands 16
 //           lanes that address 4 k x 16 columns the 4 k of one column each; float:
@@ -39,6 +39,24 @@
 
 namespace ml {
 
+// Division of 0 <= n < 2^31 by a positive int known to the host: (mulhi(n, mul) + n) >> shift with
+// mul = floor(2^32 (2^shift - d) / d) + 1, 2^shift >= d.
+struct FastDiv {
+  uint32_t mul, shift;
+  int d;
+};
+inline FastDiv fast_div(int64_t d) {
+  FastDiv f;
+  f.d = (int)d;
+  f.shift = 0;
+  while (((int64_t)1 << f.shift) < d) ++f.shift;
+  f.mul = (uint32_t)(((((uint64_t)1 << f.shift) - (uint64_t)d) << 32) / (uint64_t)d + 1);
+  return f;
+}
+__device__ __forceinline__ int div_by(int n, const FastDiv& f) {
+  return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift);
+}
+
 struct GroupedArgs {
   const void *a, *b;       // row operand and matrix; weight gradient: operands by columns
   int64_t lda, ldb, ldc;   // row lengths, elements
@@ -50,6 +68,12 @@ struct GroupedArgs {
   int splits;              // parts of the reduction, each with its own float plane
   int64_t plane;           // elements of one plane (splits > 1)
   void* c;                 // output, or the planes
+  int segments;            // row ranges with a matrix: the groups, or (merged) the matrices
+  int merged;              // the rows of the groups that share a matrix make tiles together
+  FastDiv layers;          // groups per matrix
+  FastDiv cols, parts;     // column tiles; splits
+  FastDiv mtiles;          // row tiles of a matrix (weight gradient)
+  int ntiles;              // column tiles
 };
 
 template <int DT>
@@ -65,13 +89,15 @@ struct GMma<ML_BF16> {
 template <>
 struct GMma<ML_F16> {
   typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4_t mma(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const h2 v = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, v);
+    // as the compiler's own conversion (round to nearest even), which it would move away from
+    // the store, one accumulator after another into spilled registers
+    uint32_t v;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(v) : "v"(a), "v"(b));
+    return v;
   }
 };
 template <>
@@ -91,46 +117,67 @@ typedef u32x2_t u32x2_loose __attribute__((aligned(2)));
 typedef f32x4_t f32x4_loose __attribute__((aligned(4)));
 __device__ __forceinline__ u32x4_t load16(const void* p) { return *(const u32x4_loose*)p; }
 
-constexpr int kStepBytes = 128;  // bytes of the reduced index per step
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// A ds_read_b128 passes 16 lanes at a time, lanes 0-3, 12-15 and 20-27 first, then 4-11, 16-19 and
+// 28-31, and so on.  With rows of 64 bytes and chunk l / 16 of row l % 16 wanted by lane l,
+// these values for the rows' fours (0, 2, 3, 1) put the 16 into different banks each time.
+__device__ __forceinline__ int swizzle64(int row) {
+  const int lo = (row >> 2) & 1, hi = (row >> 3) & 1;
+  return ((lo ^ hi) << 1) | hi;
+}
 
 // One operand of a tile: R rows (KC) or columns (not KC) by one step of the reduced
-// index, staged by NT threads.
-template <int DT, bool KC, int R, int NT>
+// index (SB bytes), staged by NT threads.
+template <int DT, bool KC, int R, int NT, int SB = 128>
 struct Operand {
   using E = typename std::conditional<DT == ML_F32, float, uint16_t>::type;
   static constexpr int ES = sizeof(E), CH = 16 / ES;  // elements of a chunk
-  static constexpr int BK = kStepBytes / ES;
+  static constexpr int BK = SB / ES;
   static constexpr int CPR = (KC ? BK : R) / CH;      // chunks of an LDS row
   static constexpr int ROWB = CPR * 16;
   static constexpr int BYTES = R * BK * ES;
   static constexpr int PER = BYTES / 16 / NT;
   static_assert(PER * NT * 16 == BYTES, "whole chunks per thread");
   static_assert(KC || R * ES >= 256, "a row that holds the swizzle");
+  static_assert(SB == 64 || SB == 128, "the swizzles");
+
+  // chunk c of LDS row r lies at chunk swizzled(r, c), and the other way round
+  static __device__ __forceinline__ int swizzled(int r, int c) {
+    if constexpr (KC) return c ^ (SB == 128 ? (r >> 1) & 7 : swizzle64(r));
+    else if constexpr (ES == 2) return c ^ (((r & 3) | ((r >> 1) & 4)) << 1);
+    else return c ^ (((r >> 2) & 3) << 2);
+  }
 
   u32x4_t reg[PER];
+
+  uint32_t off[PER];  // bytes of this thread's chunks from a step's first element
 
   static __device__ __forceinline__ int chunk_row(int i) { return ((int)threadIdx.x + i * NT) / CPR; }
   static __device__ __forceinline__ int chunk_col(int i) { return ((int)threadIdx.x + i * NT) % CPR; }
 
-  // base: the operand's element (first row, first reduced index) of this step; ld: row
-  // length; lim: valid rows (KC) or columns (not KC), at least 1; kleft: valid reduced
-  // indices from here on.  Offsets inside a step stay below 2^32 bytes (host check).
-  __device__ __forceinline__ void load(const E* base, int64_t ld, int lim, int kleft) {
+  // ld: row length; lim: valid rows (KC) or columns (not KC) of the tile, at least 1.  row_at(r): where
+  // row r of the tile lies (KC), in rows from the base.  Offsets stay below 2^32 bytes (host check).
+  template <class F>
+  __device__ __forceinline__ void aim(int64_t ld, int lim, F&& row_at) {
     const uint32_t ldb = (uint32_t)ld * ES;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      // rows past the last read the last one (their outputs are not stored)
+      off[i] = (uint32_t)(KC ? row_at(min(chunk_row(i), lim - 1)) : chunk_row(i)) * ldb + (uint32_t)chunk_col(i) * 16u;
+  }
+  // base: the step's first element; kleft: valid reduced indices from here on
+  __device__ __forceinline__ void load(const E* base, int lim, int kleft) {
     if (kleft >= BK && (KC || lim >= R)) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        // rows past the last read the last one (their outputs are not stored)
-        const uint32_t r = KC ? (uint32_t)min(chunk_row(i), lim - 1) : (uint32_t)chunk_row(i);
-        reg[i] = load16((const char*)base + (r * ldb + (uint32_t)chunk_col(i) * 16u));
-      }
+      for (int i = 0; i < PER; ++i) reg[i] = load16((const char*)base + off[i]);
       return;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int row = chunk_row(i), col = chunk_col(i) * CH;
       const int n = KC ? (row < lim ? kleft - col : 0) : (row < kleft ? lim - col : 0);  // valid elements
-      const E* p = (const E*)((const char*)base + ((uint32_t)row * ldb + (uint32_t)col * ES));
+      const E* p = (const E*)((const char*)base + off[i]);
       u32x4_t v = {0u, 0u, 0u, 0u};
       if (n >= CH) {
         v = load16(p);
@@ -150,22 +197,18 @@ struct Operand {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = chunk_row(i), c = chunk_col(i);
-      int at;
-      if constexpr (KC) at = r * ROWB + ((c ^ ((r >> 1) & 7)) << 4);
-      else if constexpr (ES == 2) at = r * ROWB + ((((c >> 1) ^ ((r & 3) | ((r >> 1) & 4))) << 5) | ((c & 1) << 4));
-      else at = r * ROWB + ((((c >> 2) ^ ((r >> 2) & 3)) << 6) | ((c & 3) << 4));
-      *(u32x4_t*)(lds + at) = reg[i];
+      *(u32x4_t*)(lds + r * ROWB + (swizzled(r, c) << 4)) = reg[i];
     }
   }
 
   // The fragment of rows / columns row0 .. row0 + 15 (a multiple of 16) in sub-step s
-  // (of two) of the step: lane l holds index row0 + l % 16 and 16 bytes of the
+  // (64 bytes) of the step: lane l holds index row0 + l % 16 and 16 bytes of the
   // reduced index, the same ones for both operands.
   static __device__ __forceinline__ u32x4_t frag(const unsigned char* lds, int row0, int s) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     if constexpr (KC) {
-      const int row = row0 + r;
-      return *(const u32x4_t*)(lds + row * ROWB + (((4 * s + g) ^ ((row >> 1) & 7)) << 4));
+      // (row0 does not change the swizzle)
+      return *(const u32x4_t*)(lds + (row0 + r) * ROWB + (swizzled(r, 4 * s + g) << 4));
     } else if constexpr (ES == 2) {
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -206,22 +249,136 @@ __device__ __forceinline__ void group_edges(const GroupedArgs& a, int* e) {
   __syncthreads();
 }
 
-// Rows of segment q: the groups, those that share a matrix next to each other,
-// then the rows before the first group and behind the last (g = -1: zeros).
-__device__ __forceinline__ void segment(const GroupedArgs& a, const int* e, int q, int& g, int& r0, int& r1) {
-  g = -1;
+// Segment q: rows r0 .. r1 that make tiles of their own.  The groups, those that share a matrix
+// (q / layers) next to each other, or (merged) each matrix's rows of all its groups, counted from 0;
+// then the rows before the first group and behind the last (zeros).
+__device__ __forceinline__ void segment(const GroupedArgs& a, const int* e, int q, int& r0, int& r1) {
   r0 = r1 = 0;
-  if (q < a.groups) {
-    const int layers = a.groups / a.matrices;
-    g = (q % layers) * a.matrices + q / layers;
-    r0 = e[g];
-    r1 = e[g + 1];
-  } else if (q == a.groups) {
+  if (q < a.segments) {
+    if (a.merged) {
+      for (int g = q; g < a.groups; g += a.matrices) r1 += e[g + 1] - e[g];
+    } else {
+      const int w = div_by(q, a.layers), g = (q - w * a.layers.d) * a.matrices + w;
+      r0 = e[g];
+      r1 = e[g + 1];
+    }
+  } else if (q == a.segments) {
     r1 = e[0];
-  } else if (q == a.groups + 1) {
+  } else if (q == a.segments + 1) {
     r0 = e[a.groups];
     r1 = a.rows;
   }
+}
+// Row v of matrix w's rows (merged).
+__device__ __forceinline__ int merged_row(const GroupedArgs& a, const int* e, int w, int v) {
+  int g = w;
+  for (; g + a.matrices < a.groups && v >= e[g + 1] - e[g]; g += a.matrices) v -= e[g + 1] - e[g];
+  return e[g] + v;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Tiles of BM rows up to and with each segment, t[0 .. segments + 1]; returns their number.  Every wave
+// writes the same values.
+template <int BM>
+__device__ __forceinline__ int segment_tiles(const GroupedArgs& a, const int* e, int* t) {
+  const int lane = threadIdx.x & 63;
+  int tiles = 0;
+  for (int base = 0; base < a.segments + 2; base += 64) {
+    int r0, r1;
+    segment(a, e, base + lane, r0, r1);
+    int v = (r1 - r0 + BM - 1) / BM;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(v, d, 64);
+      v += lane >= d ? u : 0;
+    }
+    v += tiles;
+    if (base + lane < a.segments + 2) t[base + lane] = v;
+    tiles = __shfl(v, 63, 64);
+  }
+  __syncthreads();
+  return uniform(tiles);
+}
+
+// A work item: a tile of the output and its part of the reduction, `steps` steps of BK from reduced
+// index k on; k runs to kend, then (weight gradient) through the matrix's next groups.
+struct Work {
+  int m0, n0, mlim, w, split, steps;
+  int seg, k, kend;
+  int mapped;  // m0 counts matrix w's rows (merged_row), not the tensor's
+};
+
+// Steps of part `part` begin at this one of n.
+__device__ __forceinline__ int part_start(const GroupedArgs& a, int n, int part) {
+  const int each = div_by(n, a.parts);
+  return each * part + min(part, n - each * a.splits);
+}
+
+constexpr int kBand = 4;
+// Rows kernels, item id of tiles * ntiles * splits.  Bands of kBand row tiles pass over the columns
+// together: their rows and the matrix's columns are both met again while they are in the L2.
+template <int BM, int BN, int BK>
+__device__ __forceinline__ Work rows_work(const GroupedArgs& a, const int* e, const int* t, int tiles, int id) {
+  const int lane = threadIdx.x & 63;
+  Work it;
+  it.seg = 0;
+  const int band = div_by(div_by(id >> 2, a.cols), a.parts);  // kBand = 4
+  const int height = min(kBand, tiles - band * kBand);
+  const int rest = id - band * kBand * a.ntiles * a.splits;
+  const int y = height == 4 ? rest >> 2 : height == 3 ? (int)(__umulhi((uint32_t)rest, 0xAAAAAAABu) >> 1)
+                                                      : rest >> (height - 1);
+  it.split = div_by(y, a.cols);
+  it.n0 = (y - it.split * a.ntiles) * BN;
+  const int tile = band * kBand + rest - y * height;
+  int q = 0;
+  for (int base = 0; base < a.segments + 2; base += 64)
+    q += __popcll(__ballot(base + lane < a.segments + 2 && t[base + lane] <= tile));
+  int r0, r1;
+  segment(a, e, q, r0, r1);
+  it.m0 = uniform(r0 + (tile - (q ? t[q - 1] : 0)) * BM);
+  it.mlim = uniform(r1) - it.m0;
+  const bool zero = q >= a.segments;
+  it.w = zero ? 0 : a.merged ? q : div_by(q, a.layers);
+  it.mapped = a.merged && !zero;
+  const int steps = zero ? 0 : (a.K + BK - 1) / BK;
+  const int s0 = part_start(a, steps, it.split);
+  it.steps = part_start(a, steps, it.split + 1) - s0;
+  it.k = s0 * BK;
+  it.kend = zero ? 0 : a.K;
+  return it;
+}
+
+// Weight gradient, item id of matrices * splits * ntiles * mtiles.
+template <int BM, int BN, int BK>
+__device__ __forceinline__ Work weight_work(const GroupedArgs& a, const int* e, int id) {
+  Work it;
+  it.mapped = 0;
+  const int x = div_by(id, a.mtiles), y = div_by(x, a.cols);
+  it.m0 = (id - x * a.mtiles.d) * BM;
+  it.mlim = a.M - it.m0;
+  it.n0 = (x - y * a.ntiles) * BN;
+  it.w = div_by(y, a.parts);
+  it.split = y - it.w * a.splits;
+  const int* ew = e + it.w;
+  int steps = 0;
+  for (int s = 0; s < a.layers.d; ++s) steps += (ew[s * a.matrices + 1] - ew[s * a.matrices] + BK - 1) / BK;
+  steps = uniform(steps);
+  const int s0 = part_start(a, steps, it.split);
+  it.steps = part_start(a, steps, it.split + 1) - s0;
+  it.k = it.kend = 0;
+  int skip = s0;
+  for (it.seg = 0; it.seg < a.layers.d; ++it.seg) {
+    const int lo = uniform(ew[it.seg * a.matrices]), hi = uniform(ew[it.seg * a.matrices + 1]);
+    const int n = (hi - lo + BK - 1) / BK;
+    if (skip < n) {
+      it.k = lo + skip * BK;
+      it.kend = hi;
+      break;
+    }
+    skip -= n;
+  }
+  return it;
 }
 
 constexpr int kXcds = 8;
@@ -247,108 +404,42 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
   extern __shared__ int e[];  // groups + 1 group edges, then groups + 2 tile counts (rows kernel)
 
   group_edges(a, e);
-  const int ntiles = (a.N + BN - 1) / BN;
   const int lane = threadIdx.x & 63;
-  int m0, n0, split, mlim;   // tile's first output row and column, its rows
-  int w = 0;                 // matrix
-  // reduced range of this workgroup: [k, kend) of segment `seg` of nseg
-  int k = 0, kend = 0, seg = 0, nseg = 1, steps_left;
-  if constexpr (!WG) {
-    // tiles up to and with each segment
-    int* t = e + a.groups + 1;
-    int tiles = 0;
-    for (int base = 0; base < a.groups + 2; base += 64) {
-      int gg, r0, r1;
-      segment(a, e, base + lane, gg, r0, r1);
-      int v = (r1 - r0 + BM - 1) / BM;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d, 64);
-        v += lane >= d ? u : 0;
-      }
-      v += tiles;
-      if (base + lane < a.groups + 2) t[base + lane] = v;
-      tiles = __shfl(v, 63, 64);
-    }
-    const int id = xcd_item(tiles * ntiles * a.splits);
+  Work it;
+  if constexpr (WG) {
+    const int id = xcd_item(a.matrices * a.mtiles.d * a.ntiles * a.splits);
     if (id < 0) return;
-    // bands of kBand row tiles pass over the columns together: their rows and the
-    // matrix's columns are both met again while they are in the L2
-    constexpr int kBand = 4;
-    const int band = id / (kBand * ntiles * a.splits);
-    const int height = min(kBand, tiles - band * kBand);
-    int rest = id - band * kBand * ntiles * a.splits;
-    split = rest / (height * ntiles);
-    rest -= split * height * ntiles;
-    n0 = rest / height * BN;
-    const int tile = band * kBand + rest % height;
-    __syncthreads();
-    int q = 0;
-    for (int base = 0; base < a.groups + 2; base += 64)
-      q += __popcll(__ballot(base + lane < a.groups + 2 && t[base + lane] <= tile));
-    int g, r0, r1;
-    segment(a, e, q, g, r0, r1);
-    m0 = r0 + (tile - (q ? t[q - 1] : 0)) * BM;
-    mlim = r1 - m0;
-    w = g < 0 ? 0 : g % a.matrices;
-    const int steps = g < 0 ? 0 : (a.K + BK - 1) / BK;
-    const int s0 = (int)((int64_t)steps * split / a.splits), s1 = (int)((int64_t)steps * (split + 1) / a.splits);
-    k = s0 * BK;
-    kend = a.K;
-    steps_left = s1 - s0;
+    it = weight_work<BM, BN, BK>(a, e, id);
   } else {
-    const int mtiles = (a.M + BM - 1) / BM;
-    const int id = xcd_item(a.matrices * mtiles * ntiles * a.splits);
+    int* t = e + a.groups + 1;
+    const int tiles = segment_tiles<BM>(a, e, t), id = xcd_item(tiles * a.ntiles * a.splits);
     if (id < 0) return;
-    w = id / (mtiles * ntiles * a.splits);
-    int rest = id - w * mtiles * ntiles * a.splits;
-    split = rest / (mtiles * ntiles);
-    rest -= split * mtiles * ntiles;
-    n0 = rest / mtiles * BN;
-    m0 = rest % mtiles * BM;
-    mlim = a.M - m0;
-    nseg = a.groups / a.matrices;
-    int steps = 0;
-    for (int s = 0; s < nseg; ++s) steps += (e[s * a.matrices + w + 1] - e[s * a.matrices + w] + BK - 1) / BK;
-    const int s0 = (int)((int64_t)steps * split / a.splits), s1 = (int)((int64_t)steps * (split + 1) / a.splits);
-    steps_left = s1 - s0;
-    // the segment that holds step s0
-    int skip = s0;
-    for (; seg < nseg; ++seg) {
-      const int lo = e[seg * a.matrices + w], hi = e[seg * a.matrices + w + 1], n = (hi - lo + BK - 1) / BK;
-      if (skip < n) {
-        k = lo + skip * BK;
-        kend = hi;
-        break;
-      }
-      skip -= n;
-    }
+    it = rows_work<BM, BN, BK>(a, e, t, tiles, id);
   }
-  m0 = __builtin_amdgcn_readfirstlane(m0);
-  n0 = __builtin_amdgcn_readfirstlane(n0);
-  mlim = __builtin_amdgcn_readfirstlane(mlim);
-  w = __builtin_amdgcn_readfirstlane(w);
-  seg = __builtin_amdgcn_readfirstlane(seg);
-  k = __builtin_amdgcn_readfirstlane(k);
-  kend = __builtin_amdgcn_readfirstlane(kend);
-  steps_left = __builtin_amdgcn_readfirstlane(steps_left);
+  const int m0 = uniform(it.m0), n0 = uniform(it.n0), mlim = uniform(it.mlim), w = uniform(it.w);
+  const int steps_left = uniform(it.steps), split = it.split;
+  int k = uniform(it.k), kend = uniform(it.kend), seg = uniform(it.seg);
   const int nlim = a.N - n0;
 
-  const E* pa = (const E*)a.a + (WG ? (int64_t)m0 : (int64_t)m0 * a.lda);
+  const bool mapped = uniform(it.mapped) != 0;
+  auto row_at = [&](int r) { return mapped ? merged_row(a, e, w, m0 + r) : r; };
+  const E* pa = (const E*)a.a + (WG ? (int64_t)m0 : mapped ? (int64_t)0 : (int64_t)m0 * a.lda);
   const E* pb = (const E*)a.b + (WG ? (int64_t)n0 : (int64_t)w * a.bstride + (BKC ? (int64_t)n0 * a.ldb : n0));
   OA oa;
   OB ob;
+  oa.aim(a.lda, mlim, row_at);
+  ob.aim(a.ldb, nlim, [](int r) { return r; });
   auto fetch = [&]() {  // the step at k
-    oa.load(pa + (WG ? (int64_t)k * a.lda : (int64_t)k), a.lda, mlim, kend - k);
-    ob.load(pb + (BKC ? (int64_t)k : (int64_t)k * a.ldb), a.ldb, nlim, kend - k);
+    oa.load(pa + (WG ? (int64_t)k * a.lda : (int64_t)k), mlim, kend - k);
+    ob.load(pb + (BKC ? (int64_t)k : (int64_t)k * a.ldb), nlim, kend - k);
   };
   auto advance = [&]() {
     k += BK;
     if constexpr (WG) {
-      while (k >= kend && seg + 1 < nseg) {
+      while (k >= kend && seg + 1 < a.layers.d) {
         ++seg;
-        k = __builtin_amdgcn_readfirstlane(e[seg * a.matrices + w]);
-        kend = __builtin_amdgcn_readfirstlane(e[seg * a.matrices + w + 1]);
+        k = uniform(e[seg * a.matrices + w]);
+        kend = uniform(e[seg * a.matrices + w + 1]);
       }
     }
   };
@@ -404,7 +495,7 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
   for (int j = 0; j < TM; ++j) {
     const int m = wm + 16 * j + (lane & 15);
     if (m >= mlim) continue;
-    const int64_t row = first + (int64_t)(m0 + m) * a.ldc;
+    const int64_t row = first + (int64_t)(mapped ? row_at(m) : m0 + m) * a.ldc;
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
       const int n = wn + 16 * i + 4 * (lane >> 4);
@@ -432,6 +523,305 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
       }
     }
   }
+}
+
+// ---- aligned operands: stages filled by direct loads into LDS ------------------------
+// Where every row starts on a 16-byte boundary, global_load_lds_dwordx4 moves the operands
+// straight into LDS, without registers.  The LDS images are grouped_kernel's (a load
+// instruction writes 64 consecutive 16-byte slots, so the swizzle is in the lane's source
+// address).  A ring of NS stages of SB bytes of the reduced index is in LDS; the workgroups
+// are persistent: each XCD's take turns over one run of consecutive work items, and the
+// ring runs on from item to item, so the first loads of a tile are in flight while the
+// tile before is finished and stored.
+//
+// A turn of the loop makes the products of one stage, in sub-steps of 64 bytes whose
+// fragments are read from LDS beside the products of the sub-step before (interleave()):
+//
+//   products of sub-step 0     beside reads of sub-step 1 (SB = 128 only)
+//   wait: the next stage has landed, every wave has read all of this one; its slot takes
+//   the loads NS stages on (zeros where none is left)
+//   products of the last one   beside reads of the next stage's sub-step 0
+//
+// The loads are issued by assembly: the compiler, which cannot tell the stages apart, would
+// otherwise wait for all of them before any LDS read.  They have no output registers;
+// ring_wait() waits for the ones that matter and keeps LDS reads on their side of the
+// barrier.
+static __device__ __align__(16) unsigned char g_zeros[16];  // the reduced index past its end
+
+// 16 bytes from base + off, or from p, of each lane to LDS at `lds` + 16 lane.  (m0 is no
+// register of the compiler's: where it needs one it sets it itself.)
+__device__ __forceinline__ void ring_load(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory");
+}
+__device__ __forceinline__ void ring_load(const char* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(p)
+               : "memory");
+}
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  return (const char*)(uintptr_t)((uint64_t)(uint32_t)uniform((int)(uint32_t)u) |
+                                  ((uint64_t)(uint32_t)uniform((int)(uint32_t)(u >> 32)) << 32));
+}
+// Until at most N vector-memory operations are outstanding (they complete in order), and
+// every wave of the workgroup is here with its LDS reads done.
+template <int N>
+__device__ __forceinline__ void ring_wait() {
+  static_assert(N < 64, "vmcnt");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// One operand of a stage, filled by NW waves.
+template <int DT, bool KC, int R, int NW, int SB>
+struct RingOperand : Operand<DT, KC, R, 64 * NW, SB> {
+  using O = Operand<DT, KC, R, 64 * NW, SB>;
+  static constexpr int ES = O::ES, CH = O::CH;
+  static constexpr int PER = O::BYTES / 1024 / NW;        // load instructions of a wave
+  static constexpr int READS = KC ? 1 : ES == 2 ? 2 : 4;  // LDS reads of a fragment
+  static_assert(PER * NW * 1024 == O::BYTES, "whole instructions per wave");
+
+  uint32_t off[PER];  // as Operand's, for the chunks of this lane's loads
+
+  // the chunk of load i: its row in the LDS image, and its column there before the swizzle
+  static __device__ __forceinline__ void chunk(int i, int wave, int& row, int& c) {
+    const int slot = (wave * PER + i) * 64 + (int)(threadIdx.x & 63), s = slot % O::CPR;
+    row = slot / O::CPR;
+    c = O::swizzled(row, s);
+  }
+  // as Operand's; lim is a multiple of CH where it counts columns, and columns past it read the last ones
+  template <class F>
+  __device__ __forceinline__ void aim(int64_t ld, int lim, int wave, F&& row_at) {
+    const uint32_t ldb = (uint32_t)ld * ES;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row, c;
+      chunk(i, wave, row, c);
+      off[i] = KC ? (uint32_t)row_at(min(row, lim - 1)) * ldb + (uint32_t)c * 16u
+                  : (uint32_t)row * ldb + (uint32_t)min(c * CH, lim - CH) * ES;
+    }
+  }
+  // base: the stage's first element; kleft: valid reduced indices from there on
+  __device__ __forceinline__ void load(const char* base, int kleft, uint32_t lds, int wave) const {
+    if (kleft >= O::BK) {
+      const char* b = uniform(base);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) ring_load(b, off[i], lds + (wave * PER + i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int row, c;
+        chunk(i, wave, row, c);
+        ring_load((KC ? c * CH : row) < kleft ? base + off[i] : (const char*)g_zeros, lds + (wave * PER + i) * 1024);
+      }
+    }
+  }
+};
+
+// Order of a sub-step's LDS reads (RB and RA for a fragment of either operand) and products
+// (N times NM for each of M fragments).
+template <int RB, int RA, int N, int M, int NM>
+__device__ __forceinline__ void interleave() {
+  constexpr int kMfma = 0x8, kRead = 0x100;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kRead, RB, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, NM, 0);
+  }
+#pragma unroll
+  for (int j = 1; j < M; ++j) {
+    __builtin_amdgcn_sched_group_barrier(kRead, RA, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, N * NM, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kRead, RA, 0);
+}
+
+// Template arguments and dynamic LDS as grouped_kernel's; OCC workgroups to a compute unit.
+template <int DT, bool WG, bool BKC, int BM, int BN, int WM, int WN, int SB, int NS, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_kernel(GroupedArgs a) {
+  constexpr int NW = WM * WN;
+  using OA = RingOperand<DT, !WG, BM, NW, SB>;
+  using OB = RingOperand<DT, BKC, BN, NW, SB>;
+  constexpr int ES = OA::ES, BK = OA::BK, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr int STAGE = OA::BYTES + OB::BYTES, P = OA::PER + OB::PER;
+  // stores of a full tile: a lane's 16 bytes are 8 columns of two tiles, or 4 floats
+  constexpr int ST = TM * TN / (DT == ML_F32 ? 1 : 2);
+  static_assert(TN % 2 == 0, "tiles in pairs");
+  constexpr int kQueue = 8;  // items between the loads and the products: at most NS + 2, as each has a stage
+  __shared__ __align__(1024) unsigned char lds[NS * STAGE];
+  __shared__ int queue[kQueue][8];
+  extern __shared__ int e[];
+
+  group_edges(a, e);
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  int* t = e + a.groups + 1;
+  int tiles;
+  if constexpr (WG) tiles = a.matrices * a.mtiles.d;
+  else tiles = segment_tiles<BM>(a, e, t);
+  const int items = tiles * a.ntiles * a.splits;
+  const int per = (items + kXcds - 1) / kXcds, xcd = (int)blockIdx.x % kXcds, turns = (int)gridDim.x / kXcds;
+  const int first = xcd * per + (int)blockIdx.x / kXcds, last = min((xcd + 1) * per, items);
+  if (first >= last) return;
+
+  // ---- loads
+  OA oa;
+  OB ob;
+  const uint32_t ring = (uint32_t)(uintptr_t)(lds_void_t*)lds;
+  // the item being loaded (next: the one after it), and the stages left of it
+  int next = first, opened = 0, left = 0, k = 0, kend = 0, seg = 0, w = 0;
+  const char *pa = nullptr, *pb = nullptr;  // the tile's operands at reduced index 0
+  auto open_item = [&]() {
+    if (next >= last) {  // nothing more: zeros
+      left = INT32_MAX;
+      k = kend = 0;
+      seg = a.layers.d;
+      return;
+    }
+    Work it;
+    if constexpr (WG) it = weight_work<BM, BN, BK>(a, e, next);
+    else it = rows_work<BM, BN, BK>(a, e, t, tiles, next);
+    next += turns;
+    it.steps = max(it.steps, 1);  // nothing to reduce: one stage of zeros
+    if (lane == 0) {
+      int* q = queue[opened % kQueue];
+      q[0] = it.m0;
+      q[1] = it.n0;
+      q[2] = it.mlim;
+      q[3] = it.w;
+      q[4] = it.split;
+      q[5] = it.steps;
+      q[6] = it.mapped;
+    }
+    ++opened;
+    left = uniform(it.steps);
+    k = uniform(it.k);
+    kend = uniform(it.kend);
+    seg = uniform(it.seg);
+    w = uniform(it.w);
+    const int m0 = uniform(it.m0), n0 = uniform(it.n0);
+    const bool mapped = uniform(it.mapped) != 0;
+    pa = (const char*)a.a + (WG ? (int64_t)m0 : mapped ? (int64_t)0 : (int64_t)m0 * a.lda) * ES;
+    pb = (const char*)a.b + (WG ? (int64_t)n0 : (int64_t)w * a.bstride + (BKC ? (int64_t)n0 * a.ldb : (int64_t)n0)) * ES;
+    if (mapped) oa.aim(a.lda, uniform(it.mlim), wave, [&](int r) { return merged_row(a, e, w, m0 + r); });
+    else oa.aim(a.lda, uniform(it.mlim), wave, [](int r) { return r; });
+    ob.aim(a.ldb, a.N - n0, wave, [](int r) { return r; });
+  };
+  auto load = [&](uint32_t at) {  // the next stage's loads, into the slot at this LDS offset
+    if (left == 0) open_item();
+    --left;
+    if constexpr (WG) {
+      while (k >= kend && seg + 1 < a.layers.d) {
+        ++seg;
+        k = uniform(e[seg * a.matrices + w]);
+        kend = uniform(e[seg * a.matrices + w + 1]);
+      }
+    }
+    oa.load(pa + (WG ? k * a.lda : (int64_t)k) * ES, kend - k, ring + at, wave);
+    ob.load(pb + (BKC ? (int64_t)k : k * a.ldb) * ES, kend - k, ring + at + OA::BYTES, wave);
+    k += BK;
+  };
+#pragma unroll 1
+  for (int s = 0; s < NS; ++s) load(s * STAGE);
+
+  // ---- products
+  const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+  u32x4_t fa[TM], fb[TN], fn[TN];
+  ring_wait<(NS - 1) * P>();
+#pragma unroll
+  for (int i = 0; i < TN; ++i) fb[i] = OB::frag(lds + OA::BYTES, wn + 16 * i, 0);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fa[i] = OA::frag(lds, wm + 16 * i, 0);
+  uint32_t cur = 0;  // LDS offset of the stage in turn
+  int credit = 0;    // stages whose loads were issued before the last tile's stores
+  const int count = (last - first + turns - 1) / turns;
+  for (int n = 0; n < count; ++n) {
+    const int* q = queue[n % kQueue];
+    const int steps = uniform(q[5]);
+    f32x4_t acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // products of the fragments in b and fa, and reads of those of sub-step h of the stage at
+    // `from` into bn and, as they fall free, fa
+    auto sub_step = [&](const u32x4_t(&b)[TN], u32x4_t(&bn)[TN], const unsigned char* from, int h) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i) bn[i] = OB::frag(from + OA::BYTES, wn + 16 * i, h);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) acc[i][j] = GMma<DT>::mma(b[i], fa[j], acc[i][j]);
+        fa[j] = OA::frag(from, wm + 16 * j, h);
+      }
+      // in this order: the scheduler would put the reads behind the products
+      interleave<OB::READS, OA::READS, TN, TM, DT == ML_F32 ? 4 : 1>();
+    };
+    for (int s = 0; s < steps; ++s) {
+      if constexpr (SB == 128) sub_step(fb, fn, lds + cur, 1);
+      // issued after the next stage's loads: those of NS - 2 more and, where they came between, a
+      // full tile's stores
+      constexpr int kLoads = (NS - 2) * P;
+      if (credit > 0) {
+        --credit;
+        ring_wait<(kLoads + ST < 63 ? kLoads + ST : 63)>();
+      } else {
+        ring_wait<kLoads>();
+      }
+      load(cur);
+      cur = cur == (NS - 1) * STAGE ? 0 : cur + STAGE;
+      if constexpr (SB == 128) {
+        sub_step(fn, fb, lds + cur, 0);
+      } else {
+        sub_step(fb, fn, lds + cur, 0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) fb[i] = fn[i];
+      }
+    }
+
+    // lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile; columns come in
+    // whole chunks
+    const int m0 = uniform(q[0]), n0 = uniform(q[1]), tm = uniform(q[2]), iw = uniform(q[3]), split = uniform(q[4]);
+    const bool mapped = uniform(q[6]) != 0;
+    const int tn = a.N - n0;
+    const bool planes = a.splits > 1, full = tm >= BM && tn >= BN && !planes;
+    const int64_t origin = (planes ? (int64_t)split * a.plane : 0) + (WG ? (int64_t)iw * a.cstride : 0) + n0;
+    const int mr = wm + (lane & 15), g = lane >> 4;
+    auto row_start = [&](int j) {  // of the lane's row in row tile j
+      const int r = mr + 16 * j;
+      return origin + (int64_t)(mapped ? merged_row(a, e, iw, m0 + min(r, tm - 1)) : m0 + r) * a.ldc;
+    };
+    if (planes || DT == ML_F32) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        float* c = (float*)a.c + row_start(j) + wn + 4 * g;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+          if (full || (mr + 16 * j < tm && wn + 16 * i + 4 * g < tn)) *(f32x4_loose*)(c + 16 * i) = acc[i][j];
+      }
+    } else if constexpr (DT != ML_F32) {
+      // two tiles' columns change places between lane groups 0 and 1, 2 and 3, so that a lane
+      // has eight consecutive ones: of the first tile in even groups, of the second in odd ones
+      const int col = wn + 16 * (g & 1) + 8 * (g >> 1);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        uint16_t* c = (uint16_t*)a.c + row_start(j) + col;
+#pragma unroll
+        for (int i = 0; i < TN; i += 2) {
+          const f32x4_t u = acc[i][j], v = acc[i + 1][j];
+          const auto x = __builtin_amdgcn_permlane16_swap(GMma<DT>::pack(u[0], u[1]), GMma<DT>::pack(v[0], v[1]), false, false);
+          const auto y = __builtin_amdgcn_permlane16_swap(GMma<DT>::pack(u[2], u[3]), GMma<DT>::pack(v[2], v[3]), false, false);
+          if (full || (mr + 16 * j < tm && col + 16 * i < tn))
+            *(u32x4_loose*)(c + 16 * i) = u32x4_t{x[0], y[0], x[1], y[1]};
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one row tile's conversions at a time: registers
+      }
+    }
+    credit = full ? NS - 1 : 0;
+  }
+  ring_wait<0>();  // the last loads, of zeros, end before the LDS goes to another workgroup
 }
 
 }  // namespace ml

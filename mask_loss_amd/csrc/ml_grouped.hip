@@ -1,6 +1,20 @@
-// Grouped products: plans, launches and C entry points (the kernel: ml_grouped.h).
+// Grouped products: plans, launches and C entry points (the kernels: ml_grouped.h).
 //
-// Three tile shapes... see grouped_plan.
+// Tiles, and what the listed products of perf/operators.py take with each (us; KC: the operand's
+// reduced index is contiguous):
+//
+//                                      KC x KC          KC x rows        rows x rows
+//                                      experts  masks   experts  masks   experts  masks
+//                                      forward  d in    d in     forward d weight d weight
+//   128 x 128, 2 stages of 128 bytes   163      216     191      289     266      287
+//   128 x 256, 3 stages of 64 bytes    182      248     182      278     211      238
+//   256 x 256, 4 stages of 64 bytes    180      233     217      254     190      216
+//   grouped_kernel, 128 x 128          229      229     258      402     315      380
+//
+// (experts: 16,384 rows in 16 groups, K = 1,024, N = 4,096; masks: 16 groups of 200 rows, K = 256,
+// N = 65,536; bf16.)  Where both operands' reduced index is contiguous, 128-byte stages read whole
+// HBM lines and win; operands by rows are whole lines anyway, and the larger tiles read LDS less
+// often.  The choice also weighs how the tiles fill the compute units (grouped_plan).
 #include <algorithm>
 
 #include "ml_grouped.h"
@@ -26,19 +40,29 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const float* planes, 
   }
 }
 
+// Tiles: a workgroup's part of the output, and workgroups to a compute unit.
+enum Tile { kFew, kPlain, kDeep128, kWide128, kDeep128x256, kDeep256 };
+struct TileShape {
+  int bm, bn, occ;
+};
+constexpr TileShape kTiles[] = {{32, 128, 4}, {128, 128, 2}, {128, 128, 2}, {128, 128, 2}, {128, 256, 2}, {256, 256, 1}};
+
 struct GroupedPlan {
-  int tile;                 // 0: 32 x 128, 1: 128 x 128
+  Tile tile;
   int splits;
+  bool merged;
   int64_t m, n, k;          // output rows and columns, reduced length (weight gradient: mean rows per matrix)
-  int64_t bound;            // workgroups
+  int64_t bound;            // work items at most
   int64_t plane;            // elements of a plane
   size_t bytes;             // workspace
 };
 
 constexpr int64_t kMaxGroups = 4000;   // their edges and tile counts fit the LDS beside the tiles
 constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 bytes of its first
+constexpr int64_t kUnits = 256;
 
-int grouped_plan(const ml_grouped_shape* s, int dtype, int which, GroupedPlan& p) {
+// aligned: every row of the operands and of the result starts on a 16-byte boundary; transposed: as the call's
+int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transposed, bool aligned, GroupedPlan& p) {
   if (!s || s->rows < 0 || s->K < 0 || s->N < 0 || s->groups < 1 || s->matrices < 1 || s->groups % s->matrices)
     return fail(ML_EINVAL, "grouped_matmul: invalid shape (groups must be a positive multiple of the matrices)");
   if (dtype != ML_F32 && dtype != ML_BF16 && dtype != ML_F16)
@@ -47,39 +71,102 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, GroupedPlan& p
     return fail(ML_EUNSUPPORTED, "grouped_matmul: at most " + std::to_string(kMaxGroups) + " groups are supported");
   if (s->rows > INT32_MAX || s->K > kMaxLength || s->N > kMaxLength)
     return fail(ML_EUNSUPPORTED, "grouped_matmul: at most 2^31 - 1 rows and K, N of at most 4194304 are supported");
-  const int64_t bk = kStepBytes / (dtype == ML_F32 ? 4 : 2);
-  p.m = which == kWeight ? s->K : s->rows;
-  p.n = which == kInput ? s->K : s->N;
+  const int64_t es = dtype == ML_F32 ? 4 : 2, bk = 128 / es, layers = s->groups / s->matrices;
+  const bool wg = which == kWeight;
+  p.m = wg ? (transposed ? s->N : s->K) : s->rows;
+  p.n = wg ? (transposed ? s->K : s->N) : which == kInput ? s->K : s->N;
   p.k = which == kForward ? s->K : which == kInput ? s->N : ceil_div(s->rows, s->matrices);
-  const int64_t used = std::min(s->groups, std::max<int64_t>(s->rows, 1));  // groups that can hold rows
-  const int64_t each = ceil_div(s->rows, used);
-  p.tile = which == kWeight || each > 32;
-  const int64_t bm = p.tile ? 128 : 32, bn = 128, nt = ceil_div(p.n, bn);
-  const int64_t likely = (which == kWeight ? s->matrices * ceil_div(p.m, bm) : used * ceil_div(each, bm)) * nt;
-  // split the reduction where the tiles leave compute units without work: towards
-  // two workgroups each, at least four steps to a part
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(likely, 1), p.k / (4 * bk), 64}));
-  const int64_t mt = which == kWeight ? s->matrices * ceil_div(p.m, bm)
-                                      : s->rows / bm + std::min(s->groups + 2, s->rows);
-  p.bound = ceil_div(mt * nt * p.splits, kXcds) * kXcds;
-  if (p.bound > INT32_MAX) return fail(ML_EUNSUPPORTED, "grouped_matmul: too many tiles");
-  const int64_t out = (which == kWeight ? s->matrices : 1) * p.m * p.n;
+  // groups that share a matrix make tiles together, as far as their rows' offsets go
+  p.merged = !wg && layers > 1 && s->rows * p.k * es < ((int64_t)1 << 32);
+  const int64_t segments = p.merged ? s->matrices : s->groups;
+  const int64_t used = std::min(segments, std::max<int64_t>(s->rows, 1));  // those that can hold rows
+  const double each = (double)s->rows / used;
+  const int64_t out = (wg ? s->matrices : 1) * p.m * p.n;
+
+  const int64_t steps = std::max<int64_t>(1, ceil_div(p.k, bk));
+  // Rough time of a tile shape, in steps of 128 x 128 outputs on one compute unit.
+  auto plan = [&](Tile t, double factor, int& splits) {
+    const TileShape& T = kTiles[t];
+    const double mt = wg ? (double)s->matrices * ceil_div(p.m, T.bm)
+                         : used * (each / T.bm <= 1.0 ? 1.0 : each / T.bm + 0.5);
+    const double tiles = mt * ceil_div(p.n, T.bn), slots = (double)kUnits * T.occ;
+    // split the reduction where the tiles leave slots without work, at least four steps to a part
+    splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)(slots / tiles), steps / 4, 64}));
+    const double rounds = tiles * splits / slots;
+    const double area = T.bm * T.bn / 16384.0 * T.occ;
+    double c = (rounds < 4.0 ? std::max(1.0, std::ceil(rounds - 0.05)) : rounds + 0.5) * area * factor *
+               ((double)steps / splits + 4.0);
+    if (splits > 1) c += (double)splits * out * 8.0 * 2e-6;  // planes written and read again: 0.5 us to a step
+    return c;
+  };
+  if (!wg && each <= 32.0) {
+    p.tile = kFew;
+    plan(p.tile, 1.0, p.splits);
+  } else if (!aligned) {
+    p.tile = kPlain;
+    plan(p.tile, 1.0, p.splits);
+  } else if (dtype == ML_F32) {
+    p.tile = wg ? kDeep128 : kWide128;
+    plan(p.tile, 1.0, p.splits);
+  } else {
+    const int rowops = wg ? 2 : (which == kForward) == transposed ? 0 : 1;  // operands by rows of the reduced index
+    // by the table above, per tile area
+    constexpr double f[3][3] = {{1.0, 1.05, 1.1}, {1.1, 1.0, 0.95}, {1.3, 1.0, 0.92}};
+    const Tile ts[3] = {kWide128, kDeep128x256, kDeep256};
+    double best = 0.0;
+    int n1 = 1;
+    for (int i = 0; i < 3; ++i) {
+      const double c = plan(ts[i], f[rowops][i], n1);
+      if (i && c >= best) continue;
+      best = c;
+      p.tile = ts[i];
+      p.splits = n1;
+    }
+  }
+  const TileShape& T = kTiles[p.tile];
+  const int64_t mt = wg ? s->matrices * ceil_div(p.m, T.bm) : s->rows / T.bm + std::min(segments + 2, s->rows);
+  p.bound = mt * ceil_div(p.n, T.bn) * p.splits;
+  if (p.bound > INT32_MAX - 8) return fail(ML_EUNSUPPORTED, "grouped_matmul: too many tiles");
   p.plane = ceil_div(out, 4) * 4;
   p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
   return ML_OK;
 }
 
 template <int DT, bool WG, bool BKC>
-int grouped_launch(const GroupedPlan& p, const GroupedArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)p.bound);
+int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
+  const TileShape& T = kTiles[p.tile];
+  a.ntiles = (int)ceil_div(a.N, T.bn);
+  a.cols = fast_div(a.ntiles);
+  a.parts = fast_div(a.splits);
+  a.layers = fast_div(a.groups / a.matrices);
+  a.mtiles = fast_div(WG ? ceil_div(a.M, T.bm) : 1);
   const size_t lds = (2 * (size_t)a.groups + 3) * sizeof(int);
-  if constexpr (!WG) {
-    if (p.tile == 0) {
-      hipLaunchKernelGGL((grouped_kernel<DT, false, BKC, 32, 128, 1, 4>), grid, dim3(256), lds, st, a);
-      return check_launch("grouped_matmul");
-    }
+  // one workgroup to an item (rounded up for xcd_item), or persistent ones
+  const bool ring = p.tile >= kDeep128;
+  const dim3 grid((unsigned)(ring ? std::min<int64_t>(kUnits * T.occ, ceil_div(p.bound, kXcds) * kXcds)
+                                  : ceil_div(p.bound, kXcds) * kXcds)), blk(256);
+  switch (p.tile) {
+    case kFew:
+      if constexpr (!WG) hipLaunchKernelGGL((grouped_kernel<DT, false, BKC, 32, 128, 1, 4>), grid, blk, lds, st, a);
+      break;
+    case kPlain: hipLaunchKernelGGL((grouped_kernel<DT, WG, BKC, 128, 128, 2, 2>), grid, blk, lds, st, a); break;
+    case kDeep128:
+      if constexpr (DT == ML_F32 && WG)
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, 64, 4, 2>), grid, blk, lds, st, a);
+      break;
+    case kWide128:
+      if constexpr (DT != ML_F32 || !WG)
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, 128, 2, 2>), grid, blk, lds, st, a);
+      break;
+    case kDeep128x256:
+      if constexpr (DT != ML_F32)
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 256, 2, 2, 64, 3, 2>), grid, blk, lds, st, a);
+      break;
+    case kDeep256:
+      if constexpr (DT != ML_F32)
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 2, 64, 4, 1>), grid, blk, lds, st, a);
+      break;
   }
-  hipLaunchKernelGGL((grouped_kernel<DT, WG, BKC, 128, 128, 2, 2>), grid, dim3(256), lds, st, a);
   return check_launch("grouped_matmul");
 }
 
@@ -92,6 +179,8 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   a.rows = (int)s->rows;
   a.groups = (int)s->groups;
   a.matrices = (int)s->matrices;
+  a.segments = p.merged ? a.matrices : a.groups;
+  a.merged = p.merged;
   a.splits = p.splits;
   a.plane = p.plane;
   a.c = p.splits > 1 ? ws : out;
@@ -127,10 +216,17 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   return check_launch("grouped_matmul");
 }
 
+// rows of whole 16-byte chunks
+bool grouped_whole(const ml_grouped_shape* s, int dtype) {
+  const int64_t ch = dtype == ML_F32 ? 4 : 8;
+  return s && s->K % ch == 0 && s->N % ch == 0;
+}
+
 int grouped_call(const ml_grouped_shape* s, int dtype, int which, const void* rows, const void* other, int transposed,
                  const int64_t* offsets, void* out, void* ws, size_t ws_bytes, ml_stream_t stream) {
   GroupedPlan p;
-  const int rc = grouped_plan(s, dtype, which, p);
+  const bool aligned = grouped_whole(s, dtype) && ((uintptr_t)rows & 15) == 0 && ((uintptr_t)other & 15) == 0;
+  const int rc = grouped_plan(s, dtype, which, transposed != 0, aligned, p);
   if (rc) return rc;
   if (p.m == 0 || p.n == 0) return ML_OK;
   const bool reads = s->rows > 0 && p.k > 0;
@@ -152,10 +248,14 @@ int grouped_call(const ml_grouped_shape* s, int dtype, int which, const void* ro
 using namespace ml;
 
 extern "C" size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, int dtype, int product) {
-  GroupedPlan p;
-  if (product < ML_GROUPED_FORWARD || product > ML_GROUPED_BACKWARD_WEIGHT || grouped_plan(s, dtype, product, p))
-    return 0;
-  return p.bytes;
+  if (product < ML_GROUPED_FORWARD || product > ML_GROUPED_BACKWARD_WEIGHT) return 0;
+  size_t most = 0;  // over both storage orders, and tensors that start on 16-byte boundaries or not
+  for (int i = 0; i < 4; ++i) {
+    GroupedPlan p;
+    if (grouped_plan(s, dtype, product, (i & 1) != 0, (i & 2) && grouped_whole(s, dtype), p)) return 0;
+    most = std::max(most, p.bytes);
+  }
+  return most;
 }
 
 extern "C" int ml_grouped_matmul_forward(const ml_grouped_shape* s, int dtype, const void* x, const void* weight,
