@@ -61,7 +61,8 @@ struct GroupedArgs {
   const void *a, *b;       // row operand and matrix; weight gradient: operands by columns
   int64_t lda, ldb, ldc;   // row lengths, elements
   int64_t bstride, cstride;  // elements per matrix: of b (rows kernel), of c (weight gradient)
-  const int64_t* offsets;  // null: equal groups
+  const int64_t* offsets;  // null: groups of `equal` rows
+  int equal;
   int rows, groups, matrices;
   int K;                   // reduced length (rows kernel)
   int M, N;                // output rows (weight gradient) and columns
@@ -227,6 +228,29 @@ struct Operand {
   }
 };
 
+// Inclusive scans over the wave of values that are not negative, in the vector ALU: shifts by 1, 2, 4
+// and 8 within 16 lanes, then the last lane of a row (of two rows) to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int scan_max(int v) {
+  v = max(v, dpp_or_zero<0x111, 0xf>(v));
+  v = max(v, dpp_or_zero<0x112, 0xf>(v));
+  v = max(v, dpp_or_zero<0x114, 0xf>(v));
+  v = max(v, dpp_or_zero<0x118, 0xf>(v));
+  v = max(v, dpp_or_zero<0x142, 0xa>(v));
+  return max(v, dpp_or_zero<0x143, 0xc>(v));
+}
+__device__ __forceinline__ int scan_sum(int v) {
+  v += dpp_or_zero<0x111, 0xf>(v);
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);
+  return v + dpp_or_zero<0x143, 0xc>(v);
+}
+
 // Group edges e[0 .. groups] from the offsets, each held to 0 .. rows and to at least
 // the one before, so that any offsets give disjoint groups inside the tensors.  Every
 // wave writes the same values.
@@ -237,14 +261,12 @@ __device__ __forceinline__ void group_edges(const GroupedArgs& a, int* e) {
     const int i = base + lane;
     int v = 0;
     if (i <= a.groups) {
-      const int64_t o = a.offsets ? a.offsets[i] : (int64_t)i * (a.rows / a.groups);
+      const int64_t o = a.offsets ? a.offsets[i] : (int64_t)i * a.equal;
       v = o < 0 ? 0 : o > a.rows ? a.rows : (int)o;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_up(v, d, 64));
-    v = max(v, before);
+    v = max(scan_max(v), before);
     if (i <= a.groups) e[i] = v;
-    before = __shfl(v, 63, 64);
+    before = __builtin_amdgcn_readlane(v, 63);
   }
   __syncthreads();
 }
@@ -288,17 +310,12 @@ __device__ __forceinline__ int segment_tiles(const GroupedArgs& a, const int* e,
     int r0, r1;
     segment(a, e, base + lane, r0, r1);
     int v = (r1 - r0 + BM - 1) / BM;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(v, d, 64);
-      v += lane >= d ? u : 0;
-    }
-    v += tiles;
+    v = scan_sum(v) + tiles;
     if (base + lane < a.segments + 2) t[base + lane] = v;
-    tiles = __shfl(v, 63, 64);
+    tiles = __builtin_amdgcn_readlane(v, 63);
   }
   __syncthreads();
-  return uniform(tiles);
+  return tiles;
 }
 
 // A work item: a tile of the output and its part of the reduction, `steps` steps of BK from reduced

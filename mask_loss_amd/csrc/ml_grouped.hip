@@ -24,14 +24,34 @@ namespace {
 
 enum { kForward = 0, kInput = 1, kWeight = 2 };  // the three products
 
-// Sums of the planes of a split reduction, in plane order, four elements a thread.
+// Sums of the planes of a split reduction: four elements a thread, four slices of the planes to a
+// workgroup, each with up to eight loads in flight, in an order that the shape alone fixes.
+constexpr int kJoinQuads = 64, kJoinSlices = 4;
 template <int DT>
-__global__ __launch_bounds__(256) void grouped_join_kernel(const float* planes, int splits, int64_t plane, int64_t n,
-                                                          void* c) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4_t v = *(const f32x4_t*)(planes + i);
-  for (int s = 1; s < splits; ++s) v += *(const f32x4_t*)(planes + s * plane + i);
+__global__ __launch_bounds__(kJoinQuads* kJoinSlices) void grouped_join_kernel(const float* planes, int splits,
+                                                                              int64_t plane, int64_t n, void* c) {
+  __shared__ f32x4_t part[kJoinSlices][kJoinQuads];
+  const int ql = threadIdx.x % kJoinQuads, sl = threadIdx.x / kJoinQuads;
+  const int64_t i = ((int64_t)blockIdx.x * kJoinQuads + ql) * 4;
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (i < n) {
+    constexpr int kFlight = 8;
+    for (int s = sl; s < splits; s += kJoinSlices * kFlight) {
+      f32x4_t u[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int r = s + j * kJoinSlices;
+        u[j] = r < splits ? *(const f32x4_t*)(planes + r * plane + i) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) v += u[j];
+    }
+  }
+  part[sl][ql] = v;
+  __syncthreads();
+  if (sl || i >= n) return;
+#pragma unroll
+  for (int s = 1; s < kJoinSlices; ++s) v += part[s][ql];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (i + q >= n) break;
@@ -176,6 +196,7 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   ProfScope ps("grouped_matmul", st);
   GroupedArgs a{};
   a.offsets = offsets;
+  a.equal = (int)(s->rows / s->groups);
   a.rows = (int)s->rows;
   a.groups = (int)s->groups;
   a.matrices = (int)s->matrices;
@@ -211,7 +232,8 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   }
   if (rc || p.splits == 1) return rc;
   const int64_t n = (which == kWeight ? s->matrices : 1) * p.m * p.n;
-  hipLaunchKernelGGL(grouped_join_kernel<DT>, dim3((unsigned)ceil_div(n, 1024)), dim3(256), 0, st, (const float*)ws,
+  hipLaunchKernelGGL(grouped_join_kernel<DT>, dim3((unsigned)ceil_div(n, kJoinQuads * 4)),
+                     dim3(kJoinQuads * kJoinSlices), 0, st, (const float*)ws,
                      p.splits, p.plane, n, out);
   return check_launch("grouped_matmul");
 }

@@ -4,7 +4,8 @@
 //   g = dy w:  dx = r (g - mean g - h mean(g h)),  dw = sum_rows dy h,  db = sum_rows dy
 //
 // Both directions are bound by HBM: the forward reads x and writes y once, the
-// backward reads x and dy and writes dx once.  A row is therefore held in
+// backward reads x and dy and writes dx once (172,032 x 256 f16: forward 32 us, 5.5
+// TB/s; backward 46 + 5 us, 5.2 TB/s; a copy of 1 GiB runs at 5.2).  A row is therefore held in
 // registers between its reductions, T threads to a row and up to kEpt elements
 // to a thread, so that the variance is summed about the mean (no cancellation)
 // without a second read.  Statistics, sums and the weights' gradients are
@@ -66,14 +67,37 @@ struct alignas(V == 1 ? sizeof(typename Elem<DT>::raw) : 16) Vec {
   typename Elem<DT>::raw e[V];
 };
 
+// v plus the value of another lane, in the vector ALU: quad neighbours (xor 1, xor 2), the mirrored
+// lane of 8 and of 16 (whose fours and eights hold one value by then), the other 16 and the
+// other 32.  About 10 cycles a step where a shuffle through LDS takes 60.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int T>
+__device__ __forceinline__ float lane_sum(float v) {
+  static_assert(T == 16 || T == 32 || T == 64, "lanes");
+  v = add_dpp<0xB1>(v);   // quad_perm 1 0 3 2
+  v = add_dpp<0x4E>(v);   // quad_perm 2 3 0 1
+  v = add_dpp<0x141>(v);  // row_half_mirror
+  v = add_dpp<0x140>(v);  // row_mirror
+  if constexpr (T >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (T >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
 // Sums of N values over the T threads of a row, the same in all of them; `s` is
 // one of two alternating LDS buffers, so one barrier a sum is enough.
 template <int T, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float* s) {
 #pragma unroll
-  for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  for (int i = 0; i < N; ++i) v[i] = lane_sum<(T < 64 ? T : 64)>(v[i]);
   if constexpr (T > 64) {
     constexpr int W = T / 64;
     const int wave = threadIdx.x >> 6;
@@ -306,8 +330,20 @@ __global__ __launch_bounds__(kParamCols* kParamSlices) void norm_param_kernel(co
   const int64_t c = (int64_t)blockIdx.x * kParamCols + cl;
   const float* p = part + (int64_t)blockIdx.y * n * D;
   float a = 0.f;
-  if (c < D)
-    for (int64_t i = sl; i < n; i += kParamSlices) a += p[i * D + c];
+  if (c < D) {
+    // eight loads in flight: a slice is bound by their latency
+    constexpr int kFlight = 8;
+    for (int64_t i = sl; i < n; i += kParamSlices * kFlight) {
+      float v[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int64_t r = i + j * kParamSlices;
+        v[j] = r < n ? p[r * D + c] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) a += v[j];
+    }
+  }
   s[sl][cl] = a;
   __syncthreads();
   if (sl == 0 && c < D) {
@@ -438,13 +474,19 @@ int norm_cfg(int64_t D) {
   return i;
 }
 
-// Workgroups of the backward: each writes a row of partial sums, which
-// norm_param_kernel reads again.
+// Workgroups: a few to a compute unit that walk the rows, so that the weights are loaded once and
+// the next row's loads run beside this one's sums.  Forward, 512 / 1,024 / 2,048 / 4,096 workgroups:
+// 32,000 x 256 bf16 10.4 / 11.2 / 14.3 / 19.6 us, 172,032 x 256 f16 33.4 / 32.3 / 35.5 / 38.4,
+// 2,048 x 1,153 f32 8.0 / 6.9 / 7.0 / 7.1, 16,384 x 4,096 bf16 52.8 / 55.8 / 55.6 / 75.1.
+int64_t norm_fwd_blocks(int T, int E) { return T > kNormThreads || (T == kNormThreads && E > 8) ? 512 : 1024; }
+// Backward, where each workgroup also writes a row of partial sums that norm_param_kernel reads
+// again, 512 / 768 / 1,024: the same cases 14.3 / 13.7 / 14.0 us, 52.7 / 46.4 / 47.0, 9.9 / 10.5 /
+// 10.5, 85 / 93 / 100 (and the sums 3.9 / 3.8 / 3.9, 4.6 / 4.6 / 4.6, 3.9 / 4.6 / 5.2, 4.9 / 5.7 / 6.9).
 int64_t norm_bwd_blocks(int64_t rows, int64_t D) {
   if (D > kNormHeld) return std::min<int64_t>(rows, 64);
   const int T = kNormCfgs[norm_cfg(D)].T;
   const int64_t rounds = ceil_div(rows, wg_threads(T) / T);
-  return std::min<int64_t>(rounds, T > kNormThreads ? 256 : 512);
+  return std::min<int64_t>(rounds, T > kNormThreads ? 256 : T < kNormThreads ? 768 : 512);
 }
 
 template <class F>
@@ -482,7 +524,7 @@ int norm_forward(const void* x, const void* w, const void* b, int pf32, int64_t 
   return norm_dispatch(norm_cfg(D), [&](auto tc, auto ec) {
     constexpr int T = decltype(tc)::value, E = decltype(ec)::value;
     const int64_t rounds = ceil_div(rows, wg_threads(T) / T);
-    const dim3 grid((unsigned)std::min<int64_t>(rounds, T > kNormThreads ? 512 : 2048)), blk(wg_threads(T));
+    const dim3 grid((unsigned)std::min<int64_t>(rounds, norm_fwd_blocks(T, E))), blk(wg_threads(T));
     if (vec)
       hipLaunchKernelGGL((norm_fwd_kernel<DT, V16, E / V16, T>), grid, blk, 0, st, x, w, b, pf32, rows, D, eps, y,
                          mean, rstd);
