@@ -1084,36 +1084,95 @@ torch::Tensor grouped_matmul_backward_weight(const torch::Tensor& x, const torch
   return dw;
 }
 
+// Mask logits as grouped products: queries (L, B, Q, C) as L * B equal groups, or (R, C) with
+// offsets (B + 1,), times features (B, C, H, W) as B matrices (C, H * W).
+// Shape of the logits.
+std::vector<int64_t> mask_shape(const torch::Tensor& queries, const torch::Tensor& features,
+                     const c10::optional<torch::Tensor>& offsets) {
+  TORCH_CHECK_VALUE(features.dim() == 4, "features must be (B, C, H, W), got ", features.sizes());
+  const int64_t B = features.size(0), C = features.size(1);
+  if (offsets.has_value()) {
+    TORCH_CHECK_VALUE(queries.dim() == 2 && queries.size(1) == C, "queries must be (R, C) with offsets, for features ",
+                      features.sizes(), ", got ", queries.sizes());
+    TORCH_CHECK_VALUE(offsets->dim() == 1 && offsets->size(0) == B + 1, "offsets must have shape (B + 1,) = (", B + 1,
+                      ",), got ", offsets->sizes());
+    return {queries.size(0), features.size(2), features.size(3)};
+  }
+  TORCH_CHECK_VALUE(queries.dim() == 4 && queries.size(3) == C, "queries must be (L, B, Q, C) for features ",
+                    features.sizes(), ", got ", queries.sizes());
+  TORCH_CHECK_VALUE(queries.size(1) == B, "queries and features must have the same batch size, got ", queries.size(1),
+                    " and ", B);
+  return {queries.size(0), B, queries.size(2), features.size(2), features.size(3)};
+}
+// (L, B, n, width) -> (L * B, n, width); rows stay as they are
+torch::Tensor as_groups(const torch::Tensor& x, int64_t width, bool ragged) {
+  return ragged ? x.view({x.size(0), width}) : x.view({x.size(0) * x.size(1), x.size(2), width});
+}
+torch::Tensor as_matrices(const torch::Tensor& f) { return f.view({f.size(0), f.size(1), f.size(2) * f.size(3)}); }
+
+torch::Tensor mask_logits_forward(const torch::Tensor& queries, const torch::Tensor& features,
+                                  const c10::optional<torch::Tensor>& offsets) {
+  const auto out = mask_shape(queries, features, offsets);
+  ML_CHECK_INPUT(queries);
+  ML_CHECK_INPUT(features);
+  int64_t n = 1;
+  for (const int64_t d : out) n *= d;
+  if (n == 0 && !offsets.has_value()) return torch::empty(out, queries.options());  // perhaps no group
+  return grouped_matmul_forward(as_groups(queries, queries.size(-1), offsets.has_value()), as_matrices(features),
+                                offsets, false)
+      .view(out);
+}
+
+// A grouped product, or (maps) mask logits.
 struct GroupedNode : public torch::autograd::Function<GroupedNode> {
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input,
                                const torch::Tensor& weight, const c10::optional<torch::Tensor>& offsets,
-                               bool transposed) {
+                               bool transposed, bool maps) {
     const auto x = input.contiguous(), w = weight.contiguous();
     c10::optional<torch::Tensor> o;
     if (offsets.has_value()) o = offsets->contiguous();
-    auto y = grouped_matmul_forward(x, w, o, transposed);
+    auto y = maps ? mask_logits_forward(x, w, o) : grouped_matmul_forward(x, w, o, transposed);
     ctx->save_for_backward({x, w, o.has_value() ? *o : torch::Tensor()});
-    ctx->saved_data["transposed"] = transposed;
+    ctx->saved_data["form"] = (int64_t)(transposed ? 1 : 0) | (maps ? 2 : 0);
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list g) {
     const auto sv = ctx->get_saved_variables();
+    auto x = sv[0], w = sv[1];
     c10::optional<torch::Tensor> o;
     if (sv[2].defined()) o = sv[2];
-    const bool transposed = ctx->saved_data["transposed"].toBool();
-    const auto gy = g[0].detach().contiguous();
+    const int64_t form = ctx->saved_data["form"].toInt();
+    const bool transposed = form & 1, maps = form & 2;
+    auto gy = g[0].detach().contiguous();
     torch::Tensor dx, dw;
-    if (ctx->needs_input_grad(0)) dx = grouped_matmul_backward_input(gy, sv[1], o, transposed);
-    if (ctx->needs_input_grad(1))
-      dw = grouped_matmul_backward_weight(sv[0], gy, o, sv[1].size(0), transposed);
-    return once({dx, dw, torch::Tensor(), torch::Tensor()}, "the backward of grouped_matmul cannot be differentiated");
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    if (maps && gy.numel() == 0) {
+      if (need_x) dx = torch::zeros_like(x);
+      if (need_w) dw = torch::zeros_like(w);
+    } else {
+      if (maps) {
+        w = as_matrices(w);
+        gy = as_groups(gy, w.size(2), o.has_value());
+        x = as_groups(x, x.size(-1), o.has_value());
+      }
+      if (need_x) dx = grouped_matmul_backward_input(gy, w, o, transposed).view(sv[0].sizes());
+      if (need_w) dw = grouped_matmul_backward_weight(x, gy, o, w.size(0), transposed).view(sv[1].sizes());
+    }
+    return once({dx, dw, torch::Tensor(), torch::Tensor(), torch::Tensor()},
+                maps ? "the backward of mask_logits cannot be differentiated"
+                     : "the backward of grouped_matmul cannot be differentiated");
   }
 };
 
 torch::Tensor grouped_matmul_autograd(const torch::Tensor& input, const torch::Tensor& weight,
                                       const c10::optional<torch::Tensor>& offsets, bool transposed) {
-  return GroupedNode::apply(input, weight, offsets, transposed);
+  return GroupedNode::apply(input, weight, offsets, transposed, false);
+}
+
+torch::Tensor mask_logits_autograd(const torch::Tensor& queries, const torch::Tensor& features,
+                                   const c10::optional<torch::Tensor>& offsets) {
+  return GroupedNode::apply(queries, features, offsets, false, true);
 }
 
 // Device flag (int32, shape (1,)): 1 if any element of `x` equals `value`.
@@ -1212,6 +1271,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_matmul_backward_weight", &grouped_matmul_backward_weight,
         "Gradient of grouped_matmul_forward with respect to its matrices (HIP)", py::arg("input"),
         py::arg("grad_out"), py::arg("offsets"), py::arg("matrices"), py::arg("transposed") = false);
+  m.def("mask_logits_forward", &mask_logits_forward,
+        "Mask logits: an image's queries times its feature map (HIP)", py::arg("queries"), py::arg("features"),
+        py::arg("offsets") = py::none());
+  m.def("mask_logits_autograd", &mask_logits_autograd,
+        "Mask logits as a C++ autograd node, differentiable in queries and features (HIP)", py::arg("queries"),
+        py::arg("features"), py::arg("offsets") = py::none());
   m.def("grouped_matmul_autograd", &grouped_matmul_autograd,
         "Grouped product as a C++ autograd node, differentiable in input and weight (HIP)", py::arg("input"),
         py::arg("weight"), py::arg("offsets"), py::arg("transposed") = false);
