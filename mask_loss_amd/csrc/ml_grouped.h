@@ -66,15 +66,17 @@ struct GroupedArgs {
   int rows, groups, matrices;
   int K;                   // reduced length (rows kernel)
   int M, N;                // output rows (weight gradient) and columns
-  int splits;              // parts of the reduction, each with its own float plane
-  int64_t plane;           // elements of one plane (splits > 1)
-  void* c;                 // output, or the planes
+  int splits;              // grouped_kernel: parts of each tile's reduction, float planes in `parts`;
+                           // grouped_ring_kernel: most parts of a tile of the last round
+  int fewest;              // parts from which on they are worth their join behind whole rounds
+  int64_t plane;           // elements of one plane
+  void* c;                 // output
+  float* parts;
   int segments;            // row ranges with a matrix: the groups, or (merged) the matrices
   int merged;              // the rows of the groups that share a matrix make tiles together
   FastDiv layers;          // groups per matrix
-  FastDiv cols, parts;     // column tiles; splits
+  FastDiv cols;            // column tiles
   FastDiv mtiles;          // row tiles of a matrix (weight gradient)
-  int ntiles;              // column tiles
 };
 
 template <int DT>
@@ -300,16 +302,15 @@ __device__ __forceinline__ int merged_row(const GroupedArgs& a, const int* e, in
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Tiles of BM rows up to and with each segment, t[0 .. segments + 1]; returns their number.  Every wave
+// Tiles of bm rows up to and with each segment, t[0 .. segments + 1]; returns their number.  Every wave
 // writes the same values.
-template <int BM>
-__device__ __forceinline__ int segment_tiles(const GroupedArgs& a, const int* e, int* t) {
+__device__ __forceinline__ int segment_tiles(const GroupedArgs& a, const int* e, int* t, int bm) {
   const int lane = threadIdx.x & 63;
   int tiles = 0;
   for (int base = 0; base < a.segments + 2; base += 64) {
     int r0, r1;
     segment(a, e, base + lane, r0, r1);
-    int v = (r1 - r0 + BM - 1) / BM;
+    int v = (int)((uint32_t)(r1 - r0 + bm - 1) / (uint32_t)bm);
     v = scan_sum(v) + tiles;
     if (base + lane < a.segments + 2) t[base + lane] = v;
     tiles = __builtin_amdgcn_readlane(v, 63);
@@ -318,79 +319,80 @@ __device__ __forceinline__ int segment_tiles(const GroupedArgs& a, const int* e,
   return tiles;
 }
 
-// A work item: a tile of the output and its part of the reduction, `steps` steps of BK from reduced
-// index k on; k runs to kend, then (weight gradient) through the matrix's next groups.
+// A work item: a tile of the output and part `part` of `parts` of its reduction, `steps` steps of bk from
+// reduced index k on; k runs to kend, then (weight gradient) through the matrix's next groups.
 struct Work {
-  int m0, n0, mlim, w, split, steps;
+  int m0, n0, mlim, w, steps;
   int seg, k, kend;
   int mapped;  // m0 counts matrix w's rows (merged_row), not the tensor's
 };
 
-// Steps of part `part` begin at this one of n.
-__device__ __forceinline__ int part_start(const GroupedArgs& a, int n, int part) {
-  const int each = div_by(n, a.parts);
-  return each * part + min(part, n - each * a.splits);
+// Steps of part `part` of `parts` begin at this one of n.
+__device__ __forceinline__ int part_start(int n, int part, int parts) {
+  if (parts == 1) return part * n;
+  const int each = n / parts;
+  return each * part + min(part, n - each * parts);
 }
 
 constexpr int kBand = 4;
-// Rows kernels, item id of tiles * ntiles * splits.  Bands of kBand row tiles pass over the columns
+// Rows kernels, tile id of tiles * column tiles.  Bands of kBand row tiles pass over the columns
 // together: their rows and the matrix's columns are both met again while they are in the L2.
-template <int BM, int BN, int BK>
-__device__ __forceinline__ Work rows_work(const GroupedArgs& a, const int* e, const int* t, int tiles, int id) {
+__device__ __forceinline__ Work rows_work(const GroupedArgs& a, const int* e, const int* t, int tiles, int id, int part,
+                                          int parts, int bm, int bn, int bk) {
   const int lane = threadIdx.x & 63;
   Work it;
   it.seg = 0;
-  const int band = div_by(div_by(id >> 2, a.cols), a.parts);  // kBand = 4
+  const int band = div_by(id >> 2, a.cols);  // kBand = 4
   const int height = min(kBand, tiles - band * kBand);
-  const int rest = id - band * kBand * a.ntiles * a.splits;
+  const int rest = id - band * kBand * a.cols.d;
   const int y = height == 4 ? rest >> 2 : height == 3 ? (int)(__umulhi((uint32_t)rest, 0xAAAAAAABu) >> 1)
                                                       : rest >> (height - 1);
-  it.split = div_by(y, a.cols);
-  it.n0 = (y - it.split * a.ntiles) * BN;
+  it.n0 = y * bn;
   const int tile = band * kBand + rest - y * height;
   int q = 0;
   for (int base = 0; base < a.segments + 2; base += 64)
     q += __popcll(__ballot(base + lane < a.segments + 2 && t[base + lane] <= tile));
   int r0, r1;
   segment(a, e, q, r0, r1);
-  it.m0 = uniform(r0 + (tile - (q ? t[q - 1] : 0)) * BM);
+  it.m0 = uniform(r0 + (tile - (q ? t[q - 1] : 0)) * bm);
   it.mlim = uniform(r1) - it.m0;
   const bool zero = q >= a.segments;
   it.w = zero ? 0 : a.merged ? q : div_by(q, a.layers);
   it.mapped = a.merged && !zero;
-  const int steps = zero ? 0 : (a.K + BK - 1) / BK;
-  const int s0 = part_start(a, steps, it.split);
-  it.steps = part_start(a, steps, it.split + 1) - s0;
-  it.k = s0 * BK;
+  const int steps = zero ? 0 : (int)((uint32_t)(a.K + bk - 1) / (uint32_t)bk);
+  const int s0 = part_start(steps, part, parts);
+  it.steps = part_start(steps, part + 1, parts) - s0;
+  it.k = s0 * bk;
   it.kend = zero ? 0 : a.K;
   return it;
 }
 
-// Weight gradient, item id of matrices * splits * ntiles * mtiles.
-template <int BM, int BN, int BK>
-__device__ __forceinline__ Work weight_work(const GroupedArgs& a, const int* e, int id) {
+// Weight gradient, tile id of matrices * column tiles * row tiles.
+__device__ __forceinline__ Work weight_work(const GroupedArgs& a, const int* e, int id, int part, int parts, int bm,
+                                            int bn, int bk) {
   Work it;
   it.mapped = 0;
-  const int x = div_by(id, a.mtiles), y = div_by(x, a.cols);
-  it.m0 = (id - x * a.mtiles.d) * BM;
+  const int x = div_by(id, a.mtiles);
+  it.m0 = (id - x * a.mtiles.d) * bm;
   it.mlim = a.M - it.m0;
-  it.n0 = (x - y * a.ntiles) * BN;
-  it.w = div_by(y, a.parts);
-  it.split = y - it.w * a.splits;
+  it.w = div_by(x, a.cols);
+  it.n0 = (x - it.w * a.cols.d) * bn;
   const int* ew = e + it.w;
+  auto steps_of = [&](int s) {
+    return (int)((uint32_t)(ew[s * a.matrices + 1] - ew[s * a.matrices] + bk - 1) / (uint32_t)bk);
+  };
   int steps = 0;
-  for (int s = 0; s < a.layers.d; ++s) steps += (ew[s * a.matrices + 1] - ew[s * a.matrices] + BK - 1) / BK;
+  for (int s = 0; s < a.layers.d; ++s) steps += steps_of(s);
   steps = uniform(steps);
-  const int s0 = part_start(a, steps, it.split);
-  it.steps = part_start(a, steps, it.split + 1) - s0;
+  const int s0 = part_start(steps, part, parts);
+  it.steps = part_start(steps, part + 1, parts) - s0;
   it.k = it.kend = 0;
   int skip = s0;
   for (it.seg = 0; it.seg < a.layers.d; ++it.seg) {
-    const int lo = uniform(ew[it.seg * a.matrices]), hi = uniform(ew[it.seg * a.matrices + 1]);
-    const int n = (hi - lo + BK - 1) / BK;
+    const int n = uniform(steps_of(it.seg));
     if (skip < n) {
-      it.k = lo + skip * BK;
-      it.kend = hi;
+      it.k = uniform(ew[it.seg * a.matrices]) + skip * bk;
+      it.kend = uniform(ew[it.seg * a.matrices + 1]);
       break;
     }
     skip -= n;
@@ -423,18 +425,21 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
   group_edges(a, e);
   const int lane = threadIdx.x & 63;
   Work it;
+  int split;
   if constexpr (WG) {
-    const int id = xcd_item(a.matrices * a.mtiles.d * a.ntiles * a.splits);
+    const int count = a.matrices * a.mtiles.d * a.cols.d, id = xcd_item(count * a.splits);
     if (id < 0) return;
-    it = weight_work<BM, BN, BK>(a, e, id);
+    split = id / count;
+    it = weight_work(a, e, id - split * count, split, a.splits, BM, BN, BK);
   } else {
     int* t = e + a.groups + 1;
-    const int tiles = segment_tiles<BM>(a, e, t), id = xcd_item(tiles * a.ntiles * a.splits);
+    const int tiles = segment_tiles(a, e, t, BM), count = tiles * a.cols.d, id = xcd_item(count * a.splits);
     if (id < 0) return;
-    it = rows_work<BM, BN, BK>(a, e, t, tiles, id);
+    split = id / count;
+    it = rows_work(a, e, t, tiles, id - split * count, split, a.splits, BM, BN, BK);
   }
   const int m0 = uniform(it.m0), n0 = uniform(it.n0), mlim = uniform(it.mlim), w = uniform(it.w);
-  const int steps_left = uniform(it.steps), split = it.split;
+  const int steps_left = uniform(it.steps);
   int k = uniform(it.k), kend = uniform(it.kend), seg = uniform(it.seg);
   const int nlim = a.N - n0;
 
@@ -507,7 +512,7 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
   // lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile
   const int64_t first = WG ? (int64_t)w * a.cstride : 0;
   const bool planes = a.splits > 1;
-  float* cf = (float*)a.c + (planes ? (int64_t)split * a.plane : 0);
+  float* cf = planes ? a.parts + (int64_t)split * a.plane : (float*)a.c;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const int m = wm + 16 * j + (lane & 15);
@@ -590,6 +595,28 @@ template <int N>
 __device__ __forceinline__ void ring_wait() {
   static_assert(N < 64, "vmcnt");
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// An XCD's run of consecutive tiles, from `start` on, among its workgroups (gridDim.x / kXcds): whole ones in
+// full rounds, and those of the last round, where they would leave half of the workgroups or
+// more without work, in parts of their reduction.
+struct RingShare {
+  int start, whole, rest, parts;
+};
+__device__ __forceinline__ RingShare ring_share(const GroupedArgs& a, int count, int xcd, int turns) {
+  RingShare s;
+  const int per = (count + kXcds - 1) / kXcds;
+  s.start = xcd * per;
+  const int mine = max(0, min(per, count - s.start));
+  s.rest = mine % turns;
+  s.whole = mine - s.rest;
+  s.parts = s.rest ? min(a.splits, turns / s.rest) : 1;
+  if (s.parts < (s.whole ? a.fewest : 2)) {
+    s.whole = mine;
+    s.rest = 0;
+    s.parts = 1;
+  }
+  return s;
 }
 
 // One operand of a stage, filled by NW waves.
@@ -675,12 +702,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
   group_edges(a, e);
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   int* t = e + a.groups + 1;
-  int tiles;
-  if constexpr (WG) tiles = a.matrices * a.mtiles.d;
-  else tiles = segment_tiles<BM>(a, e, t);
-  const int items = tiles * a.ntiles * a.splits;
-  const int per = (items + kXcds - 1) / kXcds, xcd = (int)blockIdx.x % kXcds, turns = (int)gridDim.x / kXcds;
-  const int first = xcd * per + (int)blockIdx.x / kXcds, last = min((xcd + 1) * per, items);
+  const int tiles = WG ? a.matrices * a.mtiles.d : segment_tiles(a, e, t, BM);
+  const int xcd = (int)blockIdx.x % kXcds, turns = (int)gridDim.x / kXcds, first = (int)blockIdx.x / kXcds;
+  const RingShare share = ring_share(a, tiles * a.cols.d, xcd, turns);
+  const int last = share.whole + share.rest * share.parts;
   if (first >= last) return;
 
   // ---- loads
@@ -697,9 +722,16 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
       seg = a.layers.d;
       return;
     }
-    Work it;
-    if constexpr (WG) it = weight_work<BM, BN, BK>(a, e, next);
-    else it = rows_work<BM, BN, BK>(a, e, t, tiles, next);
+    int tile = share.start + next, part = 0, parts = 1;
+    if (next >= share.whole) {  // a part of one of the last tiles
+      const int p = next - share.whole, r = p / share.parts;
+      tile = share.start + share.whole + r;
+      parts = share.parts;
+      part = p - r * parts;
+    }
+    const Work it0 = WG ? weight_work(a, e, tile, part, parts, BM, BN, BK)
+                        : rows_work(a, e, t, tiles, tile, part, parts, BM, BN, BK);
+    Work it = it0;
     next += turns;
     it.steps = max(it.steps, 1);  // nothing to reduce: one stage of zeros
     if (lane == 0) {
@@ -708,7 +740,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
       q[1] = it.n0;
       q[2] = it.mlim;
       q[3] = it.w;
-      q[4] = it.split;
+      q[4] = parts > 1 ? next - turns - share.whole : -1;
       q[5] = it.steps;
       q[6] = it.mapped;
     }
@@ -800,17 +832,23 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
 
     // lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile; columns come in
     // whole chunks
-    const int m0 = uniform(q[0]), n0 = uniform(q[1]), tm = uniform(q[2]), iw = uniform(q[3]), split = uniform(q[4]);
+    const int m0 = uniform(q[0]), n0 = uniform(q[1]), tm = uniform(q[2]), iw = uniform(q[3]), block = uniform(q[4]);
     const bool mapped = uniform(q[6]) != 0;
     const int tn = a.N - n0;
-    const bool planes = a.splits > 1, full = tm >= BM && tn >= BN && !planes;
-    const int64_t origin = (planes ? (int64_t)split * a.plane : 0) + (WG ? (int64_t)iw * a.cstride : 0) + n0;
+    const bool full = tm >= BM && tn >= BN && block < 0;
+    const int64_t origin = (WG ? (int64_t)iw * a.cstride : 0) + n0;
     const int mr = wm + (lane & 15), g = lane >> 4;
     auto row_start = [&](int j) {  // of the lane's row in row tile j
       const int r = mr + 16 * j;
       return origin + (int64_t)(mapped ? merged_row(a, e, iw, m0 + min(r, tm - 1)) : m0 + r) * a.ldc;
     };
-    if (planes || DT == ML_F32) {
+    if (block >= 0) {  // in the order of the registers (grouped_tail_kernel)
+      f32x4_t* c = (f32x4_t*)a.parts + ((int64_t)(xcd * turns + block) * NW + wave) * (TN * TM * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) c[(i * TM + j) * 64] = acc[i][j];
+    } else if constexpr (DT == ML_F32) {
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         float* c = (float*)a.c + row_start(j) + wn + 4 * g;
@@ -818,7 +856,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
         for (int i = 0; i < TN; ++i)
           if (full || (mr + 16 * j < tm && wn + 16 * i + 4 * g < tn)) *(f32x4_loose*)(c + 16 * i) = acc[i][j];
       }
-    } else if constexpr (DT != ML_F32) {
+    } else {
       // two tiles' columns change places between lane groups 0 and 1, 2 and 3, so that a lane
       // has eight consecutive ones: of the first tile in even groups, of the second in odd ones
       const int col = wn + 16 * (g & 1) + 8 * (g >> 1);
@@ -839,6 +877,45 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
     credit = full ? NS - 1 : 0;
   }
   ring_wait<0>();  // the last loads, of zeros, end before the LDS goes to another workgroup
+}
+
+// The last round's tiles of a grouped_ring_kernel launch of `turns` workgroups an XCD (same arguments):
+// sums of their parts in order.  Workgroup i of an XCD takes 1 / parts of tile i / parts.  A part is
+// bm * bn floats as the waves' registers hold them.
+template <int DT>
+__global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg, int bm, int bn, int turns) {
+  extern __shared__ int e[];
+  group_edges(a, e);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* t = e + a.groups + 1;
+  const int tiles = wg ? a.matrices * a.mtiles.d : segment_tiles(a, e, t, bm);
+  const int xcd = (int)blockIdx.x % kXcds, i = (int)blockIdx.x / kXcds;
+  const RingShare share = ring_share(a, tiles * a.cols.d, xcd, turns);
+  if (i >= share.rest * share.parts) return;
+  const int r = i / share.parts, piece = i - r * share.parts, tile = share.start + share.whole + r;
+  const Work it = wg ? weight_work(a, e, tile, 0, 1, bm, bn, 1) : rows_work(a, e, t, tiles, tile, 0, 1, bm, bn, 1);
+  const int tm = bm / 32, tn = bn / 32, chunks = 4 * tm * tn;  // 2 x 2 waves; 64 x 4 values to a chunk
+  const f32x4_t* p = (const f32x4_t*)a.parts + (int64_t)(xcd * turns + r * share.parts) * chunks * 64 + lane;
+  const int c1 = (piece + 1) * chunks / share.parts;
+  for (int c = piece * chunks / share.parts + wave; c < c1; c += 4) {
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kFlight = 8;
+    for (int s = 0; s < share.parts; s += kFlight) {
+      f32x4_t u[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j)
+        u[j] = s + j < share.parts ? p[((int64_t)(s + j) * chunks + c) * 64] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) v += u[j];
+    }
+    const int wv = c / (tm * tn), x = c - wv * tm * tn, ci = x / tm, cj = x - ci * tm;
+    const int row = (wv & 1) * (bm / 2) + 16 * cj + (lane & 15), col = (wv >> 1) * (bn / 2) + 16 * ci + 4 * (lane >> 4);
+    if (row >= it.mlim || col >= a.N - it.n0) continue;  // columns come in whole chunks
+    const int64_t at = (wg ? (int64_t)it.w * a.cstride : 0) +
+                       (int64_t)(it.mapped ? merged_row(a, e, it.w, it.m0 + row) : it.m0 + row) * a.ldc + it.n0 + col;
+    if constexpr (DT == ML_F32) *(f32x4_loose*)((float*)a.c + at) = v;
+    else *(u32x2_loose*)((uint16_t*)a.c + at) = u32x2_t{GMma<DT>::pack(v[0], v[1]), GMma<DT>::pack(v[2], v[3])};
+  }
 }
 
 }  // namespace ml

@@ -16,6 +16,7 @@
 // HBM lines and win; operands by rows are whole lines anyway, and the larger tiles read LDS less
 // often.  The choice also weighs how the tiles fill the compute units (grouped_plan).
 #include <algorithm>
+#include <cmath>
 
 #include "ml_grouped.h"
 
@@ -69,7 +70,7 @@ constexpr TileShape kTiles[] = {{32, 128, 4}, {128, 128, 2}, {128, 128, 2}, {128
 
 struct GroupedPlan {
   Tile tile;
-  int splits;
+  int splits, fewest;
   bool merged;
   int64_t m, n, k;          // output rows and columns, reduced length (weight gradient: mean rows per matrix)
   int64_t bound;            // work items at most
@@ -81,8 +82,10 @@ constexpr int64_t kMaxGroups = 4000;   // their edges and tile counts fit the LD
 constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 bytes of its first
 constexpr int64_t kUnits = 256;
 
-// aligned: every row of the operands and of the result starts on a 16-byte boundary; transposed: as the call's
-int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transposed, bool aligned, GroupedPlan& p) {
+// aligned: every row of the operands and of the result starts on a 16-byte boundary; transposed: as the call's;
+// equal: without offsets
+int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transposed, bool aligned, bool equal,
+                 GroupedPlan& p) {
   if (!s || s->rows < 0 || s->K < 0 || s->N < 0 || s->groups < 1 || s->matrices < 1 || s->groups % s->matrices)
     return fail(ML_EINVAL, "grouped_matmul: invalid shape (groups must be a positive multiple of the matrices)");
   if (dtype != ML_F32 && dtype != ML_BF16 && dtype != ML_F16)
@@ -104,67 +107,86 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
   const int64_t out = (wg ? s->matrices : 1) * p.m * p.n;
 
   const int64_t steps = std::max<int64_t>(1, ceil_div(p.k, bk));
-  // Rough time of a tile shape, in steps of 128 x 128 outputs on one compute unit.
-  auto plan = [&](Tile t, double factor, int& splits) {
-    const TileShape& T = kTiles[t];
-    const double mt = wg ? (double)s->matrices * ceil_div(p.m, T.bm)
-                         : used * (each / T.bm <= 1.0 ? 1.0 : each / T.bm + 0.5);
-    const double tiles = mt * ceil_div(p.n, T.bn), slots = (double)kUnits * T.occ;
-    // split the reduction where the tiles leave slots without work, at least four steps to a part
-    splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)(slots / tiles), steps / 4, 64}));
-    const double rounds = tiles * splits / slots;
-    const double area = T.bm * T.bn / 16384.0 * T.occ;
-    double c = (rounds < 4.0 ? std::max(1.0, std::ceil(rounds - 0.05)) : rounds + 0.5) * area * factor *
-               ((double)steps / splits + 4.0);
-    if (splits > 1) c += (double)splits * out * 8.0 * 2e-6;  // planes written and read again: 0.5 us to a step
-    return c;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 64));  // parts of at least four steps
+  auto tiles_of = [&](Tile t) {
+    const double x = each / kTiles[t].bm;
+    const double mt = wg ? (double)s->matrices * ceil_div(p.m, kTiles[t].bm)
+                         : used * (equal || x <= 1.0 ? std::ceil(x) : x + 0.5);
+    return std::max(1.0, mt * ceil_div(p.n, kTiles[t].bn));
+  };
+  // Rough time in us of a round of the persistent workgroups, and of all rounds, the last one in parts
+  // (ring_share), whose join takes kJoin.
+  constexpr double kJoin = 15.0;
+  const double unit = dtype == ML_F32 ? 1.75 : 0.5;  // a step of 128 x 128 outputs on one compute unit
+  auto round = [&](Tile t) { return kTiles[t].bm * kTiles[t].bn * kTiles[t].occ / 16384.0 * (steps + 4.0) * unit; };
+  auto fewest_parts = [&](Tile t) {  // (1 - 1 / parts) of a round saved, for more than a join
+    const double r = round(t);
+    return r > kJoin * 1.02 ? std::max(2, (int)std::ceil(1.0 / (1.0 - kJoin / r))) : 1 << 30;
+  };
+  // parts of the last round's tiles that are to be expected, 1 for none
+  auto expected_parts = [&](Tile t, double& whole) {
+    const double rounds = tiles_of(t) / (kUnits * kTiles[t].occ);
+    whole = std::floor(rounds + 0.02);
+    const double rest = rounds - whole;
+    if (rest < 0.02) return 0;
+    const int parts = std::min(most, (int)(1.0 / rest + 0.02));
+    return parts < (whole > 0.0 ? fewest_parts(t) : 2) ? 1 : parts;
+  };
+  auto cost = [&](Tile t, double factor) {
+    double whole;
+    const int parts = expected_parts(t, whole);
+    return (whole + (parts ? 1.0 / parts : 0.0)) * round(t) * factor + (parts > 1 ? kJoin : 0.0);
   };
   if (!wg && each <= 32.0) {
     p.tile = kFew;
-    plan(p.tile, 1.0, p.splits);
   } else if (!aligned) {
     p.tile = kPlain;
-    plan(p.tile, 1.0, p.splits);
   } else if (dtype == ML_F32) {
     p.tile = wg ? kDeep128 : kWide128;
-    plan(p.tile, 1.0, p.splits);
   } else {
     const int rowops = wg ? 2 : (which == kForward) == transposed ? 0 : 1;  // operands by rows of the reduced index
     // by the table above, per tile area
     constexpr double f[3][3] = {{1.0, 1.05, 1.1}, {1.1, 1.0, 0.95}, {1.3, 1.0, 0.92}};
     const Tile ts[3] = {kWide128, kDeep128x256, kDeep256};
     double best = 0.0;
-    int n1 = 1;
     for (int i = 0; i < 3; ++i) {
-      const double c = plan(ts[i], f[rowops][i], n1);
+      const double c = cost(ts[i], f[rowops][i]);
       if (i && c >= best) continue;
       best = c;
       p.tile = ts[i];
-      p.splits = n1;
     }
   }
   const TileShape& T = kTiles[p.tile];
   const int64_t mt = wg ? s->matrices * ceil_div(p.m, T.bm) : s->rows / T.bm + std::min(segments + 2, s->rows);
-  p.bound = mt * ceil_div(p.n, T.bn) * p.splits;
+  const int64_t tiles = mt * ceil_div(p.n, T.bn);
+  if (p.tile >= kDeep128) {
+    double whole;
+    p.splits = expected_parts(p.tile, whole) > 1 ? most : 1;  // (the counts on the GPU decide)
+    p.fewest = fewest_parts(p.tile);
+    p.bound = tiles;
+    p.bytes = p.splits > 1 ? (size_t)kUnits * T.occ * T.bm * T.bn * sizeof(float) : 256;
+  } else {
+    // parts of each tile's reduction where the tiles leave slots without work
+    p.splits = std::max(1, std::min((int)(kUnits * T.occ / tiles_of(p.tile)), most));
+    p.bound = tiles * p.splits;
+    p.plane = ceil_div(out, 4) * 4;
+    p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
+  }
   if (p.bound > INT32_MAX - 8) return fail(ML_EUNSUPPORTED, "grouped_matmul: too many tiles");
-  p.plane = ceil_div(out, 4) * 4;
-  p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
   return ML_OK;
 }
 
 template <int DT, bool WG, bool BKC>
 int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
   const TileShape& T = kTiles[p.tile];
-  a.ntiles = (int)ceil_div(a.N, T.bn);
-  a.cols = fast_div(a.ntiles);
-  a.parts = fast_div(a.splits);
+  a.cols = fast_div(ceil_div(a.N, T.bn));
   a.layers = fast_div(a.groups / a.matrices);
   a.mtiles = fast_div(WG ? ceil_div(a.M, T.bm) : 1);
   const size_t lds = (2 * (size_t)a.groups + 3) * sizeof(int);
-  // one workgroup to an item (rounded up for xcd_item), or persistent ones
+  // one workgroup to an item (rounded up for xcd_item), or persistent ones: all that fit where tiles may be split
   const bool ring = p.tile >= kDeep128;
-  const dim3 grid((unsigned)(ring ? std::min<int64_t>(kUnits * T.occ, ceil_div(p.bound, kXcds) * kXcds)
-                                  : ceil_div(p.bound, kXcds) * kXcds)), blk(256);
+  const int64_t items = ceil_div(p.bound, kXcds) * kXcds, slots = kUnits * T.occ;
+  const dim3 grid((unsigned)(!ring ? items : a.splits > 1 ? slots : std::min(items, slots))), blk(256);
   switch (p.tile) {
     case kFew:
       if constexpr (!WG) hipLaunchKernelGGL((grouped_kernel<DT, false, BKC, 32, 128, 1, 4>), grid, blk, lds, st, a);
@@ -187,6 +209,9 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
         hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 2, 64, 4, 1>), grid, blk, lds, st, a);
       break;
   }
+  int rc = check_launch("grouped_matmul");
+  if (rc || !ring || a.splits == 1) return rc;
+  hipLaunchKernelGGL(grouped_tail_kernel<DT>, grid, blk, lds, st, a, WG ? 1 : 0, T.bm, T.bn, (int)grid.x / kXcds);
   return check_launch("grouped_matmul");
 }
 
@@ -203,8 +228,10 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   a.segments = p.merged ? a.matrices : a.groups;
   a.merged = p.merged;
   a.splits = p.splits;
+  a.fewest = p.fewest;
   a.plane = p.plane;
-  a.c = p.splits > 1 ? ws : out;
+  a.c = out;
+  a.parts = (float*)ws;
   int rc;
   if (which == kWeight) {
     // stored (K, N): columns of x by columns of grad_out; stored (N, K): the other way round
@@ -230,7 +257,7 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
     const bool kc = (which == kForward) == (transposed != 0);
     rc = kc ? grouped_launch<DT, false, true>(p, a, st) : grouped_launch<DT, false, false>(p, a, st);
   }
-  if (rc || p.splits == 1) return rc;
+  if (rc || p.splits == 1 || p.tile >= kDeep128) return rc;  // ring kernels join their own parts
   const int64_t n = (which == kWeight ? s->matrices : 1) * p.m * p.n;
   hipLaunchKernelGGL(grouped_join_kernel<DT>, dim3((unsigned)ceil_div(n, kJoinQuads * 4)),
                      dim3(kJoinQuads * kJoinSlices), 0, st, (const float*)ws,
@@ -248,7 +275,7 @@ int grouped_call(const ml_grouped_shape* s, int dtype, int which, const void* ro
                  const int64_t* offsets, void* out, void* ws, size_t ws_bytes, ml_stream_t stream) {
   GroupedPlan p;
   const bool aligned = grouped_whole(s, dtype) && ((uintptr_t)rows & 15) == 0 && ((uintptr_t)other & 15) == 0;
-  const int rc = grouped_plan(s, dtype, which, transposed != 0, aligned, p);
+  const int rc = grouped_plan(s, dtype, which, transposed != 0, aligned, !offsets, p);
   if (rc) return rc;
   if (p.m == 0 || p.n == 0) return ML_OK;
   const bool reads = s->rows > 0 && p.k > 0;
@@ -271,10 +298,11 @@ using namespace ml;
 
 extern "C" size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, int dtype, int product) {
   if (product < ML_GROUPED_FORWARD || product > ML_GROUPED_BACKWARD_WEIGHT) return 0;
-  size_t most = 0;  // over both storage orders, and tensors that start on 16-byte boundaries or not
-  for (int i = 0; i < 4; ++i) {
+  // over both storage orders, tensors that start on 16-byte boundaries or not, with and without offsets
+  size_t most = 0;
+  for (int i = 0; i < 8; ++i) {
     GroupedPlan p;
-    if (grouped_plan(s, dtype, product, (i & 1) != 0, (i & 2) && grouped_whole(s, dtype), p)) return 0;
+    if (grouped_plan(s, dtype, product, (i & 1) != 0, (i & 2) && grouped_whole(s, dtype), (i & 4) != 0, p)) return 0;
     most = std::max(most, p.bytes);
   }
   return most;
