@@ -376,7 +376,8 @@ int ml_layer_norm_backward(int dtype, int param_dtype, const void* grad_out, con
  * Rows offsets[g] .. offsets[g + 1] of x (rows, K) form group g of `groups` and take
  * matrix g % matrices of weight (matrices, K, N), or (matrices, N, K) with
  * `transposed`: y_r = x_r W.  So L * B query sets (layer major) share B feature
- * maps.  groups is a positive multiple of matrices, at most 4,000; K, N <= 2^22.
+ * maps.  groups is a positive multiple of matrices, at most 4,000; K, N <= 2^22;
+ * rows <= 2^31 - 4,096.
  * offsets: (groups + 1) int64 on the device, not decreasing; each is held to
  * 0 .. rows and to at least the one before.  NULL: groups of rows / groups rows.  Rows in no group (before the first or
  * behind the last) take zeros in y and grad_input and count for no grad_weight.

@@ -64,6 +64,7 @@ struct GroupedArgs {
   const int64_t* offsets;  // null: groups of `equal` rows
   int equal;
   int rows, groups, matrices;
+  int given;               // groups of the call; groups = 1 where there is one matrix (a range of rows)
   int K;                   // reduced length (rows kernel)
   int M, N;                // output rows (weight gradient) and columns
   int splits;              // grouped_kernel: parts of each tile's reduction, float planes in `parts`;
@@ -254,22 +255,24 @@ __device__ __forceinline__ int scan_sum(int v) {
 }
 
 // Group edges e[0 .. groups] from the offsets, each held to 0 .. rows and to at least
-// the one before, so that any offsets give disjoint groups inside the tensors.  Every
-// wave writes the same values.
+// the one before, so that any offsets give disjoint groups inside the tensors; the groups of
+// one matrix are one range of rows.  Every wave writes the same values.
 __device__ __forceinline__ void group_edges(const GroupedArgs& a, int* e) {
   const int lane = threadIdx.x & 63;
+  const bool range = a.groups < a.given;
   int before = 0;
-  for (int base = 0; base <= a.groups; base += 64) {
+  for (int base = 0; base <= a.given; base += 64) {
     const int i = base + lane;
     int v = 0;
-    if (i <= a.groups) {
+    if (i <= a.given) {
       const int64_t o = a.offsets ? a.offsets[i] : (int64_t)i * a.equal;
       v = o < 0 ? 0 : o > a.rows ? a.rows : (int)o;
     }
     v = max(scan_max(v), before);
-    if (i <= a.groups) e[i] = v;
+    if (i <= (range ? 0 : a.given)) e[i] = v;
     before = __builtin_amdgcn_readlane(v, 63);
   }
+  if (range) e[1] = before;
   __syncthreads();
 }
 
@@ -378,24 +381,30 @@ __device__ __forceinline__ Work weight_work(const GroupedArgs& a, const int* e, 
   it.w = div_by(x, a.cols);
   it.n0 = (x - it.w * a.cols.d) * bn;
   const int* ew = e + it.w;
-  auto steps_of = [&](int s) {
-    return (int)((uint32_t)(ew[s * a.matrices + 1] - ew[s * a.matrices] + bk - 1) / (uint32_t)bk);
+  // 64 groups at a time: all steps of the matrix, then the group that holds this part's first one
+  const int lane = threadIdx.x & 63;
+  auto steps_to = [&](int base) {  // steps of groups base .. base + lane
+    const int s = base + lane;
+    const int n = s < a.layers.d ? ew[s * a.matrices + 1] - ew[s * a.matrices] : 0;
+    return scan_sum((int)((uint32_t)(n + bk - 1) / (uint32_t)bk));
   };
   int steps = 0;
-  for (int s = 0; s < a.layers.d; ++s) steps += steps_of(s);
-  steps = uniform(steps);
-  const int s0 = part_start(steps, part, parts);
+  for (int base = 0; base < a.layers.d; base += 64) steps += __builtin_amdgcn_readlane(steps_to(base), 63);
+  const int s0 = uniform(part_start(steps, part, parts));
   it.steps = part_start(steps, part + 1, parts) - s0;
   it.k = it.kend = 0;
+  it.seg = a.layers.d;
   int skip = s0;
-  for (it.seg = 0; it.seg < a.layers.d; ++it.seg) {
-    const int n = uniform(steps_of(it.seg));
-    if (skip < n) {
-      it.k = uniform(ew[it.seg * a.matrices]) + skip * bk;
+  for (int base = 0; base < a.layers.d; base += 64) {
+    const int upto = steps_to(base), here = __builtin_amdgcn_readlane(upto, 63);
+    if (skip < here) {
+      const int i = __popcll(__ballot(upto <= skip));
+      it.seg = base + i;
+      it.k = uniform(ew[it.seg * a.matrices]) + (skip - (i ? __builtin_amdgcn_readlane(upto, i - 1) : 0)) * bk;
       it.kend = uniform(ew[it.seg * a.matrices + 1]);
       break;
     }
-    skip -= n;
+    skip -= here;
   }
   return it;
 }

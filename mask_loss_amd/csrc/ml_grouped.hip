@@ -79,6 +79,7 @@ struct GroupedPlan {
 };
 
 constexpr int64_t kMaxGroups = 4000;   // their edges and tile counts fit the LDS beside the tiles
+constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 4096;  // positions a step or a tile on stay 32-bit
 constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 bytes of its first
 constexpr int64_t kUnits = 256;
 
@@ -92,16 +93,18 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     return fail(ML_EINVAL, "grouped_matmul: unsupported dtype");
   if (s->groups > kMaxGroups)
     return fail(ML_EUNSUPPORTED, "grouped_matmul: at most " + std::to_string(kMaxGroups) + " groups are supported");
-  if (s->rows > INT32_MAX || s->K > kMaxLength || s->N > kMaxLength)
-    return fail(ML_EUNSUPPORTED, "grouped_matmul: at most 2^31 - 1 rows and K, N of at most 4194304 are supported");
-  const int64_t es = dtype == ML_F32 ? 4 : 2, bk = 128 / es, layers = s->groups / s->matrices;
+  if (s->rows > kMaxRows || s->K > kMaxLength || s->N > kMaxLength)
+    return fail(ML_EUNSUPPORTED, "grouped_matmul: at most 2^31 - 4096 rows and K, N of at most 4194304 are supported");
+  const int64_t es = dtype == ML_F32 ? 4 : 2, bk = 128 / es;
+  const int64_t groups = s->matrices == 1 ? 1 : s->groups, layers = groups / s->matrices;  // (group_edges)
   const bool wg = which == kWeight;
   p.m = wg ? (transposed ? s->N : s->K) : s->rows;
   p.n = wg ? (transposed ? s->K : s->N) : which == kInput ? s->K : s->N;
   p.k = which == kForward ? s->K : which == kInput ? s->N : ceil_div(s->rows, s->matrices);
-  // groups that share a matrix make tiles together, as far as their rows' offsets go
-  p.merged = !wg && layers > 1 && s->rows * p.k * es < ((int64_t)1 << 32);
-  const int64_t segments = p.merged ? s->matrices : s->groups;
+  // groups that share a matrix make tiles together, as far as their rows' offsets go (and while
+  // walking the groups for a row costs little)
+  p.merged = !wg && layers > 1 && layers <= 32 && s->rows * p.k * es < ((int64_t)1 << 32);
+  const int64_t segments = p.merged ? s->matrices : groups;
   const int64_t used = std::min(segments, std::max<int64_t>(s->rows, 1));  // those that can hold rows
   const double each = (double)s->rows / used;
   const int64_t out = (wg ? s->matrices : 1) * p.m * p.n;
@@ -182,7 +185,7 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
   a.cols = fast_div(ceil_div(a.N, T.bn));
   a.layers = fast_div(a.groups / a.matrices);
   a.mtiles = fast_div(WG ? ceil_div(a.M, T.bm) : 1);
-  const size_t lds = (2 * (size_t)a.groups + 3) * sizeof(int);
+  const size_t lds = (2 * (size_t)a.groups + 3) * sizeof(int);  // edges, tiles of the segments
   // one workgroup to an item (rounded up for xcd_item), or persistent ones: all that fit where tiles may be split
   const bool ring = p.tile >= kDeep128;
   const int64_t items = ceil_div(p.bound, kXcds) * kXcds, slots = kUnits * T.occ;
@@ -223,7 +226,8 @@ int grouped_run(const ml_grouped_shape* s, const GroupedPlan& p, int which, cons
   a.offsets = offsets;
   a.equal = (int)(s->rows / s->groups);
   a.rows = (int)s->rows;
-  a.groups = (int)s->groups;
+  a.given = (int)s->groups;
+  a.groups = s->matrices == 1 ? 1 : a.given;
   a.matrices = (int)s->matrices;
   a.segments = p.merged ? a.matrices : a.groups;
   a.merged = p.merged;

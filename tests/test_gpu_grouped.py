@@ -155,6 +155,32 @@ def test_shared_matrices(dt, L, M, n):
     compare(x, w, dy, offsets_of(counts, 1 if counts.sum() < L * M * n else 0), False)
 
 
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("G,M", [(33, 1), (1000, 1), (66, 2), (140, 2), (400, 4), (4000, 2)])
+def test_many_groups_of_a_matrix(G, M, aligned):
+    """More groups to a matrix than make tiles together, or one matrix for all: ragged, some
+    empty, rows before the first and behind the last."""
+    rng = np.random.default_rng(G)
+    rows = 3 * G + 200
+    counts = rng.multinomial(rows - 30, rng.dirichlet(np.ones(G)))
+    K, N = (64, 136) if aligned else (45, 131)
+    x, w, dy = make(rows, K, N, M, "bf16", False, G)
+    compare(x, w, dy, offsets_of(counts, 11), False)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_parts_of_the_last_tiles(dt):
+    """More tiles than the GPU holds at once and a long reduction: the last tiles are split, in
+    every product and with ragged groups, shared matrices and rows in no group."""
+    rng = np.random.default_rng(3)
+    M, K, N = 2, 384, 2304
+    counts = rng.integers(120, 300, size=3 * M)
+    x, w, dy = make(int(counts.sum()) + 20, K, N, M, dt, False, 90)
+    compare(x, w, dy, offsets_of(counts, 7), False)
+    x, w, dy = make(4300, 1152, 2200, 1, dt, True, 91)
+    compare(x, w, dy, [9, 4290], True)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_other_rows_do_not_reach_a_group(dt):
     """NaN and infinity in one group's rows, in its matrix or in rows of no group stay
