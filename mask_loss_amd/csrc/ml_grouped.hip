@@ -131,8 +131,8 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     const double rounds = tiles_of(t) / (kUnits * kTiles[t].occ);
     whole = std::floor(rounds + 0.02);
     const double rest = rounds - whole;
-    if (rest < 0.02) return 0;
-    const int parts = std::min(most, (int)(1.0 / rest + 0.02));
+    if (whole > 0.0 && rest < 0.02) return 0;
+    const int parts = (int)std::min<double>(most, 1.0 / rest + 0.02);
     return parts < (whole > 0.0 ? fewest_parts(t) : 2) ? 1 : parts;
   };
   auto cost = [&](Tile t, double factor) {
@@ -303,7 +303,7 @@ using namespace ml;
 extern "C" size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, int dtype, int product) {
   if (product < ML_GROUPED_FORWARD || product > ML_GROUPED_BACKWARD_WEIGHT) return 0;
   // over both storage orders, tensors that start on 16-byte boundaries or not, with and without offsets
-  size_t most = 0;
+  size_t most = 256;  // (a size of 0 stands for a refused shape)
   for (int i = 0; i < 8; ++i) {
     GroupedPlan p;
     if (grouped_plan(s, dtype, product, (i & 1) != 0, (i & 2) && grouped_whole(s, dtype), (i & 4) != 0, p)) return 0;

@@ -118,6 +118,13 @@ def test_long_reductions(dt, transposed):
     compare(x, w, dy, [0, 5003], transposed)
     x, w, dy = make(2100, 48, 64, 3, dt, transposed, 33)
     compare(x, w, dy, [4, 2000, 2000, 2090], transposed)
+    # the same with rows of whole 16-byte chunks, one tile and a few
+    x, w, dy = make(120, 8192, 64, 1, dt, transposed, 34)
+    compare(x, w, dy, [0, 120], transposed)
+    x, w, dy = make(390, 2056, 8192, 2, dt, transposed, 35)
+    compare(x, w, dy, [5, 180, 385], transposed)
+    x, w, dy = make(6000, 64, 128, 1, dt, transposed, 36)
+    compare(x, w, dy, [0, 5990], transposed)
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
@@ -326,6 +333,28 @@ def test_captured_step():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outs, run(x, w, dy, offsets, False)))
+
+
+def test_refusals():
+    from mask_loss_amd.functions import grouped_matmul, mask_logits
+    x, w = torch.zeros(6, 8, device="cuda"), torch.zeros(2, 8, 3, device="cuda")
+    o = torch.tensor([0, 2, 6]).cuda()
+    bad = [(x, w.half(), o, False, "same dtype"), (x.double(), w.double(), o, False, "float32, bfloat16 or float16"),
+           (x, w, o.int(), False, "int64"), (x, w, o.cpu(), False, "CUDA tensor"), (x, w.cpu(), o, False, "CUDA tensor"),
+           (x, w, o, True, "must have 3 columns"), (x, w[0], o, False, "weight must be"),
+           (x, w, torch.tensor([0, 2, 4, 6]).cuda(), False, "multiple"), (x, w[:0], o, False, "multiple"),
+           (x, w, torch.tensor([0]).cuda(), False, "groups \\+ 1"), (x, w, None, False, "without offsets"),
+           (x[None], w, o, False, "with offsets"), (x.view(3, 2, 8), w, None, False, "multiple")]
+    for x_, w_, o_, t, words in bad:
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match=words):
+                grouped_matmul(x_.detach().requires_grad_(grad), w_, o_, t)
+    q, f = torch.zeros(1, 2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, 4, device="cuda")
+    with pytest.raises(RuntimeError, match="same dtype"):
+        mask_logits(q, f.half())
+    many = torch.zeros(4002, dtype=torch.int64, device="cuda")
+    with pytest.raises(RuntimeError, match="4000 groups"):
+        grouped_matmul(x, w[:1], many)
 
 
 def test_second_derivative_is_refused():

@@ -273,6 +273,22 @@ def test_captured_step():
         assert all(torch.equal(p, q) for p, q in zip(outs, want))
 
 
+def test_refusals():
+    from mask_loss_amd.functions import layer_norm
+    x, w, b = torch.zeros(4, 64, device="cuda"), torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    bad = [(x.double(), None, None, "float32, bfloat16 or float16"), (x.half(), w.bfloat16(), None, "input's dtype"),
+           (x.half(), w, b.half(), "same dtype"), (x, w[:32], None, "shape"), (x, None, b.view(1, 64), "shape"),
+           (x, w.cpu(), None, "CUDA tensor"), (x[:, :0], None, None, "at least 1"),
+           (torch.zeros((), device="cuda"), None, None, "at least 1")]
+    for x_, w_, b_, words in bad:
+        for grad in (False, True):
+            with pytest.raises(RuntimeError, match=words):
+                layer_norm(x_.detach().requires_grad_(grad), w_, b_)
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            layer_norm(x, w, b, eps)
+
+
 def test_second_derivative_is_refused():
     from mask_loss_amd.functions import layer_norm
     x = torch.randn(4, 64, device="cuda", requires_grad=True)
