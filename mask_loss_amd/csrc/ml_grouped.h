@@ -337,6 +337,8 @@ __device__ __forceinline__ int part_start(int n, int part, int parts) {
   return each * part + min(part, n - each * parts);
 }
 
+// (1, 2, 4, 8 row tiles to a band: experts' forward of ml_grouped.hip 201, 173, 163, 173 us, masks' d input
+// 201, 203, 196, 275.)
 constexpr int kBand = 4;
 // Rows kernels, tile id of tiles * column tiles.  Bands of kBand row tiles pass over the columns
 // together: their rows and the matrix's columns are both met again while they are in the L2.
@@ -892,7 +894,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
 // sums of their parts in order.  Workgroup i of an XCD takes 1 / parts of tile i / parts.  A part is
 // bm * bn floats as the waves' registers hold them.
 template <int DT>
-__global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg, int bm, int bn, int turns) {
+__global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg, int bm, int bn, int wn, int turns) {
   extern __shared__ int e[];
   group_edges(a, e);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -903,7 +905,7 @@ __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg
   if (i >= share.rest * share.parts) return;
   const int r = i / share.parts, piece = i - r * share.parts, tile = share.start + share.whole + r;
   const Work it = wg ? weight_work(a, e, tile, 0, 1, bm, bn, 1) : rows_work(a, e, t, tiles, tile, 0, 1, bm, bn, 1);
-  const int tm = bm / 32, tn = bn / 32, chunks = 4 * tm * tn;  // 2 x 2 waves; 64 x 4 values to a chunk
+  const int tm = bm / 32, tn = bn / wn / 16, chunks = 2 * wn * tm * tn;  // 2 x wn waves; 64 x 4 values to a chunk
   const f32x4_t* p = (const f32x4_t*)a.parts + (int64_t)(xcd * turns + r * share.parts) * chunks * 64 + lane;
   const int c1 = (piece + 1) * chunks / share.parts;
   for (int c = piece * chunks / share.parts + wave; c < c1; c += 4) {
@@ -918,7 +920,7 @@ __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg
       for (int j = 0; j < kFlight; ++j) v += u[j];
     }
     const int wv = c / (tm * tn), x = c - wv * tm * tn, ci = x / tm, cj = x - ci * tm;
-    const int row = (wv & 1) * (bm / 2) + 16 * cj + (lane & 15), col = (wv >> 1) * (bn / 2) + 16 * ci + 4 * (lane >> 4);
+    const int row = (wv & 1) * (bm / 2) + 16 * cj + (lane & 15), col = (wv >> 1) * (bn / wn) + 16 * ci + 4 * (lane >> 4);
     if (row >= it.mlim || col >= a.N - it.n0) continue;  // columns come in whole chunks
     const int64_t at = (wg ? (int64_t)it.w * a.cstride : 0) +
                        (int64_t)(it.mapped ? merged_row(a, e, it.w, it.m0 + row) : it.m0 + row) * a.ldc + it.n0 + col;

@@ -6,15 +6,17 @@
 //                                      KC x KC          KC x rows        rows x rows
 //                                      experts  masks   experts  masks   experts  masks
 //                                      forward  d in    d in     forward d weight d weight
-//   128 x 128, 2 stages of 128 bytes   163      216     191      289     266      287
-//   128 x 256, 3 stages of 64 bytes    182      248     182      278     211      238
-//   256 x 256, 4 stages of 64 bytes    180      233     217      254     190      216
+//   128 x 128, 2 stages of 128 bytes   160      195      191      289     266      287
+//   128 x 256, 3 stages of 64 bytes    182      248     172      278     211      238
+//   256 x 256, 4 stages of 64 bytes    180      233     217      245     193      220
 //   grouped_kernel, 128 x 128          229      229     258      402     315      380
 //
 // (experts: 16,384 rows in 16 groups, K = 1,024, N = 4,096; masks: 16 groups of 200 rows, K = 256,
 // N = 65,536; bf16.)  Where both operands' reduced index is contiguous, 128-byte stages read whole
 // HBM lines and win; operands by rows are whole lines anyway, and the larger tiles read LDS less
-// often.  The choice also weighs how the tiles fill the compute units (grouped_plan).
+// often.  (256 x 256 by 4 waves of 128 x 128 instead of 8 of 128 x 64: masks forward 252, d weight 216,
+// experts d weight 199.)  The masks' d input varies from machine to machine, 194 to 237 with the same
+// code: rows 128 KiB apart.  The choice also weighs how the tiles fill the compute units (grouped_plan).
 #include <algorithm>
 #include <cmath>
 
@@ -209,12 +211,13 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
       break;
     case kDeep256:
       if constexpr (DT != ML_F32)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 2, 64, 4, 1>), grid, blk, lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 4, 64, 4, 1>), grid, dim3(512), lds, st, a);
       break;
   }
   int rc = check_launch("grouped_matmul");
   if (rc || !ring || a.splits == 1) return rc;
-  hipLaunchKernelGGL(grouped_tail_kernel<DT>, grid, blk, lds, st, a, WG ? 1 : 0, T.bm, T.bn, (int)grid.x / kXcds);
+  hipLaunchKernelGGL(grouped_tail_kernel<DT>, grid, blk, lds, st, a, WG ? 1 : 0, T.bm, T.bn, p.tile == kDeep256 ? 4 : 2,
+                     (int)grid.x / kXcds);
   return check_launch("grouped_matmul");
 }
 

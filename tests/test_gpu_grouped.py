@@ -186,6 +186,8 @@ def test_parts_of_the_last_tiles(dt):
     compare(x, w, dy, offsets_of(counts, 7), False)
     x, w, dy = make(4300, 1152, 2200, 1, dt, True, 91)
     compare(x, w, dy, [9, 4290], True)
+    x, w, dy = make(2600, 1024, 2048, 1, dt, False, 92)  # the weight's gradient in few large tiles
+    compare(x, w, dy, [3, 2590], False)
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
