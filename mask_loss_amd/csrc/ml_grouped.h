@@ -611,6 +611,8 @@ __device__ __forceinline__ void ring_wait() {
 // An XCD's run of consecutive tiles, from `start` on, among its workgroups (gridDim.x / kXcds): whole ones in
 // full rounds, and those of the last round, where they would leave half of the workgroups or
 // more without work, in parts of their reduction.
+constexpr int kTailParts = 8;  // behind whole rounds: with 16, a join of 67 MB cost more than the parts saved
+                               // (experts' d input of ml_grouped.hip, 32 tiles left: 172 us, with 8 162)
 struct RingShare {
   int start, whole, rest, parts;
 };
@@ -621,7 +623,7 @@ __device__ __forceinline__ RingShare ring_share(const GroupedArgs& a, int count,
   const int mine = max(0, min(per, count - s.start));
   s.rest = mine % turns;
   s.whole = mine - s.rest;
-  s.parts = s.rest ? min(a.splits, turns / s.rest) : 1;
+  s.parts = s.rest ? min(s.whole ? min(a.splits, kTailParts) : a.splits, turns / s.rest) : 1;
   if (s.parts < (s.whole ? a.fewest : 2)) {
     s.whole = mine;
     s.rest = 0;
@@ -891,7 +893,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
 }
 
 // The last round's tiles of a grouped_ring_kernel launch of `turns` workgroups an XCD (same arguments):
-// sums of their parts in order.  Workgroup i of an XCD takes 1 / parts of tile i / parts.  A part is
+// sums of their parts in order, by all workgroups of the XCD, turns / rest of them to a tile.  A part is
 // bm * bn floats as the waves' registers hold them.
 template <int DT>
 __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg, int bm, int bn, int wn, int turns) {
@@ -902,13 +904,14 @@ __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg
   const int tiles = wg ? a.matrices * a.mtiles.d : segment_tiles(a, e, t, bm);
   const int xcd = (int)blockIdx.x % kXcds, i = (int)blockIdx.x / kXcds;
   const RingShare share = ring_share(a, tiles * a.cols.d, xcd, turns);
-  if (i >= share.rest * share.parts) return;
-  const int r = i / share.parts, piece = i - r * share.parts, tile = share.start + share.whole + r;
+  if (share.rest == 0) return;
+  const int pieces = turns / share.rest, r = i / pieces, piece = i - r * pieces, tile = share.start + share.whole + r;
+  if (r >= share.rest) return;
   const Work it = wg ? weight_work(a, e, tile, 0, 1, bm, bn, 1) : rows_work(a, e, t, tiles, tile, 0, 1, bm, bn, 1);
   const int tm = bm / 32, tn = bn / wn / 16, chunks = 2 * wn * tm * tn;  // 2 x wn waves; 64 x 4 values to a chunk
   const f32x4_t* p = (const f32x4_t*)a.parts + (int64_t)(xcd * turns + r * share.parts) * chunks * 64 + lane;
-  const int c1 = (piece + 1) * chunks / share.parts;
-  for (int c = piece * chunks / share.parts + wave; c < c1; c += 4) {
+  const int c1 = (piece + 1) * chunks / pieces;
+  for (int c = piece * chunks / pieces + wave; c < c1; c += 4) {
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     constexpr int kFlight = 8;
     for (int s = 0; s < share.parts; s += kFlight) {

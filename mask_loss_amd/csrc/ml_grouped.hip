@@ -121,12 +121,14 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
   };
   // Rough time in us of a round of the persistent workgroups, and of all rounds, the last one in parts
   // (ring_share), whose join takes kJoin.
-  constexpr double kJoin = 15.0;
+  constexpr double kJoin = 10.0;
   const double unit = dtype == ML_F32 ? 1.75 : 0.5;  // a step of 128 x 128 outputs on one compute unit
   auto round = [&](Tile t) { return kTiles[t].bm * kTiles[t].bn * kTiles[t].occ / 16384.0 * (steps + 4.0) * unit; };
-  auto fewest_parts = [&](Tile t) {  // (1 - 1 / parts) of a round saved, for more than a join
-    const double r = round(t);
-    return r > kJoin * 1.02 ? std::max(2, (int)std::ceil(1.0 / (1.0 - kJoin / r))) : 1 << 30;
+  // a last round that leaves half of the workgroups without work, alone on their compute units then
+  auto last = [&](Tile t) { return kTiles[t].occ > 1 ? 0.55 : 1.0; };
+  auto fewest_parts = [&](Tile t) {  // it less 1 / parts of a round saved, for more than a join
+    const double h = last(t) - kJoin / round(t);
+    return h > 0.02 ? std::max(2, (int)std::ceil(1.0 / h)) : 1 << 30;
   };
   // parts of the last round's tiles that are to be expected, 1 for none
   auto expected_parts = [&](Tile t, double& whole) {
@@ -134,13 +136,15 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     whole = std::floor(rounds + 0.02);
     const double rest = rounds - whole;
     if (whole > 0.0 && rest < 0.02) return 0;
-    const int parts = (int)std::min<double>(most, 1.0 / rest + 0.02);
+    const int parts = (int)std::min<double>(whole > 0.0 ? std::min(most, kTailParts) : most, 1.0 / rest + 0.02);
     return parts < (whole > 0.0 ? fewest_parts(t) : 2) ? 1 : parts;
   };
   auto cost = [&](Tile t, double factor) {
     double whole;
     const int parts = expected_parts(t, whole);
-    return (whole + (parts ? 1.0 / parts : 0.0)) * round(t) * factor + (parts > 1 ? kJoin : 0.0);
+    const double rest = tiles_of(t) / (kUnits * kTiles[t].occ) - whole;
+    const double tail = parts == 0 ? 0.0 : parts > 1 ? 1.0 / parts : rest <= 0.5 ? last(t) : 1.0;
+    return (whole + tail) * round(t) * factor + (parts > 1 ? kJoin : 0.0);
   };
   if (!wg && each <= 32.0) {
     p.tile = kFew;
