@@ -413,7 +413,8 @@ int ml_any_equal(const int64_t* x, int64_t n, int64_t value, int32_t* flag, ml_s
  * When enabled, every kernel launch of this library is bracketed by HIP events
  * recorded on its own stream.  ml_profile_read() waits for those events and
  * returns, for kernel family `name` ("prep", "pair_cost", "assign", "layer",
- * "bwd_mask", "bwd_cls", "label_cost", "prefill"), the number of launches and their
+ * "bwd_mask", "bwd_cls", "label_cost", "prefill", "layer_norm", "layer_norm_backward",
+ * "grouped_matmul"), the number of launches and their
  * summed duration in milliseconds since the last reset. */
 int ml_profile_enable(int enable);
 int ml_profile_read(const char* name, int64_t* launches, double* total_ms);
