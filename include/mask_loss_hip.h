@@ -356,7 +356,7 @@ int ml_dice_loss_backward(const ml_dense_shape* s, int dtype, const float* grad_
  * in front of the mask and class logits.  weight and bias (width,) in param_dtype
  * (`dtype` or ML_F32), each NULL for ones / zeros.  mean and rstd: (rows,) float for
  * the backward, both NULL where none follows.  Statistics are float32, summed about
- * the mean.  Any width; eps >= 0.
+ * the mean.  width <= 2^26; eps >= 0.
  * Backward: grad_input (rows, width) in `dtype`, grad_weight and grad_bias (width,)
  * in param_dtype, each NULL where it is not wanted; sums over the rows are float32
  * in a fixed order.  workspace (ml_layer_norm_backward_workspace_size bytes, 0 for an
@@ -377,10 +377,11 @@ int ml_layer_norm_backward(int dtype, int param_dtype, const void* grad_out, con
  * matrix g % matrices of weight (matrices, K, N), or (matrices, N, K) with
  * `transposed`: y_r = x_r W.  So L * B query sets (layer major) share B feature
  * maps.  groups is a positive multiple of matrices, at most 4,000; K, N <= 2^22;
- * rows <= 2^31 - 4,096.
+ * rows <= 2^31 - 4,096; ML_EUNSUPPORTED also for more than 2^24 - 10 parts of the output of 32 x 128
+ * (128 x 128 with over 32 rows to a group, or in grad_weight) in calls of few or unaligned rows.
  * offsets: (groups + 1) int64 on the device, not decreasing; each is held to
- * 0 .. rows and to at least the one before.  NULL: groups of rows / groups rows.  Rows in no group (before the first or
- * behind the last) take zeros in y and grad_input and count for no grad_weight.
+ * 0 .. rows and to at least the one before.  NULL: groups of rows / groups rows.
+ * Rows in no group (before the first or behind the last) take zeros in y and grad_input and count for no grad_weight.
  * All tensors in `dtype`; sums are float32, rounded once, in an order that the
  * shape fixes.  grad_weight has weight's layout.
  * Workspace: ml_grouped_matmul_workspace_size bytes for the product, 0 for a

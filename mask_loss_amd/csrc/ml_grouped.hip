@@ -85,10 +85,12 @@ constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 4096;  // positions a step or 
 constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 bytes of its first
 constexpr int64_t kUnits = 256;
 
-// aligned: every row of the operands and of the result starts on a 16-byte boundary; transposed: as the call's;
+// aligned: every row of the operands starts on a 16-byte boundary, rows of all three tensors are whole
+// 16-byte chunks (the result may start anywhere); transposed: as the call's;
 // equal: without offsets
 int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transposed, bool aligned, bool equal,
                  GroupedPlan& p) {
+  p = GroupedPlan{};
   if (!s || s->rows < 0 || s->K < 0 || s->N < 0 || s->groups < 1 || s->matrices < 1 || s->groups % s->matrices)
     return fail(ML_EINVAL, "grouped_matmul: invalid shape (groups must be a positive multiple of the matrices)");
   if (dtype != ML_F32 && dtype != ML_BF16 && dtype != ML_F16)
@@ -181,7 +183,9 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     p.plane = ceil_div(out, 4) * 4;
     p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
   }
-  if (p.bound > INT32_MAX - 8) return fail(ML_EUNSUPPORTED, "grouped_matmul: too many tiles");
+  // ids are 32-bit; grouped_kernel has a workgroup to an item, and a launch fewer than 2^32 threads
+  if (p.bound > (p.tile >= kDeep128 ? (int64_t)INT32_MAX : (int64_t)UINT32_MAX / 256) - 8)
+    return fail(ML_EUNSUPPORTED, "grouped_matmul: too many tiles");
   return ML_OK;
 }
 

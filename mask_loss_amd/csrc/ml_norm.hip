@@ -579,12 +579,15 @@ int norm_backward(const void* g, const void* x, const void* w, int pf32, const f
   return check_launch("layer_norm_backward");
 }
 
+constexpr int64_t kNormWidth = (int64_t)1 << 26;
+
 int norm_check(int dtype, int pdtype, int64_t rows, int64_t width) {
   if (dtype != ML_F32 && dtype != ML_BF16 && dtype != ML_F16) return fail(ML_EINVAL, "layer_norm: unsupported dtype");
   if (pdtype != dtype && pdtype != ML_F32)
     return fail(ML_EINVAL, "layer_norm: weight and bias must have the input's dtype or be float32");
   if (rows < 0 || width <= 0) return fail(ML_EINVAL, "layer_norm: rows must not be negative, width must be positive");
-  if (width > INT32_MAX || (rows > 0 && width > INT64_MAX / 8 / rows))
+  // norm_param_kernel takes 32 threads a column, a launch fewer than 2^32
+  if (width > kNormWidth || (rows > 0 && width > INT64_MAX / 8 / rows))
     return fail(ML_EUNSUPPORTED, "layer_norm: too many elements");
   return ML_OK;
 }

@@ -446,3 +446,59 @@ def test_head_and_matching_together(dt):
                             (w.grad, (g64 * hat).sum(0), (g64 * hat).abs().sum(0)),
                             (b.grad, g64.sum(0), g64.abs().sum(0))):
         check(got.reshape(want.shape), want, size, 64, "norm")
+
+
+# ---- offsets past 32 bits ---------------------------------------------------------
+@pytest.mark.parametrize("K", [264, 265])
+def test_rows_past_32_bits(K):
+    """2.2e9 elements of input and d input, rows at both ends of them that are not zero."""
+    from mask_loss_amd.functions import grouped_matmul
+    R, N = (1 << 23) + 300, 16
+    keep = torch.cat([torch.arange(5), torch.arange(R - 200, R)])
+    xs, w, dys = make(205, K, N, 2, "bf16", False, 40)
+    x = torch.zeros(R, K, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(R, N, dtype=torch.bfloat16, device="cuda")
+    x[keep.cuda()], dy[keep.cuda()] = xs.cuda(), dys.cuda()
+    leaves = [x.requires_grad_(True), w.cuda().requires_grad_(True)]
+    y = grouped_matmul(*leaves, torch.tensor([0, 5, R - 200, R - 100, R]).cuda())
+    dx, dw = torch.autograd.grad(y, leaves, dy)
+    ref = reference(xs, w, dys, [0, 5, 5, 105, 205], False)
+    for got, r, name in zip((y.detach()[keep.cuda()], dx[keep.cuda()], dw), ref, ("y", "dx", "dw")):
+        check(got, *r, name)
+    assert not bool(y[5:R - 200].any()) and not bool(dx[5:R - 200].any())
+
+
+def test_matrices_past_32_bits():
+    """2.5e9 elements of weight and d weight, the last matrix in use."""
+    from mask_loss_amd.functions import grouped_matmul
+    M, K = 600, 2048
+    x, w1, dy = make(6, K, K, 1, "bf16", False, 41)
+    w = torch.zeros(M, K, K, dtype=torch.bfloat16, device="cuda")
+    w[-1] = w1[0].cuda()
+    offsets = torch.zeros(M + 1, dtype=torch.int64)
+    offsets[-1] = 6
+    leaves = [x.cuda().requires_grad_(True), w.requires_grad_(True)]
+    y = grouped_matmul(*leaves, offsets.cuda())
+    dx, dw = torch.autograd.grad(y, leaves, dy.cuda())
+    ref = reference(x, w1, dy, [0, 6], False)
+    for got, r, name in zip((y.detach(), dx, dw[-1:]), ref, ("y", "dx", "dw")):
+        check(got, *r, name)
+    assert not bool(dw[:-1].any())
+
+
+def test_logits_past_32_bits():
+    """2.2e9 logits of one image: the last queries' and the gradients from theirs."""
+    from mask_loss_amd.functions import mask_logits
+    Q, C, H, W, n = 33000, 16, 256, 256, 40
+    q = torch.randn(Q, C, generator=torch.Generator().manual_seed(42)).bfloat16()
+    _, f, dz = make(n, C, H * W, 1, "bf16", False, 43)
+    leaves = [q.view(1, 1, Q, C).cuda().requires_grad_(True), f.view(1, C, H, W).cuda().requires_grad_(True)]
+    z = mask_logits(*leaves)
+    g = torch.zeros_like(z)
+    g[0, 0, -n:] = dz.view(n, H, W).cuda()
+    dq, df = torch.autograd.grad(z, leaves, g)
+    (zv, zs, zn), (qv, qs, qn), (fv, fs, fn) = reference(q[-n:], f, dz, [0, n], False)
+    check(z.detach()[0, 0, -n:].flatten(1), zv, zs, zn, "z")
+    check(dq[0, 0, -n:], qv, qs, qn, "dq")
+    check(df.flatten(2), fv, fs, fn, "df")
+    assert not bool(dq[0, 0, :-n].any())

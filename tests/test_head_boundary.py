@@ -60,6 +60,7 @@ def test_layer_norm_refusals(lib):
     refused(lib, norm(lib, mean=PTR), EINVAL, "mean and rstd go together")
     refused(lib, norm(lib, rows=1 << 40, width=1 << 30), EUNSUPPORTED, "too many elements")
     refused(lib, norm(lib, width=1 << 32), EUNSUPPORTED, "too many elements")
+    refused(lib, norm(lib, width=(1 << 26) + 1), EUNSUPPORTED, "too many elements")
     assert norm(lib, rows=0, x=None, y=None) == 0  # nothing to do
 
 
@@ -116,6 +117,10 @@ def test_grouped_refusals(lib, name):
     assert size_of(lib, product=product, **long) > 256
     refused(lib, grouped(lib, name, ws=None, **long), EWORKSPACE, "workspace too small")
     refused(lib, grouped(lib, name, bytes=255, **long), EWORKSPACE, "workspace too small")
+    # 4,000 groups of a row or matrices of a row by 32,768 column tiles: past a launch's 2^32 threads
+    many = {"forward": dict(rows=4000, K=1, N=1 << 22), "backward_input": dict(rows=4000, K=1 << 22, N=1),
+            "backward_weight": dict(rows=4000, K=1, N=1 << 22)}[name]
+    refused(lib, grouped(lib, name, groups=4000, matrices=4000, **many), EUNSUPPORTED, "too many tiles")
     assert grouped(lib, name, K=0, N=0, x=None, w=None, out=None) == 0  # nothing to write
 
 
