@@ -850,13 +850,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
     const int tn = a.N - n0;
     const bool full = tm >= BM && tn >= BN && block < 0;
     const int64_t origin = (WG ? (int64_t)iw * a.cstride : 0) + n0;
-    const int mr = wm + (lane & 15), g = lane >> 4;
+    // (not known to the compiler as the same for every tile: it would keep what follows from it in
+    // registers, 10 more of them and spilled ones on the 256 x 256 tile)
+    int el = lane;
+    asm("" : "+v"(el));
+    const int mr = wm + (el & 15), g = el >> 4;
     auto row_start = [&](int j) {  // of the lane's row in row tile j
       const int r = mr + 16 * j;
       return origin + (int64_t)(mapped ? merged_row(a, e, iw, m0 + min(r, tm - 1)) : m0 + r) * a.ldc;
     };
     if (block >= 0) {  // in the order of the registers (grouped_tail_kernel)
-      f32x4_t* c = (f32x4_t*)a.parts + ((int64_t)(xcd * turns + block) * NW + wave) * (TN * TM * 64) + lane;
+      f32x4_t* c = (f32x4_t*)a.parts + ((int64_t)(xcd * turns + block) * NW + wave) * (TN * TM * 64) + el;
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll

@@ -8,13 +8,15 @@
 //                                      forward  d in    d in     forward d weight d weight
 //   128 x 128, 2 stages of 128 bytes   160      195      191      289     266      287
 //   128 x 256, 3 stages of 64 bytes    182      248     172      278     211      238
-//   256 x 256, 4 stages of 64 bytes    180      233     217      245     193      220
+//   256 x 256, 4 stages of 64 bytes    196      227     166      241     187      220
+//   256 x 256, 2 stages of 128 bytes   187      203     157      247     189      227
 //   grouped_kernel, 128 x 128          229      229     258      402     315      380
 //
 // (experts: 16,384 rows in 16 groups, K = 1,024, N = 4,096; masks: 16 groups of 200 rows, K = 256,
 // N = 65,536; bf16.)  Where both operands' reduced index is contiguous, 128-byte stages read whole
 // HBM lines and win; operands by rows are whole lines anyway, and the larger tiles read LDS less
-// often.  (256 x 256 by 4 waves of 128 x 128 instead of 8 of 128 x 64: masks forward 252, d weight 216,
+// often, in stages of 128 bytes (128 matrix instructions of a SIMD to a barrier, not 64) unless both
+// operands are by rows.  (64-byte stages, 4 waves of 128 x 128 instead of 8 of 128 x 64: masks forward 252, d weight 216,
 // experts d weight 199.)  The masks' d input varies from machine to machine, 194 to 237 with the same
 // code: rows 128 KiB apart.  The choice also weighs how the tiles fill the compute units (grouped_plan).
 #include <algorithm>
@@ -219,7 +221,8 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
       break;
     case kDeep256:
       if constexpr (DT != ML_F32)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 4, 64, 4, 1>), grid, dim3(512), lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 4, WG ? 64 : 128, WG ? 4 : 2, 1>), grid, dim3(512),
+                           lds, st, a);
       break;
   }
   int rc = check_launch("grouped_matmul");
