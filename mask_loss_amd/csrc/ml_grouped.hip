@@ -120,35 +120,43 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
   auto tiles_of = [&](Tile t) {
     const double x = each / kTiles[t].bm;
     const double mt = wg ? (double)s->matrices * ceil_div(p.m, kTiles[t].bm)
-                         : used * (equal || x <= 1.0 ? std::ceil(x) : x + 0.5);
+                         : used * (equal || segments == 1 ? std::ceil(x) : std::max(1.05, x + 0.5));
     return std::max(1.0, mt * ceil_div(p.n, kTiles[t].bn));
   };
   // Rough time in us of a round of the persistent workgroups, and of all rounds, the last one in parts
   // (ring_share), whose join takes kJoin.
   constexpr double kJoin = 10.0;
   const double unit = dtype == ML_F32 ? 1.75 : 0.5;  // a step of 128 x 128 outputs on one compute unit
-  auto round = [&](Tile t) { return kTiles[t].bm * kTiles[t].bn * kTiles[t].occ / 16384.0 * (steps + 4.0) * unit; };
+  auto round = [&](Tile t) { return kTiles[t].bm * kTiles[t].bn * kTiles[t].occ / 16384.0 * (steps + 3.0) * unit; };
   // a last round that leaves half of the workgroups without work, alone on their compute units then
   auto last = [&](Tile t) { return kTiles[t].occ > 1 ? 0.55 : 1.0; };
   auto fewest_parts = [&](Tile t) {  // it less 1 / parts of a round saved, for more than a join
     const double h = last(t) - kJoin / round(t);
     return h > 0.02 ? std::max(2, (int)std::ceil(1.0 / h)) : 1 << 30;
   };
-  // parts of the last round's tiles that are to be expected, 1 for none
-  auto expected_parts = [&](Tile t, double& whole) {
+  // parts of the last round's tiles that are to be expected, 1 for none; `more` rounds than the mean number
+  auto expected_parts = [&](Tile t, double& whole, double more) {
     const double rounds = tiles_of(t) / (kUnits * kTiles[t].occ);
     whole = std::floor(rounds + 0.02);
-    const double rest = rounds - whole;
+    const double rest = rounds - whole + (whole > 0.0 ? more : 0.0);
     if (whole > 0.0 && rest < 0.02) return 0;
     const int parts = (int)std::min<double>(whole > 0.0 ? std::min(most, kTailParts) : most, 1.0 / rest + 0.02);
     return parts < (whole > 0.0 ? fewest_parts(t) : 2) ? 1 : parts;
   };
-  auto cost = [&](Tile t, double factor) {
+  // Their products, or the time that the tensors take at the rate of a copy, and the parts' way through
+  // memory.  Ragged groups may make more tiles than the mean, and one too many costs a part of the last round's;
+  // the longest one's weight gradient is waited for.
+  const double bytes = ((double)s->rows * (s->K + s->N) + (double)s->matrices * s->K * s->N) * es;
+  auto cost = [&](Tile t, double products, double copies) {
     double whole;
-    const int parts = expected_parts(t, whole);
+    const bool ragged = !equal && segments > 1;
+    const int parts = expected_parts(t, whole, ragged && !wg ? 0.05 : 0.0);
     const double rest = tiles_of(t) / (kUnits * kTiles[t].occ) - whole;
     const double tail = parts == 0 ? 0.0 : parts > 1 ? 1.0 / parts : rest <= 0.5 ? last(t) : 1.0;
-    return (whole + tail) * round(t) * factor + (parts > 1 ? kJoin : 0.0);
+    const double wait = ragged && wg ? 0.4 : 0.0;
+    const double planes = parts * rest * kUnits * kTiles[t].occ * kTiles[t].bm * kTiles[t].bn * 4.0;
+    return std::max((whole + tail + wait) * round(t) * products, bytes / 5.2e6 * copies) +
+           (parts > 1 ? 4.0 + planes / 2.5e6 : 0.0);
   };
   if (!wg && each <= 32.0) {
     p.tile = kFew;
@@ -158,12 +166,15 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     p.tile = wg ? kDeep128 : kWide128;
   } else {
     const int rowops = wg ? 2 : (which == kForward) == transposed ? 0 : 1;  // operands by rows of the reduced index
-    // by the table above, per tile area
-    constexpr double f[3][3] = {{1.0, 1.05, 1.1}, {1.1, 1.0, 0.95}, {1.3, 1.0, 0.92}};
+    // by the tables above: bound by products (per tile area), by HBM.  Over 39 ragged and whole products
+    // of 1,000 to 32,768 rows, the calls take 1.00 to 1.01 times what the best of the three tiles takes,
+    // 1.14 at most (16 groups, K = 4,096 contiguous in both, N = 1,024); by products alone 1.08 and 1.5.
+    constexpr double f[3][3] = {{1.0, 1.05, 0.9}, {1.1, 1.02, 0.9}, {1.3, 1.0, 0.92}};
+    constexpr double h[3][3] = {{1.05, 1.33, 1.1}, {1.55, 1.47, 1.33}, {1.56, 1.29, 1.2}};
     const Tile ts[3] = {kWide128, kDeep128x256, kDeep256};
     double best = 0.0;
     for (int i = 0; i < 3; ++i) {
-      const double c = cost(ts[i], f[rowops][i]);
+      const double c = cost(ts[i], f[rowops][i], h[rowops][i]);
       if (i && c >= best) continue;
       best = c;
       p.tile = ts[i];
@@ -174,7 +185,7 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
   const int64_t tiles = mt * ceil_div(p.n, T.bn);
   if (p.tile >= kDeep128) {
     double whole;
-    p.splits = expected_parts(p.tile, whole) > 1 ? most : 1;  // (the counts on the GPU decide)
+    p.splits = expected_parts(p.tile, whole, 0.0) > 1 ? most : 1;  // (the counts on the GPU decide)
     p.fewest = fewest_parts(p.tile);
     p.bound = tiles;
     p.bytes = p.splits > 1 ? (size_t)kUnits * T.occ * T.bm * T.bn * sizeof(float) : 256;
