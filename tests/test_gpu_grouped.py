@@ -127,6 +127,27 @@ def test_long_reductions(dt, transposed):
     compare(x, w, dy, [0, 5990], transposed)
 
 
+# (rows, K, N, groups, matrices) whose products take the tiles of 128 x 256 and 256 x 256, whole and in parts,
+# with groups that share a matrix or not; the last one's d input leaves a round of 256 x 256 tiles an eighth full
+LARGE = [(1500, 64, 4104, 5, 5), (1500, 64, 4104, 10, 5), (300, 5120, 512, 5, 5), (300, 512, 5120, 20, 5),
+         (3000, 64, 4104, 5, 5), (3000, 64, 4104, 12, 3), (1100, 6400, 64, 3, 3), (1500, 64, 5120, 8, 2),
+         (300, 264, 8240, 10, 5), (3000, 64, 5120, 4, 1), (300, 520, 4096, 10, 5), (16384, 1024, 4096, 16, 16)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_tiles(dt, transposed, shape):
+    rows, K, N, G, M = shape
+    counts = np.random.default_rng(rows + G).multinomial(rows - 3, np.ones(G) / G)
+    x, w, dy = make(rows, K, N, M, dt, transposed, G)
+    got = run(x, w, dy, offsets_of(counts, 1), transposed)
+    with torch.device("cuda"):
+        ref = reference(x.cuda(), w.cuda(), dy.cuda(), offsets_of(counts, 1), transposed)
+    for g, (v, size, n), name in zip(got, ref, ("y", "dx", "dw")):
+        check(g, v.cpu(), size.cpu(), n, name)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_many_groups(dt):
     rng = np.random.default_rng(0)
