@@ -97,11 +97,11 @@ struct GMma<ML_F16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    // as the compiler's own conversion (round to nearest even), which it would move away from
-    // the store, one accumulator after another into spilled registers
-    uint32_t v;
-    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(v) : "v"(a), "v"(b));
-    return v;
+    // (by the compiler, which puts the wait states between a matrix instruction and its result's first
+    // reader; it does not look into assembly)
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    f32x2_t f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, h2));
   }
 };
 template <>
