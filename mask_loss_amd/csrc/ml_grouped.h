@@ -581,14 +581,31 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
 // barrier.
 static __device__ __align__(16) unsigned char g_zeros[16];  // the reduced index past its end
 
-// 16 bytes from base + off, or from p, of each lane to LDS at `lds` + 16 lane.  (m0 is no
-// register of the compiler's: where it needs one it sets it itself.)
-__device__ __forceinline__ void ring_load(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds), "v"(off), "s"(base)
-               : "memory");
+// N loads of 16 bytes from base + off[i] of each lane to LDS at `lds` + 1024 i + 16 lane.  (m0 is no
+// register of the compiler's: where it needs one it sets it itself.)  base may come right from a
+// vector instruction (uniform()): five wait states until a load reads it, which the compiler does not
+// put in front of assembly; once for all N (in front of each, the masks' d input took 201 us for 196).
+template <int N>
+__device__ __forceinline__ void ring_loads(const char* base, const uint32_t (&off)[N], uint32_t lds) {
+  static_assert(N == 2 || N == 4, "loads of an operand");
+  if constexpr (N == 2)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+        :
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
+        : "memory", "scc");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5"
+        :
+        : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
+        : "memory", "scc");
 }
+// 16 bytes from p of each lane to LDS at `lds` + 16 lane.
 __device__ __forceinline__ void ring_load(const char* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
@@ -664,9 +681,7 @@ struct RingOperand : Operand<DT, KC, R, 64 * NW, SB> {
   // base: the stage's first element; kleft: valid reduced indices from there on
   __device__ __forceinline__ void load(const char* base, int kleft, uint32_t lds, int wave) const {
     if (kleft >= O::BK) {
-      const char* b = uniform(base);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) ring_load(b, off[i], lds + (wave * PER + i) * 1024);
+      ring_loads(uniform(base), off, lds + wave * PER * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {

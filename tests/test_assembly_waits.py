@@ -24,6 +24,13 @@ __device__ void pack(const u32x4_t* in, uint32_t* out) {
 }
 extern "C" __global__ void pack_f16(const u32x4_t* in, uint32_t* out) { pack<ML_F16>(in, out); }
 extern "C" __global__ void pack_bf16(const u32x4_t* in, uint32_t* out) { pack<ML_BF16>(in, out); }
+extern "C" __global__ void load_base(const char* const* in, float* out) {
+  __shared__ __align__(1024) unsigned char lds[2048];
+  const uint32_t off[2] = {threadIdx.x * 16u, threadIdx.x * 16u + 1024u};
+  ring_loads(uniform(in[threadIdx.x]), off, (uint32_t)(uintptr_t)(lds_void_t*)lds);
+  ring_wait<0>();
+  out[threadIdx.x] = ((const float*)lds)[threadIdx.x];
+}
 """
 
 
@@ -76,3 +83,10 @@ def test_matrix_results_are_waited_for(kernels):
     own = wait_states(kernels["pack_bf16"], "v_mfma", "v_")
     assert own > 0
     assert wait_states(kernels["pack_f16"], "v_mfma", "v_") >= own
+
+
+def test_scalar_bases_are_waited_for(kernels):
+    """A load's scalar base that a vector instruction wrote: five wait states."""
+    code = kernels["load_base"]
+    assert any(name.startswith("v_readfirstlane") for name, _ in code)
+    assert wait_states(code, "v_readfirstlane", "global_load_lds") >= 5
