@@ -581,10 +581,13 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
 // barrier.
 static __device__ __align__(16) unsigned char g_zeros[16];  // the reduced index past its end
 
-// N loads of 16 bytes from base + off[i] of each lane to LDS at `lds` + 1024 i + 16 lane.  (m0 is no
-// register of the compiler's: where it needs one it sets it itself.)  base may come right from a
+// N loads of 16 bytes from base + off[i] of each lane to LDS at `lds` + 1024 i + 16 lane.  m0 is no
+// register that the compiler allocates, and it warns that the clobber list cannot keep its value; with the
+// list, a value of its own in m0 (a message's, an index) is set again behind the loads.  base may come right from a
 // vector instruction (uniform()): five wait states until a load reads it, which the compiler does not
 // put in front of assembly; once for all N (in front of each, the masks' d input took 201 us for 196).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int N>
 __device__ __forceinline__ void ring_loads(const char* base, const uint32_t (&off)[N], uint32_t lds) {
   static_assert(N == 2 || N == 4, "loads of an operand");
@@ -594,7 +597,7 @@ __device__ __forceinline__ void ring_loads(const char* base, const uint32_t (&of
         "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
         :
         : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base)
-        : "memory", "scc");
+        : "memory", "m0", "scc");
   else
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %5\n\t"
@@ -603,15 +606,16 @@ __device__ __forceinline__ void ring_loads(const char* base, const uint32_t (&of
         "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %5"
         :
         : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base)
-        : "memory", "scc");
+        : "memory", "m0", "scc");
 }
 // 16 bytes from p of each lane to LDS at `lds` + 16 lane.
 __device__ __forceinline__ void ring_load(const char* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(p)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ const char* uniform(const char* p) {
   const uint64_t u = (uint64_t)(uintptr_t)p;
   return (const char*)(uintptr_t)((uint64_t)(uint32_t)uniform((int)(uint32_t)u) |

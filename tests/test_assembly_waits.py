@@ -31,6 +31,19 @@ extern "C" __global__ void load_base(const char* const* in, float* out) {
   ring_wait<0>();
   out[threadIdx.x] = ((const float*)lds)[threadIdx.x];
 }
+extern "C" __global__ void loads_between(const char* in, int n) {
+  __shared__ __align__(1024) unsigned char lds[4096];
+  const uint32_t at = (uint32_t)(uintptr_t)(lds_void_t*)lds, off[2] = {threadIdx.x * 16u, threadIdx.x * 16u + 1024u};
+  const uint32_t off4[4] = {off[0], off[1], off[0], off[1]};
+  __builtin_amdgcn_s_sendmsg(1, n);
+  ring_loads(in, off, at);
+  __builtin_amdgcn_s_sendmsg(1, n);
+  ring_loads(in, off4, at);
+  __builtin_amdgcn_s_sendmsg(1, n);
+  ring_load(in + off[0], at);
+  __builtin_amdgcn_s_sendmsg(1, n);
+  ring_wait<0>();
+}
 """
 
 
@@ -90,3 +103,14 @@ def test_scalar_bases_are_waited_for(kernels):
     code = kernels["load_base"]
     assert any(name.startswith("v_readfirstlane") for name, _ in code)
     assert wait_states(code, "v_readfirstlane", "global_load_lds") >= 5
+
+
+def test_loads_declare_m0(kernels):
+    """A value that the compiler keeps in m0 (a message's) is set again behind loads that use m0."""
+    held, messages = None, []
+    for name, ops in kernels["loads_between"]:
+        if ops[0] == "m0":
+            held = ops[1]
+        elif name == "s_sendmsg":
+            messages.append(held)
+    assert len(messages) == 4 and len(set(messages)) == 1
