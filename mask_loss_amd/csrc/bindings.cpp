@@ -902,6 +902,9 @@ std::vector<torch::Tensor> layer_norm_backward(const torch::Tensor& grad_out, co
                                                const torch::Tensor& mean, const torch::Tensor& rstd,
                                                bool need_input, bool need_weight, bool need_bias,
                                                bool params_f32) {
+  // params_f32 stands for a bias's dtype where there is no weight
+  TORCH_CHECK(!params_f32 || !weight.has_value() || weight->scalar_type() == torch::kFloat32,
+              "layer_norm: params_f32 needs a float32 weight");
   NormArgs a = norm_args(x, weight, c10::nullopt);
   if (params_f32) a.pdt = ML_F32;
   ML_CHECK_INPUT(grad_out);
