@@ -34,6 +34,14 @@ int dtype_code(const torch::Tensor& t, const char* name) {
   return -1;
 }
 
+// Forward-mode derivatives: a result would leave its inputs' tangents behind in silence.
+bool has_tangent(const torch::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const c10::optional<torch::Tensor>& t) { return t.has_value() && has_tangent(*t); }
+template <class... T>
+void no_tangent(const char* who, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), who, ": forward-mode derivatives are not provided");
+}
+
 void ml_ok(int rc) { TORCH_CHECK(rc == ML_OK, ml_last_error()); }
 
 ml_stream_t cur_stream() { return (ml_stream_t)at::hip::getCurrentHIPStream().stream(); }
@@ -884,6 +892,7 @@ const void* ptr_or_null(const c10::optional<torch::Tensor>& t) { return t.has_va
 std::vector<torch::Tensor> layer_norm_forward(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
                                               const c10::optional<torch::Tensor>& bias, double eps,
                                               bool want_stats) {
+  no_tangent("layer_norm", x, weight, bias);
   const NormArgs a = norm_args(x, weight, bias);
   TORCH_CHECK_VALUE(eps >= 0.0, "layer_norm: eps must not be negative");
   const c10::DeviceGuard guard(x.device());
@@ -902,6 +911,7 @@ std::vector<torch::Tensor> layer_norm_backward(const torch::Tensor& grad_out, co
                                                const torch::Tensor& mean, const torch::Tensor& rstd,
                                                bool need_input, bool need_weight, bool need_bias,
                                                bool params_f32) {
+  no_tangent("layer_norm backward", grad_out, x, weight, mean, rstd);
   // params_f32 stands for a bias's dtype where there is no weight
   TORCH_CHECK(!params_f32 || !weight.has_value() || weight->scalar_type() == torch::kFloat32,
               "layer_norm: params_f32 needs a float32 weight");
@@ -1037,6 +1047,7 @@ std::vector<int64_t> with_width(const torch::Tensor& x, int64_t width) {
 
 torch::Tensor grouped_matmul_forward(const torch::Tensor& x, const torch::Tensor& weight,
                                      const c10::optional<torch::Tensor>& offsets, bool transposed) {
+  no_tangent("grouped_matmul", x, weight);
   ML_CHECK_INPUT(x);
   ML_CHECK_INPUT(weight);
   const ml_grouped_shape s = grouped_shape(x, weight, offsets, transposed, false);
@@ -1051,6 +1062,7 @@ torch::Tensor grouped_matmul_forward(const torch::Tensor& x, const torch::Tensor
 
 torch::Tensor grouped_matmul_backward_input(const torch::Tensor& grad_out, const torch::Tensor& weight,
                                             const c10::optional<torch::Tensor>& offsets, bool transposed) {
+  no_tangent("grouped_matmul backward", grad_out, weight);
   ML_CHECK_INPUT(grad_out);
   ML_CHECK_INPUT(weight);
   const ml_grouped_shape s = grouped_shape(grad_out, weight, offsets, transposed, true);
@@ -1068,6 +1080,7 @@ torch::Tensor grouped_matmul_backward_input(const torch::Tensor& grad_out, const
 torch::Tensor grouped_matmul_backward_weight(const torch::Tensor& x, const torch::Tensor& grad_out,
                                              const c10::optional<torch::Tensor>& offsets, int64_t matrices,
                                              bool transposed) {
+  no_tangent("grouped_matmul backward", x, grad_out);
   ML_CHECK_INPUT(x);
   ML_CHECK_INPUT(grad_out);
   TORCH_CHECK(matrices >= 1, "grouped_matmul: at least one matrix");
@@ -1115,6 +1128,7 @@ torch::Tensor as_matrices(const torch::Tensor& f) { return f.view({f.size(0), f.
 
 torch::Tensor mask_logits_forward(const torch::Tensor& queries, const torch::Tensor& features,
                                   const c10::optional<torch::Tensor>& offsets) {
+  no_tangent("mask_logits", queries, features);
   const auto out = mask_shape(queries, features, offsets);
   ML_CHECK_INPUT(queries);
   ML_CHECK_INPUT(features);

@@ -4,7 +4,8 @@ of an expert or a class times its weights.  No counterpart in the reference, who
 operators start at the mask logits.
 
 Tensors are float32, bfloat16 or float16, input and weight alike; sums are float32
-and rounded once.  Gradients are not differentiable a second time."""
+and rounded once.  Gradients are not differentiable a second time, and forward-mode
+derivatives raise."""
 from __future__ import annotations
 
 import torch

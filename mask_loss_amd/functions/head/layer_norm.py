@@ -4,7 +4,8 @@ logits.  No counterpart in the reference, whose operators start at the logits.
 
 The output has the input's dtype (float32, bfloat16 or float16); weight and bias
 have that dtype or are float32, and their gradients come back in their own.  The
-statistics are float32.  Gradients are not differentiable a second time."""
+statistics are float32.  Gradients are not differentiable a second time, and
+forward-mode derivatives raise."""
 from __future__ import annotations
 
 import torch

@@ -11,7 +11,7 @@ import mask_loss
 
 def mask_logits(queries, features, offsets=None):
     """Products of every image's queries with its feature map, differentiable in both
-    (once): the products of ``grouped_matmul`` with an image as a group.
+    (once, in reverse mode): the products of ``grouped_matmul`` with an image as a group.
 
     ``features``: (B, C, H, W).  ``queries``: (L, B, Q, C), every query of L layers,
     giving (L, B, Q, H, W); or (R, C) with ``offsets`` (B + 1,), int64, a set of its own

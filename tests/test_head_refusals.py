@@ -12,3 +12,27 @@ def test_params_f32_needs_a_float32_weight(dtype):
     x, stat = torch.zeros(4, 8, dtype=dtype), torch.zeros(4)
     with pytest.raises(RuntimeError, match="float32 weight"):
         mask_loss_amd.mask_loss.layer_norm_backward(x, x, torch.ones(8, dtype=dtype), stat, stat, params_f32=True)
+
+
+def test_tangents_are_refused():
+    """A tensor that carries a tangent: every form raises, none leaves the tangent behind."""
+    import mask_loss_amd
+    from torch.autograd import forward_ad
+    from mask_loss_amd.functions import grouped_matmul, layer_norm, mask_logits
+    ml = mask_loss_amd.mask_loss
+    x, w, b, wg = torch.ones(4, 8), torch.ones(8), torch.zeros(8), torch.zeros(2, 8, 3)
+    o, stat, q, f = torch.tensor([0, 2, 4]), torch.zeros(4), torch.zeros(1, 2, 3, 8), torch.zeros(2, 8, 5, 5)
+    calls = [(layer_norm, (x, w, b), 3), (grouped_matmul, (x, wg, o), 2), (mask_logits, (q, f), 2),
+             (mask_logits, (x, f, o), 2), (ml.layer_norm_backward, (x, x, w, stat, stat), 5),
+             (ml.grouped_matmul_backward_input, (torch.ones(4, 3), wg, o), 2),
+             (ml.grouped_matmul_backward_weight, (x, torch.ones(4, 3), o, 2), 2)]
+    with forward_ad.dual_level():
+        for fn, args, n in calls:
+            for i in range(n):
+                for grad in (False, True):
+                    these = [t.clone() if torch.is_tensor(t) else t for t in args]
+                    these[i] = forward_ad.make_dual(these[i], torch.ones_like(these[i]))
+                    if grad:
+                        these[0].requires_grad_(True)
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(*these)
