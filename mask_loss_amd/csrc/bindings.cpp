@@ -550,6 +550,7 @@ void check_coords(const torch::Tensor& coords, const torch::Tensor& like) {
 // (N, C, H, W) planes at (N, P, 2) or (N, Hg, Wg, 2) points -> (N, C, P) or (N, C, Hg, Wg)
 torch::Tensor point_sample(const torch::Tensor& input, const torch::Tensor& coords,
                            bool align_corners) {
+  no_tangent("point_sample", input, coords);
   ML_CHECK_INPUT(input);
   check_coords(coords, input);
   TORCH_CHECK(input.dim() == 4, "point_sample: input must be (N,C,H,W)");
@@ -569,6 +570,7 @@ torch::Tensor point_sample(const torch::Tensor& input, const torch::Tensor& coor
 // gradient of point_sample with respect to its (N, C, H, W) input
 torch::Tensor point_sample_backward(const torch::Tensor& grad_out, const torch::Tensor& coords,
                                     int64_t H, int64_t W, bool align_corners) {
+  no_tangent("point_sample backward", grad_out, coords);
   ML_CHECK_INPUT(grad_out);
   check_coords(coords, grad_out);
   TORCH_CHECK(grad_out.dim() == 3 || grad_out.dim() == 4, "point_sample backward: grad must be (N,C,P) or (N,C,Hg,Wg)");

@@ -4,7 +4,8 @@
 * ``point_sample``: bilinear sampling with ``torch.nn.functional.grid_sample``
   semantics at coordinates in [0, 1] (grid = 2 * coords - 1), zero padding
   (functions/utils.py:12-20), differentiable with respect to the sampled
-  input (grid_sample's input gradient; the coordinates take no gradient).
+  input (grid_sample's input gradient; the coordinates take no gradient;
+  forward-mode derivatives raise).
 * ``calculate_uncertainty``: -|logit| (functions/utils.py:6-9).
 * ``get_uncertain_point_coords_with_randomness``: oversampled random points,
   the most uncertain ``importance_sample_ratio * num_points`` of them, plus

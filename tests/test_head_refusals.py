@@ -1,5 +1,5 @@
 """CPU checks of calls that the head's operators (layer norm, grouped products, mask logits) refuse or answer
-without the GPU, beside those of test_head_boundary.py."""
+without the GPU, beside those of test_head_boundary.py, and of point sampling's forward mode."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -36,3 +36,17 @@ def test_tangents_are_refused():
                         these[0].requires_grad_(True)
                     with pytest.raises(NotImplementedError, match="forward-mode"):
                         fn(*these)
+
+
+def test_point_sample_refuses_tangents():
+    import mask_loss_amd
+    from torch.autograd import forward_ad
+    from mask_loss_amd.functions import point_sample
+    x, c, g = torch.ones(2, 3, 4, 4), torch.zeros(2, 5, 2), torch.ones(2, 3, 5)
+    with forward_ad.dual_level():
+        for fn, args in ((point_sample, (x, c)), (mask_loss_amd.mask_loss.point_sample_backward, (g, c, 4, 4, False))):
+            for i in (0, 1):
+                these = list(args)
+                these[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(*these)
