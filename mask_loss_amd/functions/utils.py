@@ -60,7 +60,7 @@ def point_sample(input, point_coords, **kwargs):
         raise TypeError(f"point_sample: unexpected arguments {sorted(kwargs)}")
     if point_coords.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("point_sample: no gradient with respect to the coordinates")
-    coords = point_coords.detach().to(dtype=torch.float32).contiguous()
+    coords = point_coords.to(dtype=torch.float32).contiguous()
     if input.requires_grad and torch.is_grad_enabled():
         return PointSampleFunction.apply(input.contiguous(), coords, align)
     return mask_loss.point_sample(input.contiguous(), coords, align)
