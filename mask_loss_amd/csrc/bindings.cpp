@@ -980,6 +980,7 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     const auto sv = ctx->get_saved_variables();
     c10::optional<torch::Tensor> w;
     if (sv[1].defined()) w = sv[1];
+    no_tangent("layer_norm backward", g[0]);  // (detaching drops it)
     // only tensors that were given count as inputs of the node
     const bool need_w = w.has_value() && ctx->needs_input_grad(1);
     const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.has_value() ? 2 : 1);
@@ -1163,6 +1164,7 @@ struct GroupedNode : public torch::autograd::Function<GroupedNode> {
     if (sv[2].defined()) o = sv[2];
     const int64_t form = ctx->saved_data["form"].toInt();
     const bool transposed = form & 1, maps = form & 2;
+    no_tangent(maps ? "mask_logits backward" : "grouped_matmul backward", g[0]);  // (detaching drops it)
     auto gy = g[0].detach().contiguous();
     torch::Tensor dx, dw;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
