@@ -1138,6 +1138,16 @@ torch::Tensor mask_logits_forward(const torch::Tensor& queries, const torch::Ten
   int64_t n = 1;
   for (const int64_t d : out) n *= d;
   if (n == 0 && !offsets.has_value()) return torch::empty(out, queries.options());  // perhaps no group
+  if (features.size(0) == 0) {  // offsets (1,), no group: every row is in no image's set
+    ML_CHECK_INPUT(*offsets);
+    TORCH_CHECK(offsets->scalar_type() == torch::kLong, "offsets must be int64");
+    TORCH_CHECK(queries.scalar_type() == features.scalar_type(),
+                "grouped_matmul: input and weight must have the same dtype");
+    TORCH_CHECK(queries.device() == features.device() && queries.device() == offsets->device(),
+                "all tensors must be on the same device");
+    dtype_code(queries, "input");
+    return torch::zeros(out, queries.options());
+  }
   return grouped_matmul_forward(as_groups(queries, queries.size(-1), offsets.has_value()), as_matrices(features),
                                 offsets, false)
       .view(out);
@@ -1168,7 +1178,7 @@ struct GroupedNode : public torch::autograd::Function<GroupedNode> {
     auto gy = g[0].detach().contiguous();
     torch::Tensor dx, dw;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
-    if (maps && gy.numel() == 0) {
+    if (maps && (gy.numel() == 0 || w.size(0) == 0)) {  // perhaps no group
       if (need_x) dx = torch::zeros_like(x);
       if (need_w) dw = torch::zeros_like(w);
     } else {

@@ -28,3 +28,21 @@ def test_upstream_gradients_with_tangents_are_refused():
                 torch.autograd.grad(y, leaf, dy)
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 fn(forward_ad.make_dual(args[0], args[0]), *args[1:])
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_mask_logits_of_no_image(rows):
+    """A ragged set for an empty batch: rows in no image's set give zeros."""
+    from mask_loss_amd.functions import mask_logits
+    q = torch.randn(rows, 8, device="cuda", requires_grad=True)
+    f = torch.zeros(0, 8, 4, 6, device="cuda", requires_grad=True)
+    o = torch.zeros(1, dtype=torch.int64, device="cuda")
+    z = mask_logits(q, f, o)
+    assert z.shape == (rows, 4, 6) and not z.any()
+    dq, df = torch.autograd.grad(z, (q, f), torch.ones_like(z))
+    assert dq.shape == q.shape and not dq.any() and df.shape == f.shape
+    with torch.no_grad():
+        assert torch.equal(mask_logits(q, f, o), z)
+        for bad, words in (((q, f, o.int()), "int64"), ((q, f.half(), o), "same dtype"), ((q, f, o.cpu()), "CUDA tensor")):
+            with pytest.raises(RuntimeError, match=words):
+                mask_logits(*bad)
