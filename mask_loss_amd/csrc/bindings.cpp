@@ -9,6 +9,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <chrono>
@@ -958,6 +959,31 @@ torch::autograd::variable_list once(torch::autograd::variable_list g, const char
   return g;
 }
 
+// A node made in a captured call hands its gradients to the nodes of its inputs.  One of those that was made
+// on the default stream before (a leaf's, while an output of an eager call is alive) is waited for there, which
+// a capture does not survive: the process ends.  Bit i: input i of a captured call has such a node.
+int64_t eager_edges(std::initializer_list<const torch::Tensor*> inputs) {
+  const auto stream = at::hip::getCurrentHIPStream();
+  if (stream.id() == 0) return 0;  // the default stream is not captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return 0;
+  int64_t bits = 0;
+  int i = 0;
+  for (const torch::Tensor* t : inputs) {
+    if (t->defined() && t->requires_grad()) {
+      const auto node = torch::autograd::impl::gradient_edge(*t).function;
+      const auto at = node ? node->stream() : std::nullopt;
+      if (at.has_value() && at->id() == 0) bits |= (int64_t)1 << i;
+    }
+    ++i;
+  }
+  return bits;
+}
+void no_eager_edge(const char* who, int64_t edges, int input, bool wanted) {
+  TORCH_CHECK(!wanted || !(edges >> input & 1), who, ": this backward cannot be captured, as an autograd graph that was "
+              "made on the default stream holds an input's gradient; delete the outputs of earlier calls first");
+}
+
 struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input,
                                const c10::optional<torch::Tensor>& weight,
@@ -973,6 +999,9 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     const auto& p = w.has_value() ? w : b;
     ctx->saved_data["params_f32"] = p.has_value() && p->scalar_type() == torch::kFloat32;
     ctx->saved_data["bias"] = b.has_value();
+    const torch::Tensor none;
+    ctx->saved_data["edges"] =
+        eager_edges({&input, weight.has_value() ? &*weight : &none, bias.has_value() ? &*bias : &none});
     return r[0];
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -984,6 +1013,10 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     // only tensors that were given count as inputs of the node
     const bool need_w = w.has_value() && ctx->needs_input_grad(1);
     const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(w.has_value() ? 2 : 1);
+    const int64_t edges = ctx->saved_data["edges"].toInt();
+    no_eager_edge("layer_norm", edges, 0, ctx->needs_input_grad(0));
+    no_eager_edge("layer_norm", edges, 1, need_w);
+    no_eager_edge("layer_norm", edges, 2, need_b);
     const auto r = layer_norm_backward(g[0].detach().contiguous(), sv[0], w, sv[2], sv[3], ctx->needs_input_grad(0),
                                        need_w, need_b, ctx->saved_data["params_f32"].toBool());
     return once({r[0], r[1], r[2], torch::Tensor()}, "the backward of layer_norm cannot be differentiated");
@@ -1163,7 +1196,7 @@ struct GroupedNode : public torch::autograd::Function<GroupedNode> {
     if (offsets.has_value()) o = offsets->contiguous();
     auto y = maps ? mask_logits_forward(x, w, o) : grouped_matmul_forward(x, w, o, transposed);
     ctx->save_for_backward({x, w, o.has_value() ? *o : torch::Tensor()});
-    ctx->saved_data["form"] = (int64_t)(transposed ? 1 : 0) | (maps ? 2 : 0);
+    ctx->saved_data["form"] = (int64_t)(transposed ? 1 : 0) | (maps ? 2 : 0) | eager_edges({&input, &weight}) << 2;
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -1178,6 +1211,8 @@ struct GroupedNode : public torch::autograd::Function<GroupedNode> {
     auto gy = g[0].detach().contiguous();
     torch::Tensor dx, dw;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    no_eager_edge(maps ? "mask_logits" : "grouped_matmul", form >> 2, 0, need_x);
+    no_eager_edge(maps ? "mask_logits" : "grouped_matmul", form >> 2, 1, need_w);
     if (maps && (gy.numel() == 0 || w.size(0) == 0)) {  // perhaps no group
       if (need_x) dx = torch::zeros_like(x);
       if (need_w) dw = torch::zeros_like(w);

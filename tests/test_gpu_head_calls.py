@@ -46,3 +46,53 @@ def test_mask_logits_of_no_image(rows):
         for bad, words in (((q, f, o.int()), "int64"), ((q, f.half(), o), "same dtype"), ((q, f, o.cpu()), "CUDA tensor")):
             with pytest.raises(RuntimeError, match=words):
                 mask_logits(*bad)
+
+
+def operator(name):
+    """(call, leaves, upstream gradient) of a small training call"""
+    from mask_loss_amd.functions import grouped_matmul, layer_norm, mask_logits
+    gen = torch.Generator().manual_seed(3)
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=gen).bfloat16().cuda().requires_grad_(True)
+
+    if name == "layer_norm":
+        return layer_norm, [leaf(40, 64), leaf(64), leaf(64)], torch.ones(40, 64, device="cuda").bfloat16()
+    if name == "mask_logits":
+        return mask_logits, [leaf(2, 2, 5, 64), leaf(2, 64, 8, 8)], torch.ones(2, 2, 5, 8, 8, device="cuda").bfloat16()
+    o = torch.tensor([0, 30, 40], device="cuda")
+    return (lambda x, w: grouped_matmul(x, w, o)), [leaf(40, 64), leaf(2, 64, 72)], torch.ones(40, 72, device="cuda").bfloat16()
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "grouped_matmul", "mask_logits"])
+def test_captured_backward_beside_an_eager_graph(name):
+    """While an eager call's output is alive its leaves' gradients belong to the default stream: a captured
+    backward into one of them is refused, the captured forward is not, and both work when it is gone."""
+    fn, leaves, dy = operator(name)
+    want = fn(*leaves)
+    want_grads = torch.autograd.grad(want, leaves, dy, retain_graph=True)
+    torch.cuda.synchronize()
+    for i in range(len(leaves)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = fn(*leaves)
+            with pytest.raises(RuntimeError, match="cannot be captured"):
+                torch.autograd.grad(y, leaves[i], dy)
+        for _ in range(2):
+            y.detach().zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+        del y, graph
+    value = want.detach().clone()
+    del want  # the eager graph and its nodes
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fn(*leaves)
+        grads = torch.autograd.grad(y, leaves, dy)
+    for _ in range(3):
+        for t in (y.detach(), *grads):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, value) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
