@@ -391,6 +391,18 @@ typedef struct ml_grouped_shape {
 } ml_grouped_shape;
 enum { ML_GROUPED_FORWARD = 0, ML_GROUPED_BACKWARD_INPUT = 1, ML_GROUPED_BACKWARD_WEIGHT = 2 };
 size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, int dtype, int product);
+/* What a call launches, from the host's arguments alone (no GPU needed): for tests and for reading timings.
+ * `aligned`: rows on 16-byte boundaries (K and N whole 16-byte chunks, both operands' addresses too);
+ * `equal`: offsets NULL.  tile_rows x tile_columns outputs to a workgroup.  ring: 1 for persistent
+ * workgroups (`workgroups` of them, on 8 XCDs in turn) with LDS stages of stage_bytes of the reduced index,
+ * 0 for one workgroup per tile and part.  parts: the most parts of a tile's reduction, 1 for whole tiles;
+ * with ring the tiles of the last round alone, where the groups' sizes leave few enough of them: at least
+ * fewest_parts (2 where there is no other round).  merged: groups that share a matrix make tiles together. */
+typedef struct ml_grouped_plan {
+  int32_t tile_rows, tile_columns, ring, stage_bytes, workgroups, parts, fewest_parts, merged;
+} ml_grouped_plan;
+int ml_grouped_matmul_plan(const ml_grouped_shape* s, int dtype, int product, int transposed, int aligned,
+                           int equal, ml_grouped_plan* plan);
 int ml_grouped_matmul_forward(const ml_grouped_shape* s, int dtype, const void* x, const void* weight,
                               int transposed, const int64_t* offsets, void* y, void* workspace,
                               size_t workspace_bytes, ml_stream_t stream);

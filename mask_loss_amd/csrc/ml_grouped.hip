@@ -72,6 +72,9 @@ struct TileShape {
 };
 constexpr TileShape kTiles[] = {{32, 128, 4}, {128, 128, 2}, {128, 128, 2}, {128, 128, 2}, {128, 256, 2}, {256, 256, 1}};
 
+// bytes of the reduced index in an LDS stage of the ring's tiles
+constexpr int stage_bytes(Tile t, bool wg) { return t == kWide128 || (t == kDeep256 && !wg) ? 128 : 64; }
+
 struct GroupedPlan {
   Tile tile;
   int splits, fewest;
@@ -202,6 +205,12 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
   return ML_OK;
 }
 
+// one workgroup to an item (rounded up for xcd_item), or persistent ones: all that fit where tiles may be split
+int64_t grouped_blocks(const GroupedPlan& p) {
+  const int64_t items = ceil_div(p.bound, kXcds) * kXcds, slots = kUnits * kTiles[p.tile].occ;
+  return p.tile < kDeep128 ? items : p.splits > 1 ? slots : std::min(items, slots);
+}
+
 template <int DT, bool WG, bool BKC>
 int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
   const TileShape& T = kTiles[p.tile];
@@ -209,10 +218,8 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
   a.layers = fast_div(a.groups / a.matrices);
   a.mtiles = fast_div(WG ? ceil_div(a.M, T.bm) : 1);
   const size_t lds = (2 * (size_t)a.groups + 3) * sizeof(int);  // edges, tiles of the segments
-  // one workgroup to an item (rounded up for xcd_item), or persistent ones: all that fit where tiles may be split
   const bool ring = p.tile >= kDeep128;
-  const int64_t items = ceil_div(p.bound, kXcds) * kXcds, slots = kUnits * T.occ;
-  const dim3 grid((unsigned)(!ring ? items : a.splits > 1 ? slots : std::min(items, slots))), blk(256);
+  const dim3 grid((unsigned)grouped_blocks(p)), blk(256);
   switch (p.tile) {
     case kFew:
       if constexpr (!WG) hipLaunchKernelGGL((grouped_kernel<DT, false, BKC, 32, 128, 1, 4>), grid, blk, lds, st, a);
@@ -220,20 +227,20 @@ int grouped_launch(const GroupedPlan& p, GroupedArgs& a, hipStream_t st) {
     case kPlain: hipLaunchKernelGGL((grouped_kernel<DT, WG, BKC, 128, 128, 2, 2>), grid, blk, lds, st, a); break;
     case kDeep128:
       if constexpr (DT == ML_F32 && WG)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, 64, 4, 2>), grid, blk, lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, stage_bytes(kDeep128, WG), 4, 2>), grid, blk, lds, st, a);
       break;
     case kWide128:
       if constexpr (DT != ML_F32 || !WG)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, 128, 2, 2>), grid, blk, lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 128, 2, 2, stage_bytes(kWide128, WG), 2, 2>), grid, blk, lds, st, a);
       break;
     case kDeep128x256:
       if constexpr (DT != ML_F32)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 256, 2, 2, 64, 3, 2>), grid, blk, lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 128, 256, 2, 2, stage_bytes(kDeep128x256, WG), 3, 2>), grid, blk, lds, st, a);
       break;
     case kDeep256:
       if constexpr (DT != ML_F32)
-        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 4, WG ? 64 : 128, WG ? 4 : 2, 1>), grid, dim3(512),
-                           lds, st, a);
+        hipLaunchKernelGGL((grouped_ring_kernel<DT, WG, BKC, 256, 256, 2, 4, stage_bytes(kDeep256, WG), WG ? 4 : 2, 1>), grid,
+                           dim3(512), lds, st, a);
       break;
   }
   int rc = check_launch("grouped_matmul");
@@ -335,6 +342,22 @@ extern "C" size_t ml_grouped_matmul_workspace_size(const ml_grouped_shape* s, in
     most = std::max(most, p.bytes);
   }
   return most;
+}
+
+extern "C" int ml_grouped_matmul_plan(const ml_grouped_shape* s, int dtype, int product, int transposed, int aligned,
+                                      int equal, ml_grouped_plan* plan) {
+  if (product < ML_GROUPED_FORWARD || product > ML_GROUPED_BACKWARD_WEIGHT || !plan)
+    return fail(ML_EINVAL, "grouped_matmul: unknown product, or no plan to write");
+  if (aligned && !grouped_whole(s, dtype))
+    return fail(ML_EINVAL, "grouped_matmul: rows of K or N elements are not on 16-byte boundaries");
+  GroupedPlan p;
+  const int rc = grouped_plan(s, dtype, product, transposed != 0, aligned != 0, equal != 0, p);
+  if (rc) return rc;
+  const TileShape& T = kTiles[p.tile];
+  const bool ring = p.tile >= kDeep128;
+  *plan = ml_grouped_plan{T.bm, T.bn, ring, ring ? stage_bytes(p.tile, product == kWeight) : 128, (int32_t)grouped_blocks(p),
+                          p.splits, p.fewest, p.merged};
+  return ML_OK;
 }
 
 extern "C" int ml_grouped_matmul_forward(const ml_grouped_shape* s, int dtype, const void* x, const void* weight,
