@@ -96,3 +96,81 @@ def test_captured_backward_beside_an_eager_graph(name):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, value) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("K,N", [(1 << 22, 8), ((1 << 22) - 3, 5), (8, 1 << 22), (5, (1 << 22) - 3)])
+def test_longest_reductions_and_rows(dt, K, N):
+    """K and N up to 2^22, the most that the products take."""
+    import test_gpu_grouped as grouped
+    x, w, dy = grouped.make(7, K, N, 2, dt, False, 5)
+    grouped.compare(x, w, dy, [1, 3, 6], False)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_widest_norm(dt):
+    """A width of 2^26, the most that the norm takes: a thread adds width / 1024 terms."""
+    import test_gpu_norm as norm
+    D = 1 << 26
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x, dy = ((torch.randn(2, D, generator=gen, device="cuda") + s).to(norm.TDT[dt]) for s in (0.5, 0.0))
+    w, b = ((1 + 0.2 * torch.randn(D, generator=gen, device="cuda")).to(norm.TDT[dt]) for _ in range(2))
+    got = norm.run(x, w, b, dy)
+    ref = norm.reference(x, w, b.double(), dy, 1e-5, 64 + D // 1024)
+    for g, (v, bound), name in zip(got, ref, ("y", "dx", "dw", "db")):
+        tol = bound + norm.STEP[g.dtype] * v.abs() * (1 + 2 ** -7) + 1e-37
+        assert bool(((g.double() - v).abs() <= tol).all()), name
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "grouped_matmul", "mask_logits"])
+def test_two_threads_at_once(name):
+    """Training calls of two host threads on streams of their own, side by side: each as alone."""
+    import threading
+    fn, leaves, dy = operator(name)
+    want = fn(*leaves).detach()
+    want_grads = torch.autograd.grad(fn(*leaves), leaves, dy)
+    torch.cuda.synchronize()
+    start, bad = threading.Barrier(2), []
+
+    def work():
+        own = [t.detach().clone().requires_grad_(True) for t in leaves]
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        start.wait(30)
+        with torch.cuda.stream(stream):
+            outs = []
+            for _ in range(20):
+                y = fn(*own)
+                outs.append((y.detach(), torch.autograd.grad(y, own, dy)))
+        stream.synchronize()
+        for y, grads in outs:
+            if not torch.equal(y, want) or not all(torch.equal(a, b) for a, b in zip(grads, want_grads)):
+                bad.append(name)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not any(t.is_alive() for t in threads) and not bad
+
+
+@pytest.mark.parametrize("K,rows,offsets", [(64, 40, [0, 10, 40]), (61, 400, [0, 200, 400]), (64, 400, [0, 200, 400])])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_small_float16_values(K, rows, offsets, transposed):
+    """float16 inputs below the normal range (2^-14) count in full, and so do outputs there: each kernel."""
+    import test_gpu_grouped as grouped
+    x, w, dy = grouped.make(rows, K, 72, 2, "f16", transposed, 9)
+    x, dy = (x.float() * 2.0 ** -16).half(), (dy.float() * 2.0 ** -13).half()
+    assert bool((x.abs() < 2.0 ** -14).float().mean() > 0.9)
+    grouped.compare(x, (w.float() * 64).half(), dy, offsets, transposed)
+    grouped.compare(x, w, dy, offsets, transposed)
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "grouped_matmul", "mask_logits"])
+def test_inference_mode(name):
+    fn, leaves, _ = operator(name)
+    want = fn(*leaves).detach()
+    with torch.inference_mode():
+        assert torch.equal(fn(*[t.clone() for t in leaves]), want)
+        assert torch.equal(fn(*leaves), want)
