@@ -377,15 +377,21 @@ int ml_layer_norm_backward(int dtype, int param_dtype, const void* grad_out, con
  * matrix g % matrices of weight (matrices, K, N), or (matrices, N, K) with
  * `transposed`: y_r = x_r W.  So L * B query sets (layer major) share B feature
  * maps.  groups is a positive multiple of matrices, at most 4,000; K, N <= 2^22;
- * rows <= 2^31 - 4,096; ML_EUNSUPPORTED also for more than 2^24 - 10 parts of the output of 32 x 128
+ * rows <= 2^31 - 4,096; ML_EUNSUPPORTED also for about 2^24 or more parts of the output of 32 x 128
  * (128 x 128 with over 32 rows to a group, or in grad_weight) in calls of few or unaligned rows.
  * offsets: (groups + 1) int64 on the device, not decreasing; each is held to
  * 0 .. rows and to at least the one before.  NULL: groups of rows / groups rows.
  * Rows in no group (before the first or behind the last) take zeros in y and grad_input and count for no grad_weight.
- * All tensors in `dtype`; sums are float32, rounded once, in an order that the
- * shape fixes.  grad_weight has weight's layout.
+ * All tensors in `dtype`; sums are float32, rounded once.  The same call on the same
+ * values gives the same bits; the order of a sum depends on the shape, the storage
+ * order, whether the rows start on 16-byte boundaries, the groups' sizes and whether
+ * offsets are given.  grad_weight has weight's layout.
  * Workspace: ml_grouped_matmul_workspace_size bytes for the product, 0 for a
- * shape that is refused. */
+ * shape that is refused.  It holds the parts of split reductions, at most 64 MiB
+ * (a float tile for each of 256 or 512 workgroups) or the planes of the result where
+ * few or unaligned rows are split, and covers both storage orders, any
+ * alignment, and calls with and without offsets, so a call that splits nothing may be given
+ * more than it uses. */
 typedef struct ml_grouped_shape {
   int64_t rows, K, N, groups, matrices;
 } ml_grouped_shape;

@@ -632,8 +632,10 @@ __device__ __forceinline__ void ring_wait() {
 // An XCD's run of consecutive tiles, from `start` on, among its workgroups (gridDim.x / kXcds): whole ones in
 // full rounds, and those of the last round, where they would leave half of the workgroups or
 // more without work, in parts of their reduction.
-constexpr int kTailParts = 8;  // behind whole rounds: with 16, a join of 67 MB cost more than the parts saved
-                               // (experts' d input of ml_grouped.hip, 32 tiles left: 172 us, with 8 162)
+// Behind whole rounds: 16 parts of 128 x 128 tiles cost more at their join than they save (32 tiles left of
+// 544, bf16; 8 / 16 parts: 4,352 x 4,096 x 2,048 85 / 93 us, 8,704 x 4,096 x 1,024 78 / 85, 2,176 x 8,192 x
+// 4,096 140 / 149).  The 256 x 256 tile's 32 workgroups an XCD seldom leave room for more.
+constexpr int kTailParts = 8;
 struct RingShare {
   int start, whole, rest, parts;
 };

@@ -13,7 +13,10 @@
 //   grouped_kernel, 128 x 128          229      229     258      402     315      380
 //
 // (experts: 16,384 rows in 16 groups, K = 1,024, N = 4,096; masks: 16 groups of 200 rows, K = 256,
-// N = 65,536; bf16.)  Where both operands' reduced index is contiguous, 128-byte stages read whole
+// N = 65,536; bf16.  The experts' groups are uneven, which their d weight waits for: consecutive tiles are a
+// matrix's, an XCD takes two of the 16 matrices whole, and the busiest has 1.4 to 2.0 times the mean number
+// of steps; 16 equal groups take 165 us where uneven ones take 167 to 221.)
+// Where both operands' reduced index is contiguous, 128-byte stages read whole
 // HBM lines and win; operands by rows are whole lines anyway, and the larger tiles read LDS less
 // often, in stages of 128 bytes (128 matrix instructions of a SIMD to a barrier, not 64) unless both
 // operands are by rows.  (64-byte stages, 4 waves of 128 x 128 instead of 8 of 128 x 64: masks forward 252, d weight 216,
@@ -169,9 +172,9 @@ int grouped_plan(const ml_grouped_shape* s, int dtype, int which, bool transpose
     p.tile = wg ? kDeep128 : kWide128;
   } else {
     const int rowops = wg ? 2 : (which == kForward) == transposed ? 0 : 1;  // operands by rows of the reduced index
-    // by the tables above: bound by products (per tile area), by HBM.  Over 39 ragged and whole products
-    // of 1,000 to 32,768 rows, the calls take 1.00 to 1.01 times what the best of the three tiles takes,
-    // 1.14 at most (16 groups, K = 4,096 contiguous in both, N = 1,024); by products alone 1.08 and 1.5.
+    // by the tables above: bound by products (per tile area), by HBM.  Over 156 ragged and whole products
+    // of 1,000 to 32,768 rows, half of them in float16, the calls take 1.006 times what the best of the three
+    // tiles takes on average, and 1.26 at most (55 groups of 12,542 rows, K = 832, N = 400, d weight).
     constexpr double f[3][3] = {{1.0, 1.05, 0.9}, {1.1, 1.02, 0.9}, {1.3, 1.0, 0.92}};
     constexpr double h[3][3] = {{1.05, 1.33, 1.1}, {1.55, 1.47, 1.33}, {1.56, 1.29, 1.2}};
     const Tile ts[3] = {kWide128, kDeep128x256, kDeep256};

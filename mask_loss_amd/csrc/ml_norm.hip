@@ -6,8 +6,8 @@
 // Both directions are bound by HBM: the forward reads x and writes y once, the
 // backward reads x and dy and writes dx once (172,032 x 256 f16: forward 32 us, 5.5
 // TB/s; backward 46 + 5 us, 5.2 TB/s; a copy of 1 GiB runs at 5.2).  A row is therefore held in
-// registers between its reductions, T threads to a row and up to kEpt elements
-// to a thread, so that the variance is summed about the mean (no cancellation)
+// registers between its reductions, T threads to a row and 8 or 16 elements
+// to a thread (kNormCfgs), so that the variance is summed about the mean (no cancellation)
 // without a second read.  Statistics, sums and the weights' gradients are
 // float32 whatever the input's type; each result is rounded once.
 //
