@@ -963,7 +963,7 @@ torch::autograd::variable_list once(torch::autograd::variable_list g, const char
 // on the default stream before (a leaf's, while an output of an eager call is alive) is waited for there, which
 // a capture does not survive: the process ends.  Bit i: input i of a captured call has such a node.
 int64_t eager_edges(std::initializer_list<const torch::Tensor*> inputs) {
-  const auto stream = at::hip::getCurrentHIPStream();
+  const auto stream = at::hip::getCurrentHIPStream((*inputs.begin())->device().index());
   if (stream.id() == 0) return 0;  // the default stream is not captured
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return 0;
