@@ -421,6 +421,62 @@ int ml_grouped_matmul_backward_weight(const ml_grouped_shape* s, int dtype, cons
                                       void* grad_weight, void* workspace, size_t workspace_bytes,
                                       ml_stream_t stream);
 
+/* ---- root-mean-square norm with a residual (no counterpart in the reference) --------
+ * Over the last dimension of (rows, width) in `dtype`: sum = x + residual rounded to `dtype` (residual and sum NULL:
+ * the norm of x), r = 1 / sqrt(mean sum^2 + eps), y = sum r w.  weight (width,) in param_dtype (`dtype` or ML_F32), NULL
+ * for ones.  rstd: (rows,) float for the backward, NULL where none follows.  Statistics are float32.  width <= 2^26;
+ * eps >= 0.  sum may be x or residual itself, y may not overlap an input.
+ * ml_rms_norm_mx_forward: y in microscaled values (below), width a multiple of 32, all pointers but weight and scales
+ * on 16-byte boundaries.
+ * Backward: `sum` is what the norm read (x without a residual), grad_sum the gradient that reaches the sum past the norm
+ * (NULL: none); grad_input (rows, width), the gradient of x and of the residual, and grad_weight (width,) in param_dtype, each
+ * NULL where it is not wanted.  workspace (ml_rms_norm_backward_workspace_size bytes, 0 for an invalid shape) is needed
+ * for grad_weight, whose sums over the rows are float32 in a fixed order. */
+int ml_rms_norm_forward(int dtype, int param_dtype, const void* x, const void* residual, const void* weight, int64_t rows,
+                        int64_t width, float eps, void* sum, void* y, float* rstd, ml_stream_t stream);
+int ml_rms_norm_mx_forward(int dtype, int param_dtype, const void* x, const void* residual, const void* weight, int64_t rows,
+                           int64_t width, float eps, int format, void* sum, void* codes, uint8_t* scales,
+                           ml_stream_t stream);
+size_t ml_rms_norm_backward_workspace_size(int64_t rows, int64_t width);
+int ml_rms_norm_backward(int dtype, int param_dtype, const void* grad_out, const void* grad_sum, const void* sum,
+                         const void* weight, const float* rstd, int64_t rows, int64_t width, void* grad_input,
+                         void* grad_weight, void* workspace, size_t workspace_bytes, ml_stream_t stream);
+
+/* ---- microscaled values (no counterpart in the reference) -----------------------------
+ * The OCP microscaling formats: 32 consecutive values of a row share a scale, 2^(byte - 127), 255 for NaN.  Values are
+ * e2m1 (4 bits, two to a byte, the first in the low bits: rows of width / 2 bytes) or e4m3 (8 bits).  The scale's exponent
+ * is that of the block's largest magnitude less the format's (2, 8), held to -127 .. 127; values are rounded to nearest, ties to
+ * even, and held to the format's largest (6, 448).  A block with a NaN or an infinity gets the scale NaN, one of zeros the
+ * smallest.  x (rows, width) in `dtype`, width a multiple of 32; scales (rows, width / 32).  x and codes on 16-byte boundaries. */
+enum { ML_MX_E2M1 = 0, ML_MX_E4M3 = 1 };
+int ml_mx_quantize(int dtype, const void* x, int64_t rows, int64_t width, int format, void* codes, uint8_t* scales,
+                   ml_stream_t stream);
+
+/* ---- rows by expert (no counterpart in the reference) -----------------------------------
+ * Assignment a = t k + j of `tokens` tokens has the expert ids[a]; a number outside 0 .. experts - 1 drops it.
+ * ml_sort_by_expert: order (tokens * k), the assignments by expert, those of one expert in their order, the dropped ones last;
+ * slots (tokens, k), each assignment's place in that order; offsets (experts + 1), each expert's first place and that of the
+ * dropped ones: what ml_grouped_matmul_* takes.  workspace: ml_sort_by_expert_workspace_size bytes, 0 for refused sizes.
+ * ml_to_experts: rows[slot of (t, j)] = x[t], rows of row_bytes bytes each, of any type; zeros in the dropped places.
+ * ml_from_experts_forward: out[t] = sum over j of weights[t, j] rows[slot of (t, j)], dropped assignments left out; weights
+ * (tokens, k) in weight_dtype (`dtype` or ML_F32), NULL for ones (the gradient of ml_to_experts).  Sums are float32 in
+ * the order of j, rounded once.
+ * ml_from_experts_backward: grad_rows (tokens * k, width), zeros in the dropped places, and grad_weights (tokens, k), zeros
+ * for the dropped assignments; each NULL where it is not wanted.
+ * experts <= 4,000, at most 2^31 - 4,096 assignments.  slots and offsets are read on the GPU alone; places outside the
+ * kept ones count as dropped, so no value reads or writes outside the tensors. */
+size_t ml_sort_by_expert_workspace_size(int64_t tokens, int64_t k, int64_t experts);
+int ml_sort_by_expert(const int64_t* ids, int64_t tokens, int64_t k, int64_t experts, int64_t* order, int64_t* slots,
+                      int64_t* offsets, void* workspace, size_t workspace_bytes, ml_stream_t stream);
+int ml_to_experts(const void* x, int64_t tokens, int64_t k, int64_t row_bytes, const int64_t* slots, const int64_t* offsets,
+                  int64_t experts, void* rows, ml_stream_t stream);
+int ml_from_experts_forward(int dtype, int weight_dtype, const void* rows, const void* weights, int64_t tokens, int64_t k,
+                            int64_t width, const int64_t* slots, const int64_t* offsets, int64_t experts, void* out,
+                            ml_stream_t stream);
+int ml_from_experts_backward(int dtype, int weight_dtype, const void* grad_out, const void* rows, const void* weights,
+                             int64_t tokens, int64_t k, int64_t width, const int64_t* slots, const int64_t* offsets,
+                             int64_t experts, void* grad_rows, void* grad_weights, ml_stream_t stream);
+
 /* ---- input validation helper ------------------------------------------------
  * flag[0] = 1 if any of x[0..n) equals `value`, else 0 (one small kernel, no
  * synchronisation).  Replaces the device-wide comparison + reduction behind
@@ -433,7 +489,8 @@ int ml_any_equal(const int64_t* x, int64_t n, int64_t value, int32_t* flag, ml_s
  * recorded on its own stream.  ml_profile_read() waits for those events and
  * returns, for kernel family `name` ("prep", "pair_cost", "assign", "layer",
  * "bwd_mask", "bwd_cls", "label_cost", "prefill", "layer_norm", "layer_norm_backward",
- * "grouped_matmul"), the number of launches and their
+ * "grouped_matmul", "rms_norm", "rms_norm_backward", "mx_quantize", "sort_by_expert", "to_experts", "from_experts",
+ * "from_experts_backward"), the number of launches and their
  * summed duration in milliseconds since the last reset. */
 int ml_profile_enable(int enable);
 int ml_profile_read(const char* name, int64_t* launches, double* total_ms);

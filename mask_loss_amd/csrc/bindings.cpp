@@ -1241,6 +1241,357 @@ torch::Tensor mask_logits_autograd(const torch::Tensor& queries, const torch::Te
   return GroupedNode::apply(queries, features, offsets, false, true);
 }
 
+// --------------------------------------------------------------------------
+// root-mean-square norm with a residual, microscaled values (no counterpart in
+// the reference)
+// --------------------------------------------------------------------------
+// (rows, width) of the norm's input, weight and residual as given to it
+NormArgs rms_args(const char* who, const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
+                  const c10::optional<torch::Tensor>& residual) {
+  ML_CHECK_INPUT(x);
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, who, ": input must have a last dimension of at least 1");
+  NormArgs a;
+  a.width = x.size(-1);
+  a.rows = x.numel() / a.width;
+  a.dt = a.pdt = dtype_code(x, "input");
+  if (weight.has_value()) {
+    const torch::Tensor& w = *weight;
+    ML_CHECK_INPUT(w);
+    TORCH_CHECK(w.dim() == 1 && w.size(0) == a.width, who, ": weight must have shape (", a.width,
+                ",), the input's last dimension");
+    TORCH_CHECK(w.device() == x.device(), "all tensors must be on the same device");
+    a.pdt = dtype_code(w, "weight");
+    TORCH_CHECK(a.pdt == a.dt || a.pdt == ML_F32, who, ": weight must have the input's dtype or be float32");
+  }
+  if (residual.has_value()) {
+    const torch::Tensor& r = *residual;
+    ML_CHECK_INPUT(r);
+    TORCH_CHECK(r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type(), who,
+                ": residual must match the input in shape and dtype");
+    TORCH_CHECK(r.device() == x.device(), "all tensors must be on the same device");
+  }
+  return a;
+}
+
+// y, the sum (undefined without a residual), 1 / root mean square of the rows (undefined unless asked for)
+std::vector<torch::Tensor> rms_norm_forward(const torch::Tensor& x, const c10::optional<torch::Tensor>& weight,
+                                            const c10::optional<torch::Tensor>& residual, double eps, bool want_stats) {
+  no_tangent("rms_norm", x, weight, residual);
+  const NormArgs a = rms_args("rms_norm", x, weight, residual);
+  TORCH_CHECK_VALUE(eps >= 0.0, "rms_norm: eps must not be negative");
+  const c10::DeviceGuard guard(x.device());
+  const auto y = torch::empty_like(x);
+  torch::Tensor sum, rstd;
+  if (residual.has_value()) sum = torch::empty_like(x);
+  if (want_stats) rstd = torch::empty({a.rows}, x.options().dtype(torch::kFloat32));
+  ml_ok(ml_rms_norm_forward(a.dt, a.pdt, x.data_ptr(), ptr_or_null(residual), ptr_or_null(weight), a.rows, a.width, (float)eps,
+                            sum.defined() ? sum.data_ptr() : nullptr, y.data_ptr(),
+                            rstd.defined() ? rstd.data_ptr<float>() : nullptr, cur_stream()));
+  return {y, sum, rstd};
+}
+
+// gradients of the input (and the residual) and of the weight, those asked for (the others undefined); sum: what the
+// norm read
+std::vector<torch::Tensor> rms_norm_backward(const torch::Tensor& grad_out, const c10::optional<torch::Tensor>& grad_sum,
+                                             const torch::Tensor& sum, const c10::optional<torch::Tensor>& weight,
+                                             const torch::Tensor& rstd, bool need_input, bool need_weight) {
+  no_tangent("rms_norm backward", grad_out, grad_sum, sum, weight, rstd);
+  const NormArgs a = rms_args("rms_norm", sum, weight, c10::nullopt);
+  ML_CHECK_INPUT(grad_out);
+  ML_CHECK_INPUT(rstd);
+  TORCH_CHECK(grad_out.sizes() == sum.sizes() && grad_out.scalar_type() == sum.scalar_type(),
+              "rms_norm: grad_out must match the input in shape and dtype");
+  if (grad_sum.has_value()) {
+    ML_CHECK_INPUT(*grad_sum);
+    TORCH_CHECK(grad_sum->sizes() == sum.sizes() && grad_sum->scalar_type() == sum.scalar_type(),
+                "rms_norm: grad_sum must match the input in shape and dtype");
+    TORCH_CHECK(grad_sum->device() == sum.device(), "all tensors must be on the same device");
+  }
+  TORCH_CHECK(rstd.scalar_type() == torch::kFloat32 && rstd.numel() == a.rows,
+              "rms_norm: rstd must be float32, one value per row");
+  TORCH_CHECK(grad_out.device() == sum.device() && rstd.device() == sum.device(), "all tensors must be on the same device");
+  TORCH_CHECK(!need_weight || weight.has_value(), "rms_norm: no weight to give a gradient for");
+  const c10::DeviceGuard guard(sum.device());
+  torch::Tensor dx, dw, ws;
+  if (need_input) dx = torch::empty_like(sum);
+  if (need_weight) {
+    dw = torch::empty_like(*weight);
+    ws = workspace(ml_rms_norm_backward_workspace_size(a.rows, a.width), sum);
+  }
+  auto p = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  ml_ok(ml_rms_norm_backward(a.dt, a.pdt, grad_out.data_ptr(), ptr_or_null(grad_sum), sum.data_ptr(), ptr_or_null(weight),
+                             rstd.data_ptr<float>(), a.rows, a.width, p(dx), p(dw), p(ws), ws.defined() ? ws.numel() : 0,
+                             cur_stream()));
+  return {dx, dw};
+}
+
+c10::optional<torch::Tensor> contiguous_or_none(const c10::optional<torch::Tensor>& t) {
+  return t.has_value() ? c10::optional<torch::Tensor>(t->contiguous()) : t;
+}
+
+struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input,
+                                                const c10::optional<torch::Tensor>& weight,
+                                                const c10::optional<torch::Tensor>& residual, double eps) {
+    const auto x = input.contiguous();
+    const auto w = contiguous_or_none(weight), res = contiguous_or_none(residual);
+    const auto r = rms_norm_forward(x, w, res, eps, true);
+    ctx->save_for_backward({res.has_value() ? r[1] : x, w.has_value() ? *w : torch::Tensor(), r[2]});
+    ctx->set_materialize_grads(false);  // a sum that nothing uses has no gradient to read
+    const torch::Tensor none;
+    ctx->saved_data["residual"] = res.has_value();
+    ctx->saved_data["edges"] =
+        eager_edges({&input, weight.has_value() ? &*weight : &none, residual.has_value() ? &*residual : &none});
+    return res.has_value() ? torch::autograd::variable_list{r[0], r[1]} : torch::autograd::variable_list{r[0]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto sv = ctx->get_saved_variables();
+    const auto& sum = sv[0];
+    c10::optional<torch::Tensor> w, gs;
+    if (sv[1].defined()) w = sv[1];
+    for (const auto& t : g) no_tangent("rms_norm backward", t);  // (detaching drops it)
+    // only tensors that were given count as inputs of the node
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const bool need_x = ctx->needs_input_grad(0), need_w = w.has_value() && ctx->needs_input_grad(1);
+    const bool need_r = residual && ctx->needs_input_grad(w.has_value() ? 2 : 1);
+    const int64_t edges = ctx->saved_data["edges"].toInt();
+    no_eager_edge("rms_norm", edges, 0, need_x);
+    no_eager_edge("rms_norm", edges, 1, need_w);
+    no_eager_edge("rms_norm", edges, 2, need_r);
+    if (residual && g[1].defined()) gs = g[1].detach().contiguous();
+    torch::Tensor dx, dw, dr;
+    if (g[0].defined()) {
+      const auto r = rms_norm_backward(g[0].detach().contiguous(), gs, sum, w, sv[2], need_x || need_r, need_w);
+      dx = r[0];
+      dw = r[1];
+    } else {  // the sum alone was used
+      if (gs.has_value() && (need_x || need_r)) dx = *gs;
+      if (need_w) dw = torch::zeros_like(*w);
+    }
+    if (need_r) dr = dx;
+    if (!need_x) dx = torch::Tensor();
+    return once({dx, dw, dr, torch::Tensor()}, "the backward of rms_norm cannot be differentiated");
+  }
+};
+
+std::vector<torch::Tensor> rms_norm_autograd(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
+                                             const c10::optional<torch::Tensor>& residual, double eps) {
+  return RmsNormNode::apply(input, weight, residual, eps);
+}
+
+// Codes and scales of microscaled values: e2m1 two to a byte in uint8, e4m3 as torch has it.
+int mx_format_code(const std::string& format) {
+  TORCH_CHECK_VALUE(format == "e2m1" || format == "e4m3", "format must be 'e2m1' or 'e4m3', got '", format, "'");
+  return format == "e2m1" ? ML_MX_E2M1 : ML_MX_E4M3;
+}
+void no_gradient(const char* who, std::initializer_list<const torch::Tensor*> tensors) {
+  for (const torch::Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->requires_grad() || !torch::GradMode::is_enabled(), who,
+                                ": no gradient is provided for quantised values; call it under torch.no_grad()");
+}
+std::pair<torch::Tensor, torch::Tensor> mx_empty(const torch::Tensor& x, int format) {
+  const int64_t width = x.size(-1);
+  return {torch::empty(with_width(x, format == ML_MX_E2M1 ? width / 2 : width),
+                       x.options().dtype(format == ML_MX_E2M1 ? torch::kUInt8 : torch::kFloat8_e4m3fn)),
+          torch::empty(with_width(x, width / 32), x.options().dtype(torch::kFloat8_e8m0fnu))};
+}
+// The kernels read and write 16 bytes at once.
+torch::Tensor on_16_bytes(const torch::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
+}
+
+std::vector<torch::Tensor> mx_quantize(const torch::Tensor& input, const std::string& format) {
+  no_tangent("mx_quantize", input);
+  const int f = mx_format_code(format);
+  no_gradient("mx_quantize", {&input});
+  ML_CHECK_INPUT(input);
+  TORCH_CHECK(input.dim() >= 1 && input.size(-1) % 32 == 0, "mx_quantize: the last dimension must be a multiple of 32");
+  const int dt = dtype_code(input, "input");
+  const c10::DeviceGuard guard(input.device());
+  const auto x = on_16_bytes(input);
+  const auto out = mx_empty(x, f);
+  const int64_t width = x.size(-1), rows = width ? x.numel() / width : 0;
+  ml_ok(ml_mx_quantize(dt, x.data_ptr(), rows, width, f, out.first.data_ptr(), (uint8_t*)out.second.data_ptr(), cur_stream()));
+  return {out.first, out.second};
+}
+
+// codes, scales, the sum (undefined without a residual)
+std::vector<torch::Tensor> rms_norm_mx_forward(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
+                                               const c10::optional<torch::Tensor>& residual, double eps,
+                                               const std::string& format) {
+  no_tangent("rms_norm_mx", input, weight, residual);
+  const int f = mx_format_code(format);
+  const torch::Tensor none;
+  no_gradient("rms_norm_mx", {&input, weight.has_value() ? &*weight : &none, residual.has_value() ? &*residual : &none});
+  const NormArgs a = rms_args("rms_norm_mx", input, weight, residual);
+  TORCH_CHECK_VALUE(eps >= 0.0, "rms_norm_mx: eps must not be negative");
+  TORCH_CHECK(a.width % 32 == 0, "rms_norm_mx: the last dimension must be a multiple of 32");
+  const c10::DeviceGuard guard(input.device());
+  const auto x = on_16_bytes(input);
+  torch::Tensor res, sum;
+  if (residual.has_value()) {
+    res = on_16_bytes(*residual);
+    sum = torch::empty_like(x);
+  }
+  const auto out = mx_empty(x, f);
+  ml_ok(ml_rms_norm_mx_forward(a.dt, a.pdt, x.data_ptr(), res.defined() ? res.data_ptr() : nullptr, ptr_or_null(weight), a.rows,
+                               a.width, (float)eps, f, sum.defined() ? sum.data_ptr() : nullptr, out.first.data_ptr(),
+                               (uint8_t*)out.second.data_ptr(), cur_stream()));
+  return {out.first, out.second, sum};
+}
+
+// --------------------------------------------------------------------------
+// rows by expert (no counterpart in the reference)
+// --------------------------------------------------------------------------
+std::vector<torch::Tensor> sort_by_expert(const torch::Tensor& ids, int64_t experts) {
+  ML_CHECK_INPUT(ids);
+  TORCH_CHECK(ids.scalar_type() == torch::kLong, "sort_by_expert: expert numbers must be int64");
+  TORCH_CHECK(ids.dim() == 2, "sort_by_expert: expert numbers must be (tokens, k)");
+  const c10::DeviceGuard guard(ids.device());
+  const int64_t tokens = ids.size(0), k = ids.size(1);
+  const size_t bytes = ml_sort_by_expert_workspace_size(tokens, k, experts);
+  TORCH_CHECK(bytes > 0, ml_last_error());
+  auto order = torch::empty({tokens * k}, ids.options()), slots = torch::empty_like(ids),
+       offsets = torch::empty({experts + 1}, ids.options()), ws = workspace(bytes, ids);
+  ml_ok(ml_sort_by_expert(ids.data_ptr<int64_t>(), tokens, k, experts, order.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                          offsets.data_ptr<int64_t>(), ws.data_ptr(), ws.numel(), cur_stream()));
+  return {order, slots, offsets};
+}
+
+// `rows`: one of each token (there), or of each assignment (back)
+void expert_args(const char* who, const torch::Tensor& rows, const torch::Tensor& slots, const torch::Tensor& offsets,
+                 bool back) {
+  ML_CHECK_INPUT(rows);
+  ML_CHECK_INPUT(slots);
+  ML_CHECK_INPUT(offsets);
+  TORCH_CHECK(slots.scalar_type() == torch::kLong && offsets.scalar_type() == torch::kLong, who,
+              ": slots and offsets must be int64");
+  TORCH_CHECK(slots.dim() == 2 && offsets.dim() == 1 && offsets.size(0) >= 2, who,
+              ": slots must be (tokens, k) and offsets (experts + 1,)");
+  TORCH_CHECK(rows.device() == slots.device() && rows.device() == offsets.device(), "all tensors must be on the same device");
+  const int64_t n = back ? slots.numel() : slots.size(0);
+  TORCH_CHECK(rows.dim() == 2 && rows.size(0) == n, who, ": input must be (", back ? "tokens * k" : "tokens", ", width) with ", n,
+              " rows, got ", rows.sizes());
+}
+
+torch::Tensor to_experts_forward(const torch::Tensor& x, const torch::Tensor& slots, const torch::Tensor& offsets) {
+  no_tangent("to_experts", x);
+  expert_args("to_experts", x, slots, offsets, false);
+  const c10::DeviceGuard guard(x.device());
+  auto rows = torch::empty({slots.numel(), x.size(1)}, x.options());
+  ml_ok(ml_to_experts(x.data_ptr(), x.size(0), slots.size(1), x.size(1) * (int64_t)x.element_size(), slots.data_ptr<int64_t>(),
+                      offsets.data_ptr<int64_t>(), offsets.size(0) - 1, rows.data_ptr(), cur_stream()));
+  return rows;
+}
+
+// ML dtype of the weights (the rows' own where there are none)
+int weights_dtype(const torch::Tensor& rows, const torch::Tensor& slots, const c10::optional<torch::Tensor>& weights) {
+  const int dt = dtype_code(rows, "input");
+  if (!weights.has_value()) return dt;
+  ML_CHECK_INPUT(*weights);
+  TORCH_CHECK(weights->sizes() == slots.sizes(), "from_experts: weights must be (tokens, k) = ", slots.sizes(), ", got ",
+              weights->sizes());
+  TORCH_CHECK(weights->device() == rows.device(), "all tensors must be on the same device");
+  const int wd = dtype_code(*weights, "weights");
+  TORCH_CHECK(wd == dt || wd == ML_F32, "from_experts: weights must have the input's dtype or be float32");
+  return wd;
+}
+
+torch::Tensor from_experts_forward(const torch::Tensor& rows, const torch::Tensor& slots, const torch::Tensor& offsets,
+                                   const c10::optional<torch::Tensor>& weights) {
+  no_tangent("from_experts", rows, weights);
+  expert_args("from_experts", rows, slots, offsets, true);
+  const int wd = weights_dtype(rows, slots, weights);
+  const c10::DeviceGuard guard(rows.device());
+  auto out = torch::empty({slots.size(0), rows.size(1)}, rows.options());
+  ml_ok(ml_from_experts_forward(dtype_code(rows, "input"), wd, rows.data_ptr(), ptr_or_null(weights), slots.size(0),
+                                slots.size(1), rows.size(1), slots.data_ptr<int64_t>(), offsets.data_ptr<int64_t>(),
+                                offsets.size(0) - 1, out.data_ptr(), cur_stream()));
+  return out;
+}
+
+// gradients of the rows and the weights, those asked for (the others undefined)
+std::vector<torch::Tensor> from_experts_backward(const torch::Tensor& grad_out, const torch::Tensor& rows,
+                                                 const torch::Tensor& slots, const torch::Tensor& offsets,
+                                                 const c10::optional<torch::Tensor>& weights, bool need_input,
+                                                 bool need_weights) {
+  no_tangent("from_experts backward", grad_out, rows, weights);
+  expert_args("from_experts", rows, slots, offsets, true);
+  const int wd = weights_dtype(rows, slots, weights);
+  ML_CHECK_INPUT(grad_out);
+  TORCH_CHECK(grad_out.dim() == 2 && grad_out.size(0) == slots.size(0) && grad_out.size(1) == rows.size(1) &&
+                  grad_out.scalar_type() == rows.scalar_type() && grad_out.device() == rows.device(),
+              "from_experts: grad_out must be (tokens, width) in the input's dtype");
+  TORCH_CHECK(!need_weights || weights.has_value(), "from_experts: no weights to give a gradient for");
+  const c10::DeviceGuard guard(rows.device());
+  torch::Tensor dr, dw;
+  if (need_input) dr = torch::empty_like(rows);
+  if (need_weights) dw = torch::empty_like(*weights);
+  auto p = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  ml_ok(ml_from_experts_backward(dtype_code(rows, "input"), wd, grad_out.data_ptr(), rows.data_ptr(), ptr_or_null(weights),
+                                 slots.size(0), slots.size(1), rows.size(1), slots.data_ptr<int64_t>(),
+                                 offsets.data_ptr<int64_t>(), offsets.size(0) - 1, p(dr), p(dw), cur_stream()));
+  return {dr, dw};
+}
+
+struct ToExpertsNode : public torch::autograd::Function<ToExpertsNode> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input, const torch::Tensor& slots,
+                               const torch::Tensor& offsets) {
+    const auto x = input.contiguous(), s = slots.contiguous(), o = offsets.contiguous();
+    dtype_code(x, "input");  // the gradient's sums
+    auto rows = to_experts_forward(x, s, o);
+    ctx->save_for_backward({s, o});
+    ctx->saved_data["edges"] = eager_edges({&input});
+    return rows;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto sv = ctx->get_saved_variables();
+    no_tangent("to_experts backward", g[0]);  // (detaching drops it)
+    no_eager_edge("to_experts", ctx->saved_data["edges"].toInt(), 0, ctx->needs_input_grad(0));
+    torch::Tensor dx;
+    if (ctx->needs_input_grad(0)) dx = from_experts_forward(g[0].detach().contiguous(), sv[0], sv[1], c10::nullopt);
+    return once({dx, torch::Tensor(), torch::Tensor()}, "the backward of to_experts cannot be differentiated");
+  }
+};
+
+torch::Tensor to_experts_autograd(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets) {
+  return ToExpertsNode::apply(input, slots, offsets);
+}
+
+struct FromExpertsNode : public torch::autograd::Function<FromExpertsNode> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& input, const torch::Tensor& slots,
+                               const torch::Tensor& offsets, const c10::optional<torch::Tensor>& weights) {
+    const auto rows = input.contiguous(), s = slots.contiguous(), o = offsets.contiguous();
+    const auto w = contiguous_or_none(weights);
+    auto out = from_experts_forward(rows, s, o, w);
+    ctx->save_for_backward({rows, s, o, w.has_value() ? *w : torch::Tensor()});
+    const torch::Tensor none;
+    ctx->saved_data["edges"] = eager_edges({&input, weights.has_value() ? &*weights : &none});
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list g) {
+    const auto sv = ctx->get_saved_variables();
+    c10::optional<torch::Tensor> w;
+    if (sv[3].defined()) w = sv[3];
+    no_tangent("from_experts backward", g[0]);  // (detaching drops it)
+    // (slots and offsets are inputs 1 and 2)
+    const bool need_x = ctx->needs_input_grad(0), need_w = w.has_value() && ctx->needs_input_grad(3);
+    const int64_t edges = ctx->saved_data["edges"].toInt();
+    no_eager_edge("from_experts", edges, 0, need_x);
+    no_eager_edge("from_experts", edges, 1, need_w);
+    const auto r = from_experts_backward(g[0].detach().contiguous(), sv[0], sv[1], sv[2], w, need_x, need_w);
+    return once({r[0], torch::Tensor(), torch::Tensor(), r[1]}, "the backward of from_experts cannot be differentiated");
+  }
+};
+
+torch::Tensor from_experts_autograd(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets,
+                                    const c10::optional<torch::Tensor>& weights) {
+  return FromExpertsNode::apply(input, slots, offsets, weights);
+}
+
 // Device flag (int32, shape (1,)): 1 if any element of `x` equals `value`.
 torch::Tensor any_equal(const torch::Tensor& x, int64_t value) {
   ML_CHECK_INPUT(x);
@@ -1346,6 +1697,37 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_matmul_autograd", &grouped_matmul_autograd,
         "Grouped product as a C++ autograd node, differentiable in input and weight (HIP)", py::arg("input"),
         py::arg("weight"), py::arg("offsets"), py::arg("transposed") = false);
+  m.def("rms_norm_forward", &rms_norm_forward,
+        "Root-mean-square norm: output, the sum with a residual, and per row 1/rms if asked for (HIP)", py::arg("input"),
+        py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("want_stats") = false);
+  m.def("rms_norm_backward", &rms_norm_backward,
+        "Gradients of rms_norm_forward with respect to input (and residual) and weight (HIP)", py::arg("grad_out"),
+        py::arg("grad_sum"), py::arg("sum"), py::arg("weight"), py::arg("rstd"), py::arg("need_input") = true,
+        py::arg("need_weight") = true);
+  m.def("rms_norm_autograd", &rms_norm_autograd,
+        "Root-mean-square norm as a C++ autograd node, differentiable in input, weight and residual (HIP)", py::arg("input"),
+        py::arg("weight"), py::arg("residual"), py::arg("eps"));
+  m.def("rms_norm_mx_forward", &rms_norm_mx_forward,
+        "Root-mean-square norm with microscaled output: codes, scales, and the sum with a residual (HIP)", py::arg("input"),
+        py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("format") = "e4m3");
+  m.def("mx_quantize", &mx_quantize, "Microscaled values of the last dimension's blocks of 32: codes, scales (HIP)",
+        py::arg("input"), py::arg("format") = "e4m3");
+  m.def("sort_by_expert", &sort_by_expert, "(tokens, k) expert numbers sorted by expert: order, slots, offsets (HIP)",
+        py::arg("ids"), py::arg("experts"));
+  m.def("to_experts_forward", &to_experts_forward, "Tokens' rows at their experts' places (HIP)", py::arg("input"),
+        py::arg("slots"), py::arg("offsets"));
+  m.def("to_experts_autograd", &to_experts_autograd,
+        "Tokens' rows at their experts' places as a C++ autograd node, differentiable in input (HIP)", py::arg("input"),
+        py::arg("slots"), py::arg("offsets"));
+  m.def("from_experts_forward", &from_experts_forward, "Experts' rows summed back with weights (HIP)", py::arg("input"),
+        py::arg("slots"), py::arg("offsets"), py::arg("weights") = py::none());
+  m.def("from_experts_backward", &from_experts_backward,
+        "Gradients of from_experts_forward with respect to input and weights (HIP)", py::arg("grad_out"), py::arg("input"),
+        py::arg("slots"), py::arg("offsets"), py::arg("weights"), py::arg("need_input") = true,
+        py::arg("need_weights") = true);
+  m.def("from_experts_autograd", &from_experts_autograd,
+        "Experts' rows summed back as a C++ autograd node, differentiable in input and weights (HIP)", py::arg("input"),
+        py::arg("slots"), py::arg("offsets"), py::arg("weights") = py::none());
   m.def("any_equal", &any_equal, "Device flag: any element equal to value (HIP)");
   m.attr("__backend__") = "hip-gfx950";
 }

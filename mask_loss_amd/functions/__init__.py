@@ -22,6 +22,10 @@ from .mask.matching import MaskMatchingFunction
 from .mask.mask_logits import mask_logits
 from .head.grouped_matmul import GroupedMatmulFunction, grouped_matmul
 from .head.layer_norm import LayerNormFunction, layer_norm
+from .head.rms_norm import RMSNormFunction, rms_norm, rms_norm_mx
+from .head.experts import (ExpertOrder, FromExpertsFunction, ToExpertsFunction, from_experts, sort_by_expert,
+                           to_experts)
+from .head.mx import mx_quantize
 from .losses import sigmoid_cross_entropy_loss, dice_loss
 
 __all__ = [
@@ -46,4 +50,14 @@ __all__ = [
     "grouped_matmul",
     "LayerNormFunction",
     "layer_norm",
+    "RMSNormFunction",
+    "rms_norm",
+    "rms_norm_mx",
+    "ExpertOrder",
+    "ToExpertsFunction",
+    "FromExpertsFunction",
+    "sort_by_expert",
+    "to_experts",
+    "from_experts",
+    "mx_quantize",
 ]
