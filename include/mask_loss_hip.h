@@ -452,6 +452,20 @@ enum { ML_MX_E2M1 = 0, ML_MX_E4M3 = 1 };
 int ml_mx_quantize(int dtype, const void* x, int64_t rows, int64_t width, int format, void* codes, uint8_t* scales,
                    ml_stream_t stream);
 
+/* Products of ragged groups of microscaled rows with one microscaled matrix per group: ml_grouped_matmul_forward's groups,
+ * matrices (matrices, N, K) and limits, for inference.  x: codes (rows, K) in x_format on 16-byte boundaries and x_scales
+ * (rows, K / 32); weight: codes (matrices, N, K) in weight_format on 16-byte boundaries and weight_scales (matrices, N, K / 32);
+ * K a multiple of 32; y (rows, N) in `dtype`.
+ * Sums are float32 in an order that the shape, the formats, the groups' sizes and whether offsets are given fix, rounded
+ * once.  Where an operand is e4m3 and `dtype` has 16 bits, the matrix instruction lines up the products of eight neighbours
+ * of the reduced index on the largest and drops what lies over 13 bits below its leading one (1.5e-5 of a result's size with
+ * normal operands); with ML_F32 nothing is dropped: such operands go through bfloat16 with their scales, where values of
+ * 2^128 and more are infinite and values below 2^-126 may count as zero. */
+size_t ml_grouped_matmul_mx_workspace_size(const ml_grouped_shape* s, int x_format, int weight_format, int dtype);
+int ml_grouped_matmul_mx(const ml_grouped_shape* s, int x_format, const void* x, const uint8_t* x_scales, int weight_format,
+                         const void* weight, const uint8_t* weight_scales, const int64_t* offsets, int dtype, void* y,
+                         void* workspace, size_t workspace_bytes, ml_stream_t stream);
+
 /* ---- rows by expert (no counterpart in the reference) -----------------------------------
  * Assignment a = t k + j of `tokens` tokens has the expert ids[a]; a number outside 0 .. experts - 1 drops it.
  * ml_sort_by_expert: order (tokens * k), the assignments by expert, those of one expert in their order, the dropped ones last;
@@ -489,7 +503,7 @@ int ml_any_equal(const int64_t* x, int64_t n, int64_t value, int32_t* flag, ml_s
  * recorded on its own stream.  ml_profile_read() waits for those events and
  * returns, for kernel family `name` ("prep", "pair_cost", "assign", "layer",
  * "bwd_mask", "bwd_cls", "label_cost", "prefill", "layer_norm", "layer_norm_backward",
- * "grouped_matmul", "rms_norm", "rms_norm_backward", "mx_quantize", "sort_by_expert", "to_experts", "from_experts",
+ * "grouped_matmul", "rms_norm", "rms_norm_backward", "mx_quantize", "grouped_matmul_mx", "sort_by_expert", "to_experts", "from_experts",
  * "from_experts_backward"), the number of launches and their
  * summed duration in milliseconds since the last reset. */
 int ml_profile_enable(int enable);

@@ -1441,6 +1441,70 @@ std::vector<torch::Tensor> rms_norm_mx_forward(const torch::Tensor& input, const
   return {out.first, out.second, sum};
 }
 
+// Codes and scales as mx_quantize gives them; returns the format, `width` in values.
+int mx_operand(const char* what, const torch::Tensor& codes, const torch::Tensor& scales, int64_t& width) {
+  ML_CHECK_INPUT(codes);
+  ML_CHECK_INPUT(scales);
+  const bool e2m1 = codes.scalar_type() == torch::kUInt8;
+  TORCH_CHECK(e2m1 || codes.scalar_type() == torch::kFloat8_e4m3fn, "grouped_matmul_mx: the codes of the ", what,
+              " must be uint8 (e2m1) or float8_e4m3fn");
+  TORCH_CHECK(scales.scalar_type() == torch::kFloat8_e8m0fnu, "grouped_matmul_mx: the scales of the ", what,
+              " must be float8_e8m0fnu");
+  TORCH_CHECK(codes.dim() >= 1 && codes.dim() == scales.dim(), "grouped_matmul_mx: the scales of the ", what,
+              " must have its dimensions");
+  width = codes.size(-1) * (e2m1 ? 2 : 1);
+  TORCH_CHECK(width % 32 == 0 && scales.sizes() == c10::IntArrayRef(with_width(codes, width / 32)),
+              "grouped_matmul_mx: the ", what, " must have whole blocks of 32 values and a scale for each, got ", codes.sizes(),
+              " and ", scales.sizes());
+  TORCH_CHECK(codes.device() == scales.device(), "all tensors must be on the same device");
+  return e2m1 ? ML_MX_E2M1 : ML_MX_E4M3;
+}
+
+torch::Tensor grouped_matmul_mx(const torch::Tensor& input, const torch::Tensor& scales, const torch::Tensor& weight,
+                                const torch::Tensor& weight_scales, const c10::optional<torch::Tensor>& offsets,
+                                torch::ScalarType dtype) {
+  no_tangent("grouped_matmul_mx", input, scales, weight, weight_scales);
+  no_gradient("grouped_matmul_mx", {&input, &scales, &weight, &weight_scales});
+  int64_t K, Kw;
+  const int fx = mx_operand("input", input, scales, K), fw = mx_operand("weight", weight, weight_scales, Kw);
+  TORCH_CHECK(weight.dim() == 3, "grouped_matmul_mx: weight must be (matrices, N, K)");
+  TORCH_CHECK(K == Kw, "grouped_matmul_mx: input and weight must have the same K, got ", K, " and ", Kw);
+  TORCH_CHECK(input.device() == weight.device(), "all tensors must be on the same device");
+  TORCH_CHECK(dtype == torch::kFloat32 || dtype == torch::kBFloat16 || dtype == torch::kFloat16,
+              "grouped_matmul_mx: dtype must be float32, bfloat16 or float16");
+  const int dt = dtype == torch::kFloat32 ? ML_F32 : dtype == torch::kBFloat16 ? ML_BF16 : ML_F16;
+  ml_grouped_shape s;
+  s.matrices = weight.size(0);
+  s.K = K;
+  s.N = weight.size(1);
+  if (offsets.has_value()) {
+    const torch::Tensor& o = *offsets;
+    ML_CHECK_INPUT(o);
+    TORCH_CHECK(o.scalar_type() == torch::kLong, "offsets must be int64");
+    TORCH_CHECK(o.dim() == 1 && o.size(0) >= 2, "grouped_matmul_mx: offsets must have shape (groups + 1,)");
+    TORCH_CHECK(o.device() == input.device(), "all tensors must be on the same device");
+    TORCH_CHECK(input.dim() == 2, "grouped_matmul_mx: input must be (rows, K) with offsets");
+    s.groups = o.size(0) - 1;
+    s.rows = input.size(0);
+  } else {
+    TORCH_CHECK(input.dim() == 3, "grouped_matmul_mx: input must be (groups, rows, K) without offsets");
+    s.groups = input.size(0);
+    s.rows = s.groups * input.size(1);
+  }
+  TORCH_CHECK(s.matrices >= 1 && s.groups >= 1 && s.groups % s.matrices == 0,
+              "grouped_matmul_mx: the number of groups must be a positive multiple of the number of matrices");
+  const c10::DeviceGuard guard(input.device());
+  const auto x = on_16_bytes(input), w = on_16_bytes(weight);
+  auto y = torch::empty(with_width(x, s.N), x.options().dtype(dtype));
+  const size_t bytes = ml_grouped_matmul_mx_workspace_size(&s, fx, fw, dt);
+  TORCH_CHECK(bytes > 0, ml_last_error());
+  auto ws = workspace(bytes, x);
+  ml_ok(ml_grouped_matmul_mx(&s, fx, x.data_ptr(), (const uint8_t*)scales.data_ptr(), fw, w.data_ptr(),
+                             (const uint8_t*)weight_scales.data_ptr(), offsets_ptr(offsets), dt, y.data_ptr(), ws.data_ptr(),
+                             ws.numel(), cur_stream()));
+  return y;
+}
+
 // --------------------------------------------------------------------------
 // rows by expert (no counterpart in the reference)
 // --------------------------------------------------------------------------
@@ -1712,6 +1776,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("format") = "e4m3");
   m.def("mx_quantize", &mx_quantize, "Microscaled values of the last dimension's blocks of 32: codes, scales (HIP)",
         py::arg("input"), py::arg("format") = "e4m3");
+  m.def(
+      "grouped_matmul_mx",
+      [](const torch::Tensor& input, const torch::Tensor& scales, const torch::Tensor& weight,
+         const torch::Tensor& weight_scales, const c10::optional<torch::Tensor>& offsets, const py::object& dtype) {
+        return grouped_matmul_mx(input, scales, weight, weight_scales, offsets,
+                                 torch::python::detail::py_object_to_dtype(dtype));
+      },
+      "Microscaled rows in ragged groups times one microscaled matrix per group (HIP)", py::arg("input"), py::arg("scales"),
+      py::arg("weight"), py::arg("weight_scales"), py::arg("offsets"), py::arg("dtype"));
   m.def("sort_by_expert", &sort_by_expert, "(tokens, k) expert numbers sorted by expert: order, slots, offsets (HIP)",
         py::arg("ids"), py::arg("experts"));
   m.def("to_experts_forward", &to_experts_forward, "Tokens' rows at their experts' places (HIP)", py::arg("input"),

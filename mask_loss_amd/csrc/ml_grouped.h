@@ -957,4 +957,40 @@ __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg
   }
 }
 
+// Sums of the planes of a split reduction: four elements a thread, four slices of the planes to a
+// workgroup, each with up to eight loads in flight, in an order that the shape alone fixes.
+constexpr int kJoinQuads = 64, kJoinSlices = 4;
+template <int DT>
+__global__ __launch_bounds__(kJoinQuads* kJoinSlices) void grouped_join_kernel(const float* planes, int splits,
+                                                                              int64_t plane, int64_t n, void* c) {
+  __shared__ f32x4_t part[kJoinSlices][kJoinQuads];
+  const int ql = threadIdx.x % kJoinQuads, sl = threadIdx.x / kJoinQuads;
+  const int64_t i = ((int64_t)blockIdx.x * kJoinQuads + ql) * 4;
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (i < n) {
+    constexpr int kFlight = 8;
+    for (int s = sl; s < splits; s += kJoinSlices * kFlight) {
+      f32x4_t u[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int r = s + j * kJoinSlices;
+        u[j] = r < splits ? *(const f32x4_t*)(planes + r * plane + i) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) v += u[j];
+    }
+  }
+  part[sl][ql] = v;
+  __syncthreads();
+  if (sl || i >= n) return;
+#pragma unroll
+  for (int s = 1; s < kJoinSlices; ++s) v += part[s][ql];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (i + q >= n) break;
+    if constexpr (DT == ML_F32) ((float*)c)[i + q] = v[q];
+    else ((uint16_t*)c)[i + q] = (uint16_t)GMma<DT>::pack(v[q], 0.f);
+  }
+}
+
 }  // namespace ml

@@ -25,7 +25,7 @@ from .head.layer_norm import LayerNormFunction, layer_norm
 from .head.rms_norm import RMSNormFunction, rms_norm, rms_norm_mx
 from .head.experts import (ExpertOrder, FromExpertsFunction, ToExpertsFunction, from_experts, sort_by_expert,
                            to_experts)
-from .head.mx import mx_quantize
+from .head.mx import grouped_matmul_mx, mx_quantize
 from .losses import sigmoid_cross_entropy_loss, dice_loss
 
 __all__ = [
@@ -60,4 +60,5 @@ __all__ = [
     "to_experts",
     "from_experts",
     "mx_quantize",
+    "grouped_matmul_mx",
 ]
