@@ -590,8 +590,13 @@ static __device__ __align__(16) unsigned char g_zeros[16];  // the reduced index
 #pragma clang diagnostic ignored "-Winline-asm"
 template <int N>
 __device__ __forceinline__ void ring_loads(const char* base, const uint32_t (&off)[N], uint32_t lds) {
-  static_assert(N == 2 || N == 4, "loads of an operand");
-  if constexpr (N == 2)
+  static_assert(N == 1 || N == 2 || N == 4, "loads of an operand");
+  if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(off[0]), "s"(base)
+                 : "memory", "m0");
+  else if constexpr (N == 2)
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
         "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"

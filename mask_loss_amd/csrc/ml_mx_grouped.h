@@ -275,4 +275,425 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_kernel(MxArgs x) {
   }
 }
 
+// ---- scales in whole fours: stages filled by direct loads into LDS ---------------------
+// Where K is a multiple of 128 (and the scales start on 4-byte boundaries), a row's four scales of a fragment are one
+// dword, and everything of a stage comes by direct loads: grouped_ring_kernel's ring (there: stages, persistent workgroups, turns,
+// waits), with the dwords of the stage's scales behind its codes, [128 of the reduced index][rows of both operands].
+
+// Four bytes from base + off, or from p, of each lane to LDS at `lds` + 4 lane; base as ring_loads'.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void ring_dwords(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void ring_dwords(const char* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds), "v"(p)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// One operand of a stage, filled by NW waves.
+template <int F, int R, int NW, int BK>
+struct MxRing : RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)> {
+  using O = typename RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)>::O;
+  // 128 values from 128 s on, of rows row0 .. (the scale is elsewhere)
+  static __device__ __forceinline__ MxFrag<F> frag(const unsigned char* lds, int row0, int s) {
+    MxFrag<F> f;
+    f.v[0] = O::frag(lds, row0, F == ML_MX_E4M3 ? 0 : s);
+    if constexpr (F == ML_MX_E4M3) f.v[1] = O::frag(lds, row0, 1);
+    f.scale = 0;
+    return f;
+  }
+};
+
+// The scales of 64 rows: from lane l's dword of row l (its blocks 0 .. 3) to lane l's four bytes of block l / 16 in rows
+// l % 16 + 16 j, of which the instruction is told byte j.  A transpose among the lanes l % 16 + 16 g: neighbours g, g ^ 1
+// exchange their dwords, each keeps the bytes of blocks g and g ^ 2 of the two, and hands the latter to g ^ 2.
+struct MxTurn {
+  uint32_t mine, theirs;  // selectors of v_perm_b32
+  __device__ __forceinline__ MxTurn() {
+    const uint32_t g = (threadIdx.x >> 4) & 3, o = g ^ 2;
+    mine = g | (4 + g) << 8 | o << 16 | (4 + o) << 24;
+    // of the pairs 0, 1 and 2, 3: what they kept, or what they handed over
+    theirs = g < 2 ? 0x07060100u : 0x05040302u;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t d) const {
+    const auto n = __builtin_amdgcn_permlane16_swap(d, d, false, false);  // the even and the odd neighbour's
+    const uint32_t u = __builtin_amdgcn_perm(n[1], n[0], mine);
+    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_amdgcn_perm(p[1], p[0], theirs);
+  }
+};
+// (byte: an immediate of the instruction, a constant where the loops are unrolled)
+template <int FA, int FB, int BA, int BB>
+__device__ __forceinline__ f32x4_t mx_mma_at(const MxFrag<FA>& a, const MxFrag<FB>& b, uint32_t sa, uint32_t sb, const f32x4_t& c) {
+  constexpr int ca = FA == ML_MX_E4M3 ? 0 : 4, cb = FB == ML_MX_E4M3 ? 0 : 4;
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.wide(), b.wide(), c, ca, cb, BA, (int)sa, BB, (int)sb);
+}
+template <int FA, int FB>
+__device__ __forceinline__ f32x4_t mx_mma_at(int ba, int bb, const MxFrag<FA>& a, const MxFrag<FB>& b, uint32_t sa, uint32_t sb,
+                                             const f32x4_t& c) {
+  switch (ba * 4 + bb) {
+#define ML_MX_CASE(i) case i: return mx_mma_at<FA, FB, i / 4, i % 4>(a, b, sa, sb, c);
+    ML_MX_CASE(0) ML_MX_CASE(1) ML_MX_CASE(2) ML_MX_CASE(3) ML_MX_CASE(4) ML_MX_CASE(5) ML_MX_CASE(6) ML_MX_CASE(7)
+    ML_MX_CASE(8) ML_MX_CASE(9) ML_MX_CASE(10) ML_MX_CASE(11) ML_MX_CASE(12) ML_MX_CASE(13) ML_MX_CASE(14)
+#undef ML_MX_CASE
+    default: return mx_mma_at<FA, FB, 3, 3>(a, b, sa, sb, c);
+  }
+}
+
+// Order of a sub-step's LDS reads (the scales' first, RB and RA for a fragment of either operand) and products (N for each
+// of M fragments).
+template <int RS, int RB, int RA, int N, int M>
+__device__ __forceinline__ void mx_interleave() {
+  constexpr int kMfma = 0x8, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, RS, 0);
+  interleave<RB, RA, N, M, 1>();
+}
+
+// What a workgroup is to do next, as rows_work tells it, for 32 of its work items at a time, one to a lane: a search
+// through the segments and divisions are a microsecond's wait, which the others of a tile would be waiting for.
+struct alignas(16) MxItem {
+  int m0, n0, mlim, w;
+  int block;       // of a split tile's parts, or -1
+  int steps, k;    // k: where the reduced index starts
+  int kind;        // 1: rows of several groups (merged_row); 2: rows in no group, zeros
+};
+constexpr int kMxItems = 32;
+
+__device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, const int* t, int tiles, const RingShare& share,
+                                          int next, int bm, int bn, int bk) {
+  int id = share.start + next, part = 0, parts = 1;
+  MxItem it;
+  it.block = -1;
+  if (next >= share.whole) {  // a part of one of the last tiles
+    const int p = next - share.whole, r = p / share.parts;
+    id = share.start + share.whole + r;
+    parts = share.parts;
+    part = p - r * parts;
+    if (parts > 1) it.block = p;
+  }
+  const int band = div_by(id >> 2, a.cols);  // kBand = 4
+  const int height = min(kBand, tiles - band * kBand);
+  const int rest = id - band * kBand * a.cols.d, y = rest / height;
+  it.n0 = y * bn;
+  const int tile = band * kBand + rest - y * height;
+  int q = 0, end = a.segments + 1;  // the first segment whose tiles end behind this one
+  while (q < end) {
+    const int mid = (q + end) >> 1;
+    if (t[mid] <= tile) q = mid + 1;
+    else end = mid;
+  }
+  int r0, r1;
+  segment(a, e, q, r0, r1);
+  const bool zero = q >= a.segments;
+  it.m0 = r0 + (tile - (q ? t[q - 1] : 0)) * bm;
+  it.mlim = r1 - it.m0;
+  it.w = zero ? 0 : a.merged ? q : div_by(q, a.layers);
+  it.kind = zero ? 2 : a.merged ? 1 : 0;
+  const int steps = zero ? 0 : (int)((uint32_t)(a.K + bk - 1) / (uint32_t)bk), s0 = part_start(steps, part, parts);
+  it.steps = part_start(steps, part + 1, parts) - s0;
+  it.k = s0 * bk;
+  return it;
+}
+
+// Template arguments as mx_kernel's; stages of BK values, OCC workgroups to a compute unit.  SW: 16, the scales come 512 of the reduced
+// index at a time, 16 bytes of a row with the first stage of them (K a multiple of 512, scales on 16-byte boundaries), in two
+// slots of [row][16]; or 4, those of a stage with it, [128 of the reduced index][row][4].  A row's scales are far from
+// the next one's, so a load of 64 rows takes 64 cache lines however few bytes of each: 8,192 x 8,192 x 8,192 in e2m1 took 396 us with
+// a stage's dwords, 303 with no scale loads, 359 with these.
+template <int FA, int FB, int OUT, int BM, int BN, int WM, int WN, int BK, int OCC, int SW>
+__global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void mx_ring_kernel(MxArgs x) {
+  constexpr int NS = 2, NW = WM * WN, H = BK / 128, TM = BM / WM / 16, TN = BN / WN / 16;
+  using OA = MxRing<FA, BM, NW, BK>;
+  using OB = MxRing<FB, BN, NW, BK>;
+  constexpr int SUPER = SW == 16 ? 512 / BK : 1;  // stages that share their scales' loads, and turns of the unrolled loop
+  constexpr int CODES = OA::BYTES + OB::BYTES, ROWS = BM + BN;
+  constexpr int SLOT = SW == 16 ? ROWS * 16 : H * ROWS * 4, SLOTS = SW == 16 ? 2 : NS;
+  constexpr int UNITS = SLOT / (64 * SW), S = (UNITS + NW - 1) / NW;  // scale loads of a slot, and of a wave
+  constexpr int ST = TM * TN / (OUT == ML_F32 ? 1 : 2);               // stores of a full tile
+  static_assert(TN % 4 == 0 && TM % 4 == 0, "whole scale fragments");
+  static_assert(BM % 64 == 0 && BN % 64 == 0, "whole scale loads of an operand");
+  static_assert(SW == 4 || SUPER % NS == 0, "a stage's slot is known where the loop is unrolled");
+  __shared__ __align__(1024) unsigned char lds[NS * CODES];
+  __shared__ __align__(1024) unsigned char slots[SLOTS * SLOT];
+  __shared__ MxItem queue[2 * kMxItems];
+  extern __shared__ int e[];
+  const GroupedArgs& a = x.g;
+
+  group_edges(a, e);
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  int* t = e + a.groups + 1;
+  const int tiles = segment_tiles(a, e, t, BM);
+  const int xcd = (int)blockIdx.x % kXcds, turns = (int)gridDim.x / kXcds, first = (int)blockIdx.x / kXcds;
+  const RingShare share = ring_share(a, tiles * a.cols.d, xcd, turns);
+  const int last = share.whole + share.rest * share.parts;
+  if (first >= last) return;
+  const int count = (last - first + turns - 1) / turns;
+  auto item = [&](int n) {
+    MxItem it = queue[n % (2 * kMxItems)];
+    int* f = (int*)&it;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = uniform(f[i]);
+    return it;
+  };
+
+  // ---- loads
+  OA oa;
+  OB ob;
+  const uint32_t ring = (uint32_t)(uintptr_t)(lds_void_t*)lds, sring = (uint32_t)(uintptr_t)(lds_void_t*)slots;
+  int opened = 0, left = 0, kleft = 0;         // stages left of the item being loaded, and its values left
+  int sslot = 0;                               // the next slot of scales
+  bool whole_a = false, whole_b = false;       // oa's, ob's offsets are those of a whole tile
+  const char *pa = nullptr, *pb = nullptr;     // the next stage's codes
+  const char *psa = nullptr, *psb = nullptr;   // and the next scales
+  uint32_t soff[S];                            // bytes of this lane's row of each of the wave's units
+  auto open_item = [&]() {
+    if (opened >= count) {  // nothing more: zeros
+      left = INT32_MAX - 2 * SUPER;
+      kleft = 0;
+      return;
+    }
+    if (opened % kMxItems == 0) {  // (every wave for itself, the same values)
+      if (lane < min(kMxItems, count - opened))
+        queue[(opened + lane) % (2 * kMxItems)] = mx_item(a, e, t, tiles, share, first + (opened + lane) * turns, BM, BN, SUPER * BK);
+    }
+    const MxItem it = item(opened++);
+    left = max(it.steps, 1) * SUPER;  // (nothing to reduce: stages of zeros)
+    kleft = it.kind == 2 ? 0 : a.K - it.k;
+    const bool mapped = it.kind == 1;
+    pa = (const char*)a.a + (mapped ? (int64_t)0 : (int64_t)it.m0 * a.lda) * 2 + mx_bytes(FA, it.k);
+    pb = (const char*)a.b + ((int64_t)it.w * a.bstride + (int64_t)it.n0 * a.ldb) * 2 + mx_bytes(FB, it.k);
+    psa = (const char*)x.sa + (mapped ? (int64_t)0 : it.m0 * x.sld) + it.k / kMxBlock;
+    psb = (const char*)x.sb + ((int64_t)it.w * a.N + it.n0) * x.sld + it.k / kMxBlock;
+    const bool wa = !mapped && it.mlim >= BM, wb = a.N - it.n0 >= BN;
+    if (wa && wb && whole_a && whole_b) return;
+    if (mapped) oa.aim(a.lda, it.mlim, wave, [&](int r) { return merged_row(a, e, it.w, it.m0 + r); });
+    else oa.aim(a.lda, it.mlim, wave, [](int r) { return r; });
+    ob.aim(a.ldb, a.N - it.n0, wave, [](int r) { return r; });
+    whole_a = wa;
+    whole_b = wb;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int row = min(wave * S + i, UNITS - 1) * 64 % ROWS + lane;  // of both operands
+      int r = row < BM ? min(row, it.mlim - 1) : min(row - BM, a.N - it.n0 - 1);
+      if (mapped && row < BM) r = merged_row(a, e, it.w, it.m0 + r);
+      soff[i] = (uint32_t)r * (uint32_t)x.sld;
+    }
+  };
+  // The next stage's loads, into this slot of the ring (zeros where nothing is left); `scales`: it is the first one of its
+  // scales, and perhaps of an item.
+  auto load = [&](int stage, bool scales) {
+    if (scales) {
+      if (left == 0) open_item();
+      left -= SUPER;
+      const uint32_t to = sring + (SW == 16 ? sslot : stage) * SLOT;
+      sslot ^= 1;
+      if (SW == 16 ? kleft > 0 : kleft >= BK) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const int u = min(wave * S + i, UNITS - 1);
+          const char* base = uniform((u * 64 % ROWS < BM ? psa : psb) + (SW == 16 ? 0 : 4 * (u * 64 / ROWS)));
+          if constexpr (SW == 16) {
+            const uint32_t o[1] = {soff[i]};
+            ring_loads(base, o, to + u * 1024);
+          } else {
+            ring_dwords(base, soff[i], to + u * 256);
+          }
+        }
+        psa += SUPER * BK / kMxBlock;
+        psb += SUPER * BK / kMxBlock;
+      } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const int u = min(wave * S + i, UNITS - 1), h = u * 64 / ROWS;
+          if constexpr (SW == 16) ring_load((const char*)g_zeros, to + u * 1024);
+          else if (h * 128 < kleft) ring_dwords(uniform((u * 64 % ROWS < BM ? psa : psb) + 4 * h), soff[i], to + u * 256);
+          else ring_dwords((const char*)g_zeros, to + u * 256);
+        }
+      }
+    }
+    const uint32_t to = ring + stage * CODES;
+    if (kleft >= BK) {
+      ring_loads(uniform(pa), oa.off, to + wave * OA::PER * 1024);
+      ring_loads(uniform(pb), ob.off, to + OA::BYTES + wave * OB::PER * 1024);
+      pa += mx_bytes(FA, BK);
+      pb += mx_bytes(FB, BK);
+    } else {
+      oa.load(pa, mx_bytes(FA, kleft) / 2, to, wave);
+      ob.load(pb, mx_bytes(FB, kleft) / 2, to + OA::BYTES, wave);
+    }
+    kleft -= BK;
+  };
+#pragma unroll
+  for (int s = 0; s < NS; ++s) load(s, s % SUPER == 0);
+
+  // ---- products
+  const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+  const MxTurn turn;
+  int at = 0;  // the slot of the scales in turn
+  auto frag_a = [&](int stage, int j, int h) { return OA::frag(lds + stage * CODES, wm + 16 * j, h); };
+  auto frag_b = [&](int stage, int i, int h) { return OB::frag(lds + stage * CODES + OA::BYTES, wn + 16 * i, h); };
+  auto scale = [&](int stage, int part, int row0, int h) {  // lane l's: row row0 + l, its four of the sub-step
+    const unsigned char* p = SW == 16 ? slots + at * SLOT + (row0 + lane) * 16 + (part * H + h) * 4
+                                      : slots + stage * SLOT + (h * ROWS + row0 + lane) * 4;
+    return *(const uint32_t*)p;
+  };
+  MxFrag<FA> fa[TM];
+  MxFrag<FB> fb[TN], fn[TN];
+  uint32_t sa[TM / 4], sb[TN / 4];
+  ring_wait<OA::PER + OB::PER>();
+#pragma unroll
+  for (int i = 0; i < TN; ++i) fb[i] = frag_b(0, i, 0);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fa[i] = frag_a(0, i, 0);
+#pragma unroll
+  for (int i = 0; i < TM / 4; ++i) sa[i] = turn(scale(0, 0, wm + 64 * i, 0));
+#pragma unroll
+  for (int i = 0; i < TN / 4; ++i) sb[i] = turn(scale(0, 0, BM + wn + 64 * i, 0));
+  int cur = 0;     // the stage in turn (SW = 4)
+  bool credit = false;  // a stage's loads were issued before the last tile's stores
+  for (int n = 0; n < count; ++n) {
+    const MxItem it = item(n);
+    f32x4_t acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // products of the fragments in b and fa, and reads of those of the stage's sub-step h into bn and, as they
+    // fall free, fa
+    auto sub_step = [&](const MxFrag<FB>(&b)[TN], MxFrag<FB>(&bn)[TN], int stage, int part, int h) {
+      uint32_t na[TM / 4], nb[TN / 4];
+#pragma unroll
+      for (int i = 0; i < TM / 4; ++i) na[i] = scale(stage, part, wm + 64 * i, h);
+#pragma unroll
+      for (int i = 0; i < TN / 4; ++i) nb[i] = scale(stage, part, BM + wn + 64 * i, h);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) bn[i] = frag_b(stage, i, h);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) acc[i][j] = mx_mma_at(i % 4, j % 4, b[i], fa[j], sb[i / 4], sa[j / 4], acc[i][j]);
+        fa[j] = frag_a(stage, j, h);
+      }
+#pragma unroll
+      for (int i = 0; i < TM / 4; ++i) sa[i] = turn(na[i]);
+#pragma unroll
+      for (int i = 0; i < TN / 4; ++i) sb[i] = turn(nb[i]);
+      mx_interleave<TM / 4 + TN / 4, FB == ML_MX_E4M3 ? 2 : 1, FA == ML_MX_E4M3 ? 2 : 1, TN, TM>();
+    };
+    for (int s = max(it.steps, 1); s > 0; --s) {
+#pragma unroll
+      for (int part = 0; part < SUPER; ++part) {
+        const int stage = SW == 16 ? part % NS : cur, next = SW == 16 ? (part + 1) % NS : cur ^ 1;
+        if constexpr (H == 2) sub_step(fb, fn, stage, part, 1);
+        // the products so far stay on this side of the wait: sunk to the next, they would keep both fragments
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
+        // the next stage's loads were issued before a full tile's stores, where they came between
+        if (part == 0 && credit) ring_wait<(ST < 63 ? ST : 63)>();
+        else ring_wait<0>();
+        if (part == 0) credit = false;
+        load(stage, (part + NS) % SUPER == 0);
+        if (part + 1 == SUPER) at ^= 1;
+        cur ^= 1;
+        if (H == 2 || part % 2 == 1) {
+          sub_step(fn, fb, next, (part + 1) % SUPER, 0);
+        } else {
+          sub_step(fb, fn, next, (part + 1) % SUPER, 0);
+          if constexpr (SUPER % 2 == 1)
+#pragma unroll
+            for (int i = 0; i < TN; ++i) fb[i] = fn[i];
+        }
+      }
+    }
+
+    // lane l holds columns 4 (l / 16) .. + 3 of row l % 16 of each 16 x 16 tile
+    const int m0 = it.m0, n0 = it.n0, tm = it.mlim, iw = it.w, block = it.block;
+    const bool mapped = it.kind == 1;
+    const int tn = a.N - n0;
+    const bool full = tm >= BM && tn >= BN && block < 0;
+    int el = lane;
+    asm("" : "+v"(el));  // (as in grouped_ring_kernel: not known to be the same for every tile)
+    const int mr = wm + (el & 15), g = el >> 4;
+    auto row_start = [&](int j) {  // of the lane's row in row tile j
+      const int r = mr + 16 * j;
+      return n0 + (int64_t)(mapped ? merged_row(a, e, iw, m0 + min(r, tm - 1)) : m0 + r) * a.ldc;
+    };
+    if (block >= 0) {  // in the order of the registers (grouped_tail_kernel)
+      f32x4_t* c = (f32x4_t*)a.parts + ((int64_t)(xcd * turns + block) * NW + wave) * (TN * TM * 64) + el;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) c[(i * TM + j) * 64] = acc[i][j];
+    } else if constexpr (OUT == ML_F32) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        float* c = (float*)a.c + row_start(j) + wn + 4 * g;
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          if (full) {
+            *(f32x4_loose*)(c + 16 * i) = acc[i][j];
+            continue;
+          }
+          const int room = mr + 16 * j < tm ? tn - (wn + 16 * i + 4 * g) : 0;
+          if (room >= 4) {
+            *(f32x4_loose*)(c + 16 * i) = acc[i][j];
+          } else {
+#pragma unroll
+            for (int q4 = 0; q4 < 3; ++q4)
+              if (q4 < room) c[16 * i + q4] = acc[i][j][q4];
+          }
+        }
+      }
+    } else {
+      // two tiles' columns change places between lane groups 0 and 1, 2 and 3, so that a lane
+      // has eight consecutive ones: of the first tile in even groups, of the second in odd ones
+      const int col = wn + 16 * (g & 1) + 8 * (g >> 1);
+      auto eight = [&](int i, int j) {
+        const f32x4_t u = acc[i][j], v = acc[i + 1][j];
+        const auto lo = __builtin_amdgcn_permlane16_swap(GMma<OUT>::pack(u[0], u[1]), GMma<OUT>::pack(v[0], v[1]), false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap(GMma<OUT>::pack(u[2], u[3]), GMma<OUT>::pack(v[2], v[3]), false, false);
+        return u32x4_t{lo[0], hi[0], lo[1], hi[1]};
+      };
+      if (full) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          uint16_t* c = (uint16_t*)a.c + row_start(j) + col;
+#pragma unroll
+          for (int i = 0; i < TN; i += 2) *(u32x4_loose*)(c + 16 * i) = eight(i, j);
+          __builtin_amdgcn_sched_barrier(0);  // one row tile's conversions at a time: registers
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          uint16_t* c = (uint16_t*)a.c + row_start(j) + col;
+#pragma unroll
+          for (int i = 0; i < TN; i += 2) {
+            const u32x4_t o = eight(i, j);
+            const int room = mr + 16 * j < tm ? tn - (col + 16 * i) : 0;
+            if (room >= 8) {
+              *(u32x4_loose*)(c + 16 * i) = o;
+            } else {
+#pragma unroll
+              for (int q8 = 0; q8 < 7; ++q8)
+                if (q8 < room) c[16 * i + q8] = (uint16_t)(o[q8 / 2] >> (16 * (q8 & 1)));
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    credit = full;
+  }
+  ring_wait<0>();  // the last loads end before the LDS goes to another workgroup
+}
+
 }  // namespace ml

@@ -13,17 +13,25 @@ constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 byte
 constexpr int64_t kUnits = 256;
 
 // Tiles: few rows to a group (64 where the rows are e2m1 and the matrix e4m3: a chunk for every thread), or many.
+// Many rows take the ring where K and the scales' alignment let them (us, the ring / mx_kernel; e2m1 by e2m1 unless named):
+// 16,384 rows in 16 groups, K = 1,024, N = 4,096 62 / 102, e4m3 by e2m1 83 / 128, e4m3 by e4m3 108 / 159; 4,096 rows in 8 groups, K =
+// 1,024, N = 2,736, e4m3 by e2m1 24 / 31; one matrix 8,192 x 8,192 x 8,192 359 / 446.  Larger tiles of the ring move fewer
+// bytes through LDS, but a tile's stores wait for less beside them: 128 x 256 and 256 x 256 on 8 waves take 68 and 80 for the
+// first of these (and 325 and 283 for the last, alone).
 constexpr int few_rows(int fa, int fb) { return fa == ML_MX_E2M1 && fb == ML_MX_E4M3 ? 64 : 32; }
-constexpr int kColumns = 128, kManyRows = 128;
+constexpr int kColumns = 128, kManyRows = 128, kRingSlots = 512;
+constexpr size_t kRingParts = (size_t)kRingSlots * kManyRows * kColumns * sizeof(float);
 
 struct MxPlan {
   bool few, merged;
+  int ring;  // 0, or the bytes of a scale load: 4, 16
   int bm, splits;
   int64_t bound, plane;
   size_t bytes;
 };
 
-int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, bool equal, MxPlan& p) {
+// aligned: bytes that x_scales' and weight_scales' addresses are multiples of (16 at most); equal: without offsets
+int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, int aligned, bool equal, MxPlan& p) {
   p = MxPlan{};
   if (!s || s->rows < 0 || s->K < 0 || s->N < 0 || s->groups < 1 || s->matrices < 1 || s->groups % s->matrices)
     return fail(ML_EINVAL, "grouped_matmul_mx: invalid shape (groups must be a positive multiple of the matrices)");
@@ -43,18 +51,28 @@ int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, bool equal, MxPl
   const double each = (double)s->rows / used;
   p.few = each <= 32.0;
   p.bm = p.few ? few_rows(fa, fb) : kManyRows;
-  const int64_t columns = ceil_div(s->N, kColumns), steps = std::max<int64_t>(1, ceil_div(s->K, mx_step(fa, fb)));
+  p.ring = p.few || mx_exact(fa, fb, out) ? 0 : s->K % 512 == 0 && aligned >= 16 ? 16 : s->K % 128 == 0 && aligned >= 4 ? 4 : 0;
+  const int64_t columns = ceil_div(s->N, kColumns);
+  // values of a part of a reduction, at least one turn of the kernel's loop
+  const int64_t step = p.ring == 16 ? 512 : mx_step(fa, fb), steps = std::max<int64_t>(1, ceil_div(s->K, step));
   const double x = each / p.bm, rows = used * (equal || segments == 1 ? std::ceil(x) : std::max(1.05, x + 0.5));
   // parts of each tile's reduction where the tiles leave slots without work
-  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 4, 64));
-  const int slots = (int)kUnits * (p.few ? 4 : 2);
+  const int slots = p.ring ? kRingSlots : (int)kUnits * (p.few ? 4 : 2);
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(p.ring == 16 ? steps : steps / 4, 64));
   p.splits = std::max(1, std::min((int)(slots / std::max(1.0, rows * columns)), most));
   const int64_t tiles = (s->rows / p.bm + std::min(segments + 2, s->rows)) * columns;
-  p.bound = tiles * p.splits;
-  p.plane = ceil_div(s->rows * s->N, 4) * 4;
-  p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
-  // a workgroup to an item, and a launch has fewer than 2^32 threads
-  if (p.bound > (int64_t)UINT32_MAX / 256 - 8) return fail(ML_EUNSUPPORTED, "grouped_matmul_mx: too many tiles");
+  if (p.ring) {
+    if (p.splits > 1) p.splits = s->N % 4 == 0 ? most : 1;  // (the counts on the GPU decide; joined by whole fours)
+    p.bound = tiles;
+    p.bytes = p.splits > 1 ? kRingParts : 256;
+  } else {
+    p.bound = tiles * p.splits;
+    p.plane = ceil_div(s->rows * s->N, 4) * 4;
+    p.bytes = p.splits > 1 ? align256((size_t)p.splits * p.plane * sizeof(float)) : 256;
+  }
+  // ids are 32-bit; mx_kernel has a workgroup to an item, and a launch fewer than 2^32 threads
+  if (p.bound > (p.ring ? (int64_t)INT32_MAX : (int64_t)UINT32_MAX / 256) - 8)
+    return fail(ML_EUNSUPPORTED, "grouped_matmul_mx: too many tiles");
   return ML_OK;
 }
 
@@ -62,7 +80,24 @@ template <int FA, int FB, int OUT>
 int mx_launch(const ml_grouped_shape* s, const MxPlan& p, MxArgs& x, hipStream_t st) {
   ProfScope ps("grouped_matmul_mx", st);
   const size_t lds = (2 * (size_t)x.g.groups + 3) * sizeof(int);  // edges, tiles of the segments
-  const dim3 grid((unsigned)(ceil_div(p.bound, kXcds) * kXcds)), blk(256);
+  const dim3 blk(256);
+  if constexpr (!mx_exact(FA, FB, OUT)) {
+    if (p.ring) {
+      // persistent workgroups, all that fit where tiles may be split
+      const int64_t items = ceil_div(p.bound, kXcds) * kXcds;
+      const dim3 grid((unsigned)(p.splits > 1 ? kRingSlots : std::min<int64_t>(items, kRingSlots)));
+      constexpr int BK = mx_step(FA, FB);
+      if (p.ring == 16)
+        hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 16>), grid, blk, lds, st, x);
+      else
+        hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 4>), grid, blk, lds, st, x);
+      const int rc = check_launch("grouped_matmul_mx");
+      if (rc || p.splits == 1) return rc;
+      hipLaunchKernelGGL(grouped_tail_kernel<OUT>, grid, blk, lds, st, x.g, 0, kManyRows, kColumns, 2, (int)grid.x / kXcds);
+      return check_launch("grouped_matmul_mx");
+    }
+  }
+  const dim3 grid((unsigned)(ceil_div(p.bound, kXcds) * kXcds));
   if (p.few)
     hipLaunchKernelGGL((mx_kernel<FA, FB, OUT, few_rows(FA, FB), kColumns, 1, 4>), grid, blk, lds, st, x);
   else
@@ -90,10 +125,10 @@ int mx_out(const ml_grouped_shape* s, const MxPlan& p, MxArgs& x, int out, hipSt
 using namespace ml;
 
 extern "C" size_t ml_grouped_matmul_mx_workspace_size(const ml_grouped_shape* s, int x_format, int weight_format, int dtype) {
-  size_t most = 256;  // with and without offsets (a size of 0 stands for a refused shape)
-  for (int i = 0; i < 2; ++i) {
+  size_t most = 256;  // with and without offsets, for any alignment (a size of 0 stands for a refused shape)
+  for (int i = 0; i < 6; ++i) {
     MxPlan p;
-    if (mx_plan(s, x_format, weight_format, dtype, i != 0, p)) return 0;
+    if (mx_plan(s, x_format, weight_format, dtype, i / 2 == 0 ? 1 : i / 2 == 1 ? 4 : 16, i % 2 != 0, p)) return 0;
     most = std::max(most, p.bytes);
   }
   return most;
@@ -104,7 +139,8 @@ extern "C" int ml_grouped_matmul_mx(const ml_grouped_shape* s, int x_format, con
                                     const int64_t* offsets, int dtype, void* y, void* workspace, size_t workspace_bytes,
                                     ml_stream_t stream) {
   MxPlan p;
-  const int rc = mx_plan(s, x_format, weight_format, dtype, !offsets, p);
+  const uintptr_t at = (uintptr_t)x_scales | (uintptr_t)weight_scales;
+  const int rc = mx_plan(s, x_format, weight_format, dtype, at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 1, !offsets, p);
   if (rc) return rc;
   if (s->rows == 0 || s->N == 0) return ML_OK;
   if (!offsets && s->rows % s->groups)
@@ -133,6 +169,7 @@ extern "C" int ml_grouped_matmul_mx(const ml_grouped_shape* s, int x_format, con
   a.segments = p.merged ? a.matrices : a.groups;
   a.merged = p.merged;
   a.splits = p.splits;
+  a.fewest = 2;
   a.plane = p.plane;
   a.c = y;
   a.parts = (float*)workspace;

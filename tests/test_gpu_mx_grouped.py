@@ -117,40 +117,46 @@ def test_normal_values(dt, fx, fw, rows, N, K, offsets):
     assert off <= (1e-4 if drops else 1e-6) + STEP[TDT[dt]]
 
 
+# K: any blocks, whole 128 and whole 512, which have kernels of their own
+@pytest.mark.parametrize("K", [192, 384, 512])
 @pytest.mark.parametrize("fx,fw", PAIRS)
 @pytest.mark.parametrize("N", [1, 2, 3, 5, 15, 16, 17, 64, 127, 128, 130, 255, 384, 1000])
-def test_columns(fx, fw, N):
+def test_columns(fx, fw, N, K):
     for rows, offsets in ((9, [0, 4, 9]), (150, [0, 70, 150])):
-        x, w = operand((rows, 192), fx, N, True, (125, 130)), operand((2, N, 192), fw, N + 1, True, (125, 130))
+        x, w = operand((rows, K), fx, N, True, (125, 130)), operand((2, N, K), fw, N + 1, True, (125, 130))
         for dtype in (torch.bfloat16, torch.float32):
             compare(x, w, offsets, dtype, False)
 
 
 GROUPS = [([0, 1], 1, 1), ([0, 0, 1], 1, 2), ([0, 0, 0, 0], 5, 3), ([2, 5, 9], 12, 2), ([0, 128, 256], 256, 2),
           ([0, 129, 257, 300], 310, 3), ([5, 3, 40, 20, 60], 50, 4), ([-4, 10, 2 ** 40], 33, 2), ([0, 40, 80, 120, 160], 170, 2),
-          ([10, 60, 61, 61, 150, 200, 333], 340, 3), ([0] + [1] * 40, 3, 40), (list(range(65)), 64, 64), ([0, 500], 500, 1)]
+          ([10, 60, 61, 61, 150, 200, 333], 340, 3), ([0] + [1] * 40, 3, 40), (list(range(65)), 64, 64), ([0, 500], 500, 1),
+          ([0, 90, 90, 300, 420, 600, 600, 777, 900], 1000, 2), (list(range(0, 3001, 50)), 3010, 60)]
 
 
+@pytest.mark.parametrize("K", [160, 256, 512])
 @pytest.mark.parametrize("fx,fw", PAIRS)
 @pytest.mark.parametrize("offsets,rows,M", GROUPS)
-def test_groups(fx, fw, offsets, rows, M):
+def test_groups(fx, fw, offsets, rows, M, K):
     """Empty groups, rows before the first and behind the last (zeros), borders that decrease or lie outside, groups
     that share a matrix, one group, many."""
-    x, w = operand((rows, 160), fx, rows, True, (125, 130)), operand((M, 72, 160), fw, M, True, (125, 130))
+    x, w = operand((rows, K), fx, rows, True, (125, 130)), operand((M, 72, K), fw, M, True, (125, 130))
     y = compare(x, w, offsets, torch.bfloat16, False)
     e = edges(offsets, rows)
     assert not y[:e[0]].any() and not y[e[-1]:].any()
 
 
 @pytest.mark.parametrize("fx,fw", PAIRS)
+@pytest.mark.parametrize("K", [96, 128, 1024])
 @pytest.mark.parametrize("G,n,M", [(1, 1, 1), (4, 5, 2), (6, 100, 3), (3, 130, 3), (2, 0, 2)])
-def test_equal_groups(fx, fw, G, n, M):
-    x, w = operand((G, n, 96), fx, 5, True, (125, 130)), operand((M, 50, 96), fw, 6, True, (125, 130))
+def test_equal_groups(fx, fw, G, n, M, K):
+    x, w = operand((G, n, K), fx, 5, True, (125, 130)), operand((M, 50, K), fw, 6, True, (125, 130))
     compare(x, w, None, torch.float16, False)
 
 
 @pytest.mark.parametrize("fx,fw", PAIRS)
-@pytest.mark.parametrize("rows,K,N", [(3, 8192, 64), (40, 16384, 20), (200, 8224, 96)])
+@pytest.mark.parametrize("rows,K,N", [(3, 8192, 64), (40, 16384, 20), (200, 8224, 96), (200, 8192, 96), (200, 8192, 97),
+                                      (130, 4224, 260), (300, 1024, 512)])
 def test_split_reductions(fx, fw, rows, K, N):
     """Few tiles and long reductions, which are split and joined."""
     x, w = operand((rows, K), fx, 7, True, (125, 130)), operand((1, N, K), fw, 8, True, (125, 130))
@@ -172,20 +178,39 @@ def test_scales(fx, fw, dt, rows):
         if lo == 0 and dt == "f32" and "e4m3" in (fx, fw):
             x[1].view(torch.uint8).clamp_(min=4)  # values below 2^-126 may count as zero
         compare(x, w, [0, rows], TDT[dt], drops)
-    x, w = operand((rows, 320), fx, 11, True), operand((2, 40, 320), fw, 12, True)
-    offsets = [1, rows // 2, rows - 2]
-    clean = call(x, w, offsets, TDT[dt])
-    for t, at in ((x, (2, 9)), (x, (0, 0)), (x, (rows - 1, 5)), (w, (1, 7, 3))):
-        b = t[1].view(torch.uint8).clone()
-        b[at] = 255
-        bad = (t[0], b.view(torch.float8_e8m0fnu))
-        y = call(bad, w, offsets, TDT[dt]) if t is x else call(x, bad, offsets, TDT[dt])
-        hit = torch.zeros_like(clean, dtype=torch.bool)
-        if t is w:
-            hit[offsets[1]:offsets[2], 7] = True
-        elif offsets[0] <= at[0] < offsets[2]:
-            hit[at[0]] = True
-        assert bool(torch.isnan(y[hit]).all()) and torch.equal(y[~hit], clean[~hit])
+    for K in (320, 384, 1024):
+        x, w = operand((rows, K), fx, 11, True), operand((2, 40, K), fw, 12, True)
+        offsets = [1, rows // 2, rows - 2]
+        clean = call(x, w, offsets, TDT[dt])
+        for t, at in ((x, (2, 9)), (x, (0, 0)), (x, (rows - 1, 5)), (w, (1, 7, 3))):
+            b = t[1].view(torch.uint8).clone()
+            b[at] = 255
+            bad = (t[0], b.view(torch.float8_e8m0fnu))
+            y = call(bad, w, offsets, TDT[dt]) if t is x else call(x, bad, offsets, TDT[dt])
+            hit = torch.zeros_like(clean, dtype=torch.bool)
+            if t is w:
+                hit[offsets[1]:offsets[2], 7] = True
+            elif offsets[0] <= at[0] < offsets[2]:
+                hit[at[0]] = True
+            assert bool(torch.isnan(y[hit]).all()) and torch.equal(y[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("fx,fw", PAIRS)
+@pytest.mark.parametrize("rows,K,N,groups", [(3000, 512, 4096, 5), (2500, 640, 2056, 3), (16640, 128, 16640, 1),
+                                             (16640, 512, 16640, 7)])
+def test_many_tiles(fx, fw, dt, rows, K, N, groups):
+    """Workgroups that make several tiles, and over 32 of them.  All scales 1 and few binades: every partial sum is
+    a float32, so any order gives the same result, rounded once."""
+    x, w = operand((rows, K), fx, 13, True, (127, 128)), operand((groups, N, K), fw, 14, True, (127, 128))
+    gen = torch.Generator().manual_seed(15)
+    cuts = torch.randint(0, rows + 1, (groups - 1,), generator=gen).sort().values.tolist()
+    offsets = [0, *cuts, rows - 7]
+    y = call(x, w, offsets, TDT[dt])
+    xv, wv = (mx.values(t[0]).float().cuda() for t in (x, w))
+    for g, (lo, hi) in enumerate(zip(edges(offsets, rows), edges(offsets, rows)[1:])):
+        assert torch.equal(y[lo:hi], (xv[lo:hi] @ wv[g].t()).to(TDT[dt])), g
+    assert not y[rows - 7:].any()
 
 
 def test_no_size():
@@ -201,10 +226,13 @@ def test_no_size():
 def test_layouts():
     """Codes on no 16-byte boundary, transposed ones, scales on an odd byte."""
     from mask_loss_amd.functions import grouped_matmul_mx
-    x, w = operand((40, 96), "e4m3", 2), operand((2, 24, 96), "e2m1", 3)
-    o = torch.tensor([0, 11, 40], device="cuda")
-    args = [t.cuda() for t in (*x, *w)]
-    want = grouped_matmul_mx(*args, o)
+    for K, rows in ((96, 40), (384, 150), (512, 150)):
+        x, w = operand((rows, K), "e4m3", 2, True), operand((2, 24, K), "e2m1", 3, True)
+        moves(grouped_matmul_mx, [t.cuda() for t in (*x, *w)], torch.tensor([0, 11, rows], device="cuda"))
+
+
+def moves(fn, args, o):
+    want = fn(*args, o)
 
     def odd(t):
         room = torch.empty(t.numel() + 1, dtype=torch.uint8, device="cuda")
@@ -215,9 +243,9 @@ def test_layouts():
         moved = list(args)
         moved[i] = odd(args[i])
         assert moved[i].data_ptr() % 16
-        assert torch.equal(grouped_matmul_mx(*moved, o), want)
+        assert torch.equal(fn(*moved, o), want)
         moved[i] = args[i].view(torch.uint8).transpose(-1, -2).contiguous().transpose(-1, -2).view(args[i].dtype)
-        assert torch.equal(grouped_matmul_mx(*moved, o), want)
+        assert torch.equal(fn(*moved, o), want)
 
 
 def test_past_32_bits():
