@@ -56,15 +56,22 @@ int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, int aligned, boo
   // values of a part of a reduction, at least one turn of the kernel's loop
   const int64_t step = p.ring == 16 ? 512 : mx_step(fa, fb), steps = std::max<int64_t>(1, ceil_div(s->K, step));
   const double x = each / p.bm, rows = used * (equal || segments == 1 ? std::ceil(x) : std::max(1.05, x + 0.5));
-  // parts of each tile's reduction where the tiles leave slots without work
-  const int slots = p.ring ? kRingSlots : (int)kUnits * (p.few ? 4 : 2);
-  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(p.ring == 16 ? steps : steps / 4, 64));
-  p.splits = std::max(1, std::min((int)(slots / std::max(1.0, rows * columns)), most));
+  // Parts of each tile's reduction where the tiles leave slots without work.  The ring takes 2 us for 512 values of a tile, and
+  // a join 4 us and what its parts' 64 KiB take to memory and back: as many parts as cost the least, if they cost less
+  // than none (512 x 8,192 x 1,024 25 us in parts, 43 whole; 512 x 4,096 x 4,096 29 in as many as fit, 25 whole).
+  const double all = std::max(1.0, rows * columns);
+  const int64_t fit = (int64_t)((p.ring ? kRingSlots : kUnits * (p.few ? 4 : 2)) / all);
+  if (p.ring) {
+    const double whole = 2.0 * s->K / 512, move = 0.026 * all;
+    const int64_t parts = std::min({fit, (int64_t)std::lround(std::sqrt(whole / move)), steps, (int64_t)64});
+    p.splits = parts > 1 && s->N % 4 == 0 && whole / parts + 4.0 + move * parts < whole ? (int)parts : 1;  // (joined by whole fours)
+  } else {
+    p.splits = (int)std::max<int64_t>(1, std::min({fit, steps / 4, (int64_t)64}));
+  }
   const int64_t tiles = (s->rows / p.bm + std::min(segments + 2, s->rows)) * columns;
   if (p.ring) {
-    if (p.splits > 1) p.splits = s->N % 4 == 0 ? most : 1;  // (the counts on the GPU decide; joined by whole fours)
     p.bound = tiles;
-    p.bytes = p.splits > 1 ? kRingParts : 256;
+    p.bytes = p.splits > 1 ? kRingParts : 256;  // (the counts on the GPU decide which tiles)
   } else {
     p.bound = tiles * p.splits;
     p.plane = ceil_div(s->rows * s->N, 4) * 4;
