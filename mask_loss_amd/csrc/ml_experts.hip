@@ -13,11 +13,11 @@
 // The sort is a counting sort: a place is the expert's first one, and the number of its assignments in the chunks before,
 // in the chunk's waves before and in the wave's lanes before (lanes of the same expert find each other by a ballot for each
 // bit of its number).  No atomics decide an order, so equal calls give equal bits.  Few assignments
-// take one workgroup and one launch, more take three: counts by chunk, their sums over the chunks, places.
+// take one workgroup and one launch, more take two or three: counts by chunk, their sums over many chunks, places.
 //
 // Everything else is bound by HBM: there reads each row once and writes it k times, back and the gradients
 // read or write each assignment's row once.  A token (back's gradient: an assignment) is a wave's or 16 lanes', which
-// pass over the row in 16-byte chunks; sums are float32 in the order of j, rounded once.
+// pass over the row in 16-byte chunks, at any alignment; sums are float32 in the order of j, rounded once.
 #include <algorithm>
 
 #include "ml_rows.h"
@@ -111,8 +111,35 @@ __global__ __launch_bounds__(64 * kSumWaves) void expert_sum_kernel(int* counts,
   }
 }
 
+// Of each key, all chunks' counts and those of the chunks before `mine`: a thread for every key and slice of the chunks,
+// up to eight loads in flight.
+constexpr int kFewKeys = 512, kFewChunks = 256;
+template <int W>
+__device__ __forceinline__ void chunk_sums(const int* counts, int chunks, int mine, int keys, int* all, int* prior) {
+  for (int i = threadIdx.x; i < keys; i += 64 * W) all[i] = prior[i] = 0;
+  __syncthreads();
+  const int slices = max(1, min(8, 64 * W / keys)), each = (chunks + slices - 1) / slices;
+  for (int i = threadIdx.x; i < keys * slices; i += 64 * W) {
+    const int slice = i / keys, key = i - slice * keys, c1 = min((slice + 1) * each, chunks);
+    int s = 0, before = 0;
+    for (int c = slice * each; c < c1; c += 8) {
+      int v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < c1 ? counts[(int64_t)(c + j) * keys + key] : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s += v[j];
+        before += c + j < mine ? v[j] : 0;
+      }
+    }
+    atomicAdd(&all[key], s);  // (whole numbers: any order)
+    atomicAdd(&prior[key], before);
+  }
+}
+
 // Places of a chunk's assignments, W waves of kSortItems each.  before: counts over the chunks before, and totals
-// (expert_sum_kernel); null where one workgroup has them all.
+// (expert_sum_kernel); or totals null: the chunks' counts themselves, of which there are few; both null where one workgroup
+// has all assignments.
 template <int W>
 __global__ __launch_bounds__(64 * W) void expert_place_kernel(const int64_t* ids, int64_t n, int experts, const int* before,
                                                               const int* totals, int64_t* order, int64_t* slots,
@@ -122,10 +149,14 @@ __global__ __launch_bounds__(64 * W) void expert_place_kernel(const int64_t* ids
   const int keys = experts + 1, stride = (keys + 1) & ~1;
   int* first = lds;                           // first place of each key
   uint16_t* count = (uint16_t*)(lds + keys);  // [wave][key]
+  __shared__ int prior[kFewKeys];             // (few chunks) counts over the chunks before
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = threadIdx.x; i < W * stride; i += 64 * W) count[i] = 0;
-  if (before)
+  if (totals) {
     for (int i = threadIdx.x; i < keys; i += 64 * W) first[i] = totals[i];
+  } else if (before) {
+    chunk_sums<W>(before, (int)gridDim.x, (int)blockIdx.x, keys, first, prior);
+  }
   __syncthreads();
 
   const int64_t base = ((int64_t)blockIdx.x * W + wave) * kSortItems;
@@ -170,7 +201,7 @@ __global__ __launch_bounds__(64 * W) void expert_place_kernel(const int64_t* ids
     const int e = key[r];
     if (e < 0) continue;
     const int64_t i = base + r * 64 + lane;
-    const int64_t at = first[e] + (before ? before[(int64_t)blockIdx.x * keys + e] : 0) + own[e] + rank[r];
+    const int64_t at = first[e] + (totals ? before[(int64_t)blockIdx.x * keys + e] : before ? prior[e] : 0) + own[e] + rank[r];
     slots[i] = at;
     order[at] = i;
   }
@@ -185,111 +216,149 @@ __device__ __forceinline__ int64_t kept_places(const int64_t* offsets, int64_t e
   return kept < 0 ? 0 : kept > n ? n : kept;
 }
 
-// Rows of `len` units each to their places, T lanes to a token.
-template <class U, int T>
-__global__ __launch_bounds__(kRowThreads) void to_experts_kernel(const U* x, int64_t tokens, int64_t k, int64_t len,
+// The row that a thread's T lanes begin with: the same for the whole wave from 64 lanes on, which the compiler is told, so that
+// what belongs to the row (places, weights) comes through scalar loads into scalar registers.
+template <int T>
+__device__ __forceinline__ int64_t first_row() {
+  const int at = (int)threadIdx.x / T;
+  return (int64_t)blockIdx.x * (kRowThreads / T) + (T >= 64 ? __builtin_amdgcn_readfirstlane(at) : at);
+}
+
+// Rows to their places, T lanes to a token, 16 bytes at once.
+template <int T>
+__global__ __launch_bounds__(kRowThreads) void to_experts_kernel(const uint8_t* x, int64_t tokens, int64_t k, int64_t bytes,
                                                                  const int64_t* slots, const int64_t* offsets,
-                                                                 int64_t experts, U* rows) {
+                                                                 int64_t experts, uint8_t* rows) {
+  typedef uint32_t loose __attribute__((ext_vector_type(4), aligned(1)));
   const int lane = threadIdx.x % T;
   const int64_t kept = kept_places(offsets, experts, tokens * k);
-  for (int64_t t = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / T; t < tokens; t += (int64_t)gridDim.x * (kRowThreads / T)) {
+  for (int64_t t = first_row<T>(); t < tokens; t += (int64_t)gridDim.x * (kRowThreads / T)) {
     const int64_t* at = slots + t * k;
-    for (int64_t c = lane; c < len; c += T) {
-      const U v = x[t * len + c];
+    for (int64_t c = (int64_t)lane * 16; c < bytes; c += T * 16) {
+      const int64_t n = bytes - c;
+      const uint8_t* from = x + t * bytes + c;
+      u32x4_t v = {0u, 0u, 0u, 0u};
+      if (n >= 16) v = *(const loose*)from;
       for (int64_t j = 0; j < k; ++j) {
         const int64_t p = at[j];
-        if ((uint64_t)p < (uint64_t)kept) rows[p * len + c] = v;
-        if (t * k + j >= kept) rows[(t * k + j) * len + c] = U{};  // each place behind them once
+        // place t k + j holds zeros if it is behind the kept ones: each such place once
+        for (int zero = 0; zero < 2; ++zero) {
+          if (zero ? t * k + j < kept : (uint64_t)p >= (uint64_t)kept) continue;
+          uint8_t* to = rows + (zero ? t * k + j : p) * bytes + c;
+          if (n >= 16) {
+            *(loose*)to = zero ? u32x4_t{0u, 0u, 0u, 0u} : v;
+          } else {
+            for (int i = 0; i < n; ++i) to[i] = zero ? 0 : from[i];
+          }
+        }
       }
     }
   }
 }
 
-// out[t] = sum_j w[t, j] rows[slot(t, j)] (w null: ones), T lanes to a token, V elements of a row at once.
-template <int DT, int V, int T>
+// out[t] = sum_j w[t, j] rows[slot(t, j)] (w null: ones), T lanes to a token.
+template <int DT, int T>
 __global__ __launch_bounds__(kRowThreads) void from_experts_kernel(const void* rowsv, const void* w, int wf32, int64_t tokens,
                                                                    int64_t k, int64_t D, const int64_t* slots,
                                                                    const int64_t* offsets, int64_t experts, void* outv) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
-  constexpr int kFlight = 8;  // rows whose loads are in flight together
+  using C = RowChunk<DT>;
+  constexpr int V = C::V, kFlight = 8;  // rows whose loads are in flight together
   const R* rows = (const R*)rowsv;
   R* out = (R*)outv;
   const int lane = threadIdx.x % T;
   const int64_t kept = kept_places(offsets, experts, tokens * k);
-  for (int64_t t = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / T; t < tokens; t += (int64_t)gridDim.x * (kRowThreads / T)) {
+  for (int64_t t = first_row<T>(); t < tokens; t += (int64_t)gridDim.x * (kRowThreads / T)) {
+    const R* from[kFlight];
+    float wj[kFlight];
+    auto places = [&](int64_t j0) {
+#pragma unroll
+      for (int q = 0; q < kFlight; ++q) {
+        const int64_t a = t * k + j0 + q, p = j0 + q < k ? slots[a] : -1;
+        const bool in = (uint64_t)p < (uint64_t)kept;
+        wj[q] = !in ? 0.f : w ? param_at<DT>(w, wf32, a) : 1.f;
+        from[q] = in ? rows + p * D : nullptr;
+      }
+    };
+    places(0);
     for (int64_t c = (int64_t)lane * V; c < D; c += T * V) {
       float acc[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = 0.f;
       for (int64_t j0 = 0; j0 < k; j0 += kFlight) {
-        VT v[kFlight];
-        float wj[kFlight];
+        if (k > kFlight) places(j0);
+        C v[kFlight];
 #pragma unroll
         for (int q = 0; q < kFlight; ++q) {
-          const int64_t a = t * k + j0 + q, p = j0 + q < k ? slots[a] : -1;
-          const bool in = (uint64_t)p < (uint64_t)kept;
-          wj[q] = !in ? 0.f : w ? param_at<DT>(w, wf32, a) : 1.f;
-          if (in) v[q] = *(const VT*)(rows + p * D + c);
-          else v[q] = VT{};
+          v[q] = C{};
+          if (from[q]) v[q].load(from[q] + c, D - c);
         }
 #pragma unroll
         for (int q = 0; q < kFlight; ++q)
 #pragma unroll
           for (int i = 0; i < V; ++i) acc[i] = fmaf(wj[q], to_f32<DT>(v[q].e[i]), acc[i]);
       }
-      VT o;
+      C o;
 #pragma unroll
       for (int i = 0; i < V; ++i) o.e[i] = from_f32<DT>(acc[i]);
-      *(VT*)(out + t * D + c) = o;
+      o.store(out + t * D + c, D - c);
     }
   }
 }
 
 // drows[slot] = w dout[t] and dw = <dout[t], rows[slot]> of an assignment, T lanes to it; either may be null.
-template <int DT, int V, int T>
+template <int DT, int T>
 __global__ __launch_bounds__(kRowThreads) void from_experts_backward_kernel(const void* gv, const void* rowsv, const void* w,
                                                                             int wf32, int64_t n, int64_t k, int64_t D,
                                                                             const int64_t* slots, const int64_t* offsets,
                                                                             int64_t experts, void* drowsv, void* dw) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
+  using C = RowChunk<DT>;
+  constexpr int V = C::V;
+  __shared__ float red[2][16];
   const R *dout = (const R*)gv, *rows = (const R*)rowsv;
   R* drows = (R*)drowsv;
   const int lane = threadIdx.x % T;
   const int64_t kept = kept_places(offsets, experts, n);
-  for (int64_t a = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) / T; a < n; a += (int64_t)gridDim.x * (kRowThreads / T)) {
+  int flip = 0;
+  // (T = 256: the workgroup makes the rounds together, for the barriers of the sum)
+  for (int64_t a = first_row<T>(); a < n; a += (int64_t)gridDim.x * (kRowThreads / T), flip ^= 1) {
     const int64_t t = a / k, p = slots[a];
     const bool in = (uint64_t)p < (uint64_t)kept;
     const float wa = !in ? 0.f : w ? param_at<DT>(w, wf32, a) : 1.f;
-    float s = 0.f;
+    float s[1] = {0.f};
     for (int64_t c = (int64_t)lane * V; c < D; c += T * V) {
       if (in) {
-        const VT g = *(const VT*)(dout + t * D + c);
+        C g, v;
+        g.load(dout + t * D + c, D - c);
         if (dw) {
-          const VT v = *(const VT*)(rows + p * D + c);
+          v.load(rows + p * D + c, D - c);
 #pragma unroll
-          for (int i = 0; i < V; ++i) s = fmaf(to_f32<DT>(g.e[i]), to_f32<DT>(v.e[i]), s);
+          for (int i = 0; i < V; ++i) s[0] = fmaf(to_f32<DT>(g.e[i]), to_f32<DT>(v.e[i]), s[0]);
         }
         if (drows) {
-          VT o;
+          C o;
 #pragma unroll
           for (int i = 0; i < V; ++i) o.e[i] = from_f32<DT>(wa * to_f32<DT>(g.e[i]));
-          *(VT*)(drows + p * D + c) = o;
+          o.store(drows + p * D + c, D - c);
         }
       }
-      if (drows && a >= kept) *(VT*)(drows + a * D + c) = VT{};  // each place behind them once
+      if (drows && a >= kept) C{}.store(drows + a * D + c, D - c);  // each place behind them once
     }
     if (dw) {
-      s = lane_sum<T>(s);
-      if (lane == 0) param_set<DT>(dw, wf32, a, s);
+      row_sum<T>(s, red[flip]);
+      if (lane == 0) param_set<DT>(dw, wf32, a, s[0]);
     }
   }
 }
 
+// Lanes to a row of so many 16-byte chunks: 16 where they reach over it, 256 where rows are few and long (8,192 tokens of 128
+// chunks, 20,011 of 65, there / back, us: 64 lanes 28 / 45, 13 / 15, 128 lanes 28 / 46, 16 / 20).
 template <class F>
-int by_lanes(int64_t chunks, F&& f) {  // lanes to a row of so many chunks
-  return chunks <= 16 ? f(std::integral_constant<int, 16>()) : f(std::integral_constant<int, 64>());
+int by_lanes(int64_t chunks, int64_t rows, F&& f) {
+  if (chunks <= 16) return f(std::integral_constant<int, 16>());
+  if (chunks > 64 && rows <= 2048) return f(std::integral_constant<int, 256>());
+  return f(std::integral_constant<int, 64>());
 }
 dim3 row_grid(int64_t rows, int T) { return dim3((unsigned)std::min<int64_t>(ceil_div(rows * T, kRowThreads), 1 << 20)); }
 
@@ -325,32 +394,13 @@ int rows_check(const char* who, int dtype, int wdtype, int64_t tokens, int64_t k
   return ML_OK;
 }
 
-template <class U>
-int to_experts_launch(const void* x, int64_t tokens, int64_t k, int64_t row_bytes, const int64_t* slots, const int64_t* offsets,
-                      int64_t experts, void* rows, hipStream_t st) {
-  const int64_t len = row_bytes / (int64_t)sizeof(U);
-  return by_lanes(len, [&](auto tc) {
-    constexpr int T = decltype(tc)::value;
-    hipLaunchKernelGGL((to_experts_kernel<U, T>), row_grid(tokens, T), dim3(kRowThreads), 0, st, (const U*)x, tokens, k, len,
-                       slots, offsets, experts, (U*)rows);
-    return check_launch("to_experts");
-  });
-}
-
 template <int DT>
 int from_experts(const void* rows, const void* w, int wf32, int64_t tokens, int64_t k, int64_t D, const int64_t* slots,
                  const int64_t* offsets, int64_t experts, void* out, hipStream_t st) {
-  constexpr int V16 = DT == ML_F32 ? 4 : 8;
-  const bool vec = D % V16 == 0 && aligned16(rows) && aligned16(out);
-  return by_lanes(vec ? D / V16 : D, [&](auto tc) {
+  return by_lanes(ceil_div(D, RowChunk<DT>::V), tokens, [&](auto tc) {
     constexpr int T = decltype(tc)::value;
-    const dim3 grid = row_grid(tokens, T), blk(kRowThreads);
-    if (vec)
-      hipLaunchKernelGGL((from_experts_kernel<DT, V16, T>), grid, blk, 0, st, rows, w, wf32, tokens, k, D, slots, offsets,
-                         experts, out);
-    else
-      hipLaunchKernelGGL((from_experts_kernel<DT, 1, T>), grid, blk, 0, st, rows, w, wf32, tokens, k, D, slots, offsets,
-                         experts, out);
+    hipLaunchKernelGGL((from_experts_kernel<DT, T>), row_grid(tokens, T), dim3(kRowThreads), 0, st, rows, w, wf32, tokens, k, D,
+                       slots, offsets, experts, out);
     return check_launch("from_experts");
   });
 }
@@ -359,17 +409,10 @@ template <int DT>
 int from_experts_backward(const void* g, const void* rows, const void* w, int wf32, int64_t n, int64_t k, int64_t D,
                           const int64_t* slots, const int64_t* offsets, int64_t experts, void* drows, void* dw,
                           hipStream_t st) {
-  constexpr int V16 = DT == ML_F32 ? 4 : 8;
-  const bool vec = D % V16 == 0 && aligned16(g) && aligned16(rows) && aligned16(drows);
-  return by_lanes(vec ? D / V16 : D, [&](auto tc) {
+  return by_lanes(ceil_div(D, RowChunk<DT>::V), n, [&](auto tc) {
     constexpr int T = decltype(tc)::value;
-    const dim3 grid = row_grid(n, T), blk(kRowThreads);
-    if (vec)
-      hipLaunchKernelGGL((from_experts_backward_kernel<DT, V16, T>), grid, blk, 0, st, g, rows, w, wf32, n, k, D, slots,
-                         offsets, experts, drows, dw);
-    else
-      hipLaunchKernelGGL((from_experts_backward_kernel<DT, 1, T>), grid, blk, 0, st, g, rows, w, wf32, n, k, D, slots,
-                         offsets, experts, drows, dw);
+    hipLaunchKernelGGL((from_experts_backward_kernel<DT, T>), row_grid(n, T), dim3(kRowThreads), 0, st, g, rows, w, wf32, n, k,
+                       D, slots, offsets, experts, drows, dw);
     return check_launch("from_experts_backward");
   });
 }
@@ -408,10 +451,12 @@ extern "C" int ml_sort_by_expert(const int64_t* ids, int64_t tokens, int64_t k, 
   int* counts = totals + keys;
   hipLaunchKernelGGL(expert_count_kernel, dim3((unsigned)chunks), dim3(64 * kManyWaves), (size_t)keys * sizeof(int), st, ids, n,
                      (int)experts, counts);
-  hipLaunchKernelGGL(expert_sum_kernel, dim3((unsigned)ceil_div(keys, 64)), dim3(64 * kSumWaves), 0, st, counts, (int)chunks,
-                     keys, totals);
+  const bool few = chunks <= kFewChunks && keys <= kFewKeys;
+  if (!few)
+    hipLaunchKernelGGL(expert_sum_kernel, dim3((unsigned)ceil_div(keys, 64)), dim3(64 * kSumWaves), 0, st, counts, (int)chunks,
+                       keys, totals);
   hipLaunchKernelGGL(expert_place_kernel<kManyWaves>, dim3((unsigned)chunks), dim3(64 * kManyWaves),
-                     place_lds<kManyWaves>(experts), st, ids, n, (int)experts, counts, totals, order, slots, offsets);
+                     place_lds<kManyWaves>(experts), st, ids, n, (int)experts, counts, few ? nullptr : totals, order, slots, offsets);
   return check_launch("sort_by_expert");
 }
 
@@ -426,11 +471,12 @@ extern "C" int ml_to_experts(const void* x, int64_t tokens, int64_t k, int64_t r
   if (!x || !slots || !offsets || !rows) return fail(ML_EINVAL, "to_experts: null pointer");
   hipStream_t st = (hipStream_t)stream;
   ProfScope ps("to_experts", st);
-  const uint64_t bits = (uint64_t)row_bytes | (uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)rows;
-  if (bits % 16 == 0) return to_experts_launch<u32x4_t>(x, tokens, k, row_bytes, slots, offsets, experts, rows, st);
-  if (bits % 4 == 0) return to_experts_launch<uint32_t>(x, tokens, k, row_bytes, slots, offsets, experts, rows, st);
-  if (bits % 2 == 0) return to_experts_launch<uint16_t>(x, tokens, k, row_bytes, slots, offsets, experts, rows, st);
-  return to_experts_launch<uint8_t>(x, tokens, k, row_bytes, slots, offsets, experts, rows, st);
+  return by_lanes(ceil_div(row_bytes, 16), tokens, [&](auto tc) {
+    constexpr int T = decltype(tc)::value;
+    hipLaunchKernelGGL(to_experts_kernel<T>, row_grid(tokens, T), dim3(kRowThreads), 0, st, (const uint8_t*)x, tokens, k,
+                       row_bytes, slots, offsets, experts, (uint8_t*)rows);
+    return check_launch("to_experts");
+  });
 }
 
 extern "C" int ml_from_experts_forward(int dtype, int weight_dtype, const void* rows, const void* weights, int64_t tokens,

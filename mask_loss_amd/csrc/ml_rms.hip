@@ -16,14 +16,15 @@
 namespace ml {
 namespace {
 
-// T threads hold a row, NV vectors of V elements each; vector k of thread t starts at column (k T + t) V.
+// T threads hold a row, NV vectors of 16 bytes (V elements) each; vector k of thread t starts at column (k T + t) V.
+// Rows are whole vectors, or V is 1.
 // RES: with a residual; MX: y as codes and scales.
 template <int DT, int V, int NV, int T, bool RES, bool MX>
 __global__ __launch_bounds__(wg_threads(T)) void rms_fwd_kernel(const void* xv, const void* rv, const void* w, int pf32,
                                                                 int64_t rows, int64_t D, float eps, int format, void* sv,
                                                                 void* yv, uint8_t* scales, float* rstd) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
+  using VT = RowChunk<DT, V>;
   constexpr int G = wg_threads(T) / T;  // rows at once
   __shared__ float red[2][16];
   const R *x = (const R*)xv, *res = (const R*)rv;
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_fwd_kernel(const void* xv, 
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int64_t c = (int64_t)(k * T + t) * V;
-    ok[k] = c < D;  // a vector lies inside the row as a whole
+    ok[k] = c < D;
 #pragma unroll
     for (int j = 0; j < V; ++j) wr[k * V + j] = ok[k] && w ? param_at<DT>(w, pf32, c + j) : 1.f;
   }
@@ -45,14 +46,10 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_fwd_kernel(const void* xv, 
   auto load = [&](VT(&v)[NV], VT(&u)[RES ? NV : 1], int64_t r) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const bool in = ok[k] && r < rows;
+      const int n = ok[k] && r < rows ? V : 0;
       const int64_t at = r * D + (int64_t)(k * T + t) * V;
-      if (in) v[k] = *(const VT*)(x + at);
-      else v[k] = VT{};
-      if constexpr (RES) {
-        if (in) u[k] = *(const VT*)(res + at);
-        else u[k] = VT{};
-      }
+      v[k].template load<true>(x + at, n);
+      if constexpr (RES) u[k].template load<true>(res + at, n);
     }
   };
   load(cur, cr, row);
@@ -80,7 +77,7 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_fwd_kernel(const void* xv, 
     for (int k = 0; k < NV; ++k) {
       const int64_t at = row * D + (int64_t)(k * T + t) * V;
       if constexpr (RES) {
-        if (ok[k] && in) *(VT*)((R*)sv + at) = cur[k];
+        if (in && ok[k]) cur[k].template store<true>((R*)sv + at, V);
       }
       if constexpr (MX) {
         float y[V];
@@ -91,11 +88,11 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_fwd_kernel(const void* xv, 
           mx_store(y, code, format, at, (uint8_t*)yv);
           if (at % kMxBlock == 0) scales[at / kMxBlock] = (uint8_t)code;
         }
-      } else if (ok[k] && in) {
+      } else if (in && ok[k]) {
         VT o;
 #pragma unroll
         for (int j = 0; j < V; ++j) o.e[j] = from_f32<DT>(f[k * V + j] * r * wr[k * V + j]);
-        *(VT*)((R*)yv + at) = o;
+        o.template store<true>((R*)yv + at, V);
       }
     }
     if (in && t == 0 && rstd) rstd[row] = r;
@@ -114,7 +111,7 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_bwd_kernel(const void* gv, 
                                                                 const void* w, int pf32, const float* rstd, int64_t rows,
                                                                 int64_t D, void* dxv, float* part) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
+  using VT = RowChunk<DT, V>;
   constexpr int G = wg_threads(T) / T, E = NV * V;
   __shared__ float red[2][16];
   const R *x = (const R*)xv, *dy = (const R*)gv, *du = (const R*)uv;
@@ -144,14 +141,10 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_bwd_kernel(const void* gv, 
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int64_t o = i * D + (int64_t)(k * T + t) * V;
-      if (ok[k] && in) {
-        vx[k] = *(const VT*)(x + o);
-        vg[k] = *(const VT*)(dy + o);
-        if constexpr (SUM) vu[k] = *(const VT*)(du + o);
-      } else {
-        vx[k] = vg[k] = VT{};
-        if constexpr (SUM) vu[k] = VT{};
-      }
+      const int n = ok[k] && in ? V : 0;
+      vx[k].template load<true>(x + o, n);
+      vg[k].template load<true>(dy + o, n);
+      if constexpr (SUM) vu[k].template load<true>(du + o, n);
     }
   };
   load(cx, cg, cu, cr, row);
@@ -183,7 +176,7 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_bwd_kernel(const void* gv, 
             if constexpr (SUM) v += to_f32<DT>(cu[k].e[j]);
             o.e[j] = from_f32<DT>(v);
           }
-          *(VT*)(dx + row * D + (int64_t)(k * T + t) * V) = o;
+          o.template store<true>(dx + row * D + (int64_t)(k * T + t) * V, V);
         }
       }
     }
@@ -220,12 +213,13 @@ __global__ __launch_bounds__(wg_threads(T)) void rms_bwd_kernel(const void* gv, 
 }
 
 // ---- rows of any width: a workgroup per row, read twice ---------------------------
-template <int DT, int V, bool RES, bool MX>
+template <int DT, bool RES, bool MX>
 __global__ __launch_bounds__(kWideThreads) void rms_fwd_wide_kernel(const void* xv, const void* rv, const void* w, int pf32,
                                                                     int64_t rows, int64_t D, float eps, int format,
                                                                     void* sv, void* yv, uint8_t* scales, float* rstd) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
+  using VT = RowChunk<DT>;
+  constexpr int V = VT::V;
   __shared__ float red[2][16];
   const float inv = 1.f / (float)D;
   int flip = 0;
@@ -235,12 +229,14 @@ __global__ __launch_bounds__(kWideThreads) void rms_fwd_wide_kernel(const void* 
     R* sum = (R*)sv + (RES ? row * D : 0);
     float s[1] = {0.f};
     for (int64_t c = (int64_t)threadIdx.x * V; c < D; c += kWideThreads * V) {
-      VT v = *(const VT*)(x + c);
+      VT v;
+      v.load(x + c, D - c);
       if constexpr (RES) {
-        const VT u = *(const VT*)(res + c);
+        VT u;
+        u.load(res + c, D - c);
 #pragma unroll
         for (int j = 0; j < V; ++j) v.e[j] = from_f32<DT>(to_f32<DT>(v.e[j]) + to_f32<DT>(u.e[j]));
-        *(VT*)(sum + c) = v;  // (read again by this thread alone)
+        v.store(sum + c, D - c);  // (read again by this thread alone)
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] = fmaf(to_f32<DT>(v.e[j]), to_f32<DT>(v.e[j]), s[0]);
@@ -249,10 +245,11 @@ __global__ __launch_bounds__(kWideThreads) void rms_fwd_wide_kernel(const void* 
     const float r = 1.f / sqrtf(fmaf(s[0], inv, eps));
     const R* from = RES ? sum : x;
     for (int64_t c = (int64_t)threadIdx.x * V; c < D; c += kWideThreads * V) {
-      const VT v = *(const VT*)(from + c);
+      VT v;
+      v.load(from + c, D - c);
       float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y[j] = to_f32<DT>(v.e[j]) * r * (w ? param_at<DT>(w, pf32, c + j) : 1.f);
+      for (int j = 0; j < V; ++j) y[j] = to_f32<DT>(v.e[j]) * r * (w && c + j < D ? param_at<DT>(w, pf32, c + j) : 1.f);
       const int64_t at = row * D + c;
       if constexpr (MX) {
         // (a block's lanes leave the loop together: D is whole blocks)
@@ -263,19 +260,20 @@ __global__ __launch_bounds__(kWideThreads) void rms_fwd_wide_kernel(const void* 
         VT o;
 #pragma unroll
         for (int j = 0; j < V; ++j) o.e[j] = from_f32<DT>(y[j]);
-        *(VT*)((R*)yv + at) = o;
+        o.store((R*)yv + at, D - c);
       }
     }
     if (threadIdx.x == 0 && rstd) rstd[row] = r;
   }
 }
 
-template <int DT, int V, bool SUM>
+template <int DT, bool SUM>
 __global__ __launch_bounds__(kWideThreads) void rms_bwd_wide_kernel(const void* gv, const void* uv, const void* xv,
                                                                     const void* w, int pf32, const float* rstd,
                                                                     int64_t rows, int64_t D, void* dxv) {
   using R = typename Elem<DT>::raw;
-  using VT = Vec<DT, V>;
+  using VT = RowChunk<DT>;
+  constexpr int V = VT::V;
   __shared__ float red[2][16];
   const float inv = 1.f / (float)D;
   int flip = 0;
@@ -286,27 +284,30 @@ __global__ __launch_bounds__(kWideThreads) void rms_bwd_wide_kernel(const void* 
     const float r = rstd[row];
     float s[1] = {0.f};
     for (int64_t c = (int64_t)threadIdx.x * V; c < D; c += kWideThreads * V) {
-      const VT vx = *(const VT*)(x + c), vg = *(const VT*)(dy + c);
+      VT vx, vg;
+      vx.load(x + c, D - c);
+      vg.load(dy + c, D - c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float g = to_f32<DT>(vg.e[j]) * (w ? param_at<DT>(w, pf32, c + j) : 1.f);
+        const float g = to_f32<DT>(vg.e[j]) * (w && c + j < D ? param_at<DT>(w, pf32, c + j) : 1.f);
         s[0] = fmaf(g, to_f32<DT>(vx.e[j]) * r, s[0]);
       }
     }
     row_sum<kWideThreads>(s, red[flip]);
     const float k = s[0] * inv;
     for (int64_t c = (int64_t)threadIdx.x * V; c < D; c += kWideThreads * V) {
-      const VT vx = *(const VT*)(x + c), vg = *(const VT*)(dy + c);
-      VT vu{}, o;
-      if constexpr (SUM) vu = *(const VT*)(du + c);
+      VT vx, vg, vu, o;
+      vx.load(x + c, D - c);
+      vg.load(dy + c, D - c);
+      if constexpr (SUM) vu.load(du + c, D - c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float g = to_f32<DT>(vg.e[j]) * (w ? param_at<DT>(w, pf32, c + j) : 1.f);
+        const float g = to_f32<DT>(vg.e[j]) * (w && c + j < D ? param_at<DT>(w, pf32, c + j) : 1.f);
         float v = r * (g - to_f32<DT>(vx.e[j]) * r * k);
         if constexpr (SUM) v += to_f32<DT>(vu.e[j]);
         o.e[j] = from_f32<DT>(v);
       }
-      *(VT*)(dx + c) = o;
+      o.store(dx + c, D - c);
     }
   }
 }
@@ -346,7 +347,7 @@ struct RmsForward {
 template <int DT, int V, bool RES, bool MX>
 int rms_forward_launch(const RmsForward& a, hipStream_t st) {
   if (a.D > kNormHeld) {
-    hipLaunchKernelGGL((rms_fwd_wide_kernel<DT, V, RES, MX>), dim3((unsigned)std::min<int64_t>(a.rows, 65536)),
+    hipLaunchKernelGGL((rms_fwd_wide_kernel<DT, RES, MX>), dim3((unsigned)std::min<int64_t>(a.rows, 65536)),
                        dim3(kWideThreads), 0, st, a.x, a.res, a.w, a.pf32, a.rows, a.D, a.eps, a.format, a.sum, a.y, a.scales,
                        a.rstd);
     return check_launch("rms_norm");
@@ -364,15 +365,11 @@ int rms_forward_launch(const RmsForward& a, hipStream_t st) {
 template <int DT, bool MX>
 int rms_forward(const RmsForward& a, hipStream_t st) {
   ProfScope ps("rms_norm", st);
-  constexpr int V16 = DT == ML_F32 ? 4 : 8;
-  if constexpr (MX) {  // (rows of whole blocks on 16-byte boundaries: checked)
-    return a.res ? rms_forward_launch<DT, V16, true, true>(a, st) : rms_forward_launch<DT, V16, false, true>(a, st);
-  } else {
-    // 16-byte vectors where every row starts on a 16-byte boundary
-    const bool vec = a.D % V16 == 0 && aligned16(a.x) && aligned16(a.res) && aligned16(a.sum) && aligned16(a.y);
-    if (vec) return a.res ? rms_forward_launch<DT, V16, true, false>(a, st) : rms_forward_launch<DT, V16, false, false>(a, st);
-    return a.res ? rms_forward_launch<DT, 1, true, false>(a, st) : rms_forward_launch<DT, 1, false, false>(a, st);
-  }
+  constexpr int V16 = RowChunk<DT>::V;
+  if (a.D % V16 == 0)
+    return a.res ? rms_forward_launch<DT, V16, true, MX>(a, st) : rms_forward_launch<DT, V16, false, MX>(a, st);
+  if constexpr (!MX) return a.res ? rms_forward_launch<DT, 1, true, MX>(a, st) : rms_forward_launch<DT, 1, false, MX>(a, st);
+  return ML_OK;  // (MX: rows are whole blocks)
 }
 
 struct RmsBackward {
@@ -390,7 +387,7 @@ int rms_backward_launch(const RmsBackward& a, hipStream_t st) {
   if (a.D > kNormHeld) {
     int rc = ML_OK;
     if (a.dx) {
-      hipLaunchKernelGGL((rms_bwd_wide_kernel<DT, V, SUM>), dim3((unsigned)std::min<int64_t>(a.rows, 65536)),
+      hipLaunchKernelGGL((rms_bwd_wide_kernel<DT, SUM>), dim3((unsigned)std::min<int64_t>(a.rows, 65536)),
                          dim3(kWideThreads), 0, st, a.dy, a.du, a.x, a.w, a.pf32, a.rstd, a.rows, a.D, a.dx);
       rc = check_launch("rms_norm_backward");
     }
@@ -410,11 +407,10 @@ int rms_backward_launch(const RmsBackward& a, hipStream_t st) {
 template <int DT>
 int rms_backward(const RmsBackward& a, hipStream_t st) {
   ProfScope ps("rms_norm_backward", st);
-  constexpr int V16 = DT == ML_F32 ? 4 : 8;
-  const bool vec = a.D % V16 == 0 && aligned16(a.x) && aligned16(a.dy) && aligned16(a.du) && aligned16(a.dx);
   int rc = ML_OK;
   if (a.rows > 0) {
-    if (vec) rc = a.du ? rms_backward_launch<DT, V16, true>(a, st) : rms_backward_launch<DT, V16, false>(a, st);
+  constexpr int V16 = RowChunk<DT>::V;
+    if (a.D % V16 == 0) rc = a.du ? rms_backward_launch<DT, V16, true>(a, st) : rms_backward_launch<DT, V16, false>(a, st);
     else rc = a.du ? rms_backward_launch<DT, 1, true>(a, st) : rms_backward_launch<DT, 1, false>(a, st);
   }
   if (rc || !a.dw) return rc;

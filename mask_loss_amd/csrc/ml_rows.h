@@ -47,6 +47,43 @@ struct alignas(V == 1 ? sizeof(typename Elem<DT>::raw) : 16) Vec {
   typename Elem<DT>::raw e[V];
 };
 
+// 16 bytes of a row from element c on, at the element's alignment (one load or store of 16 bytes still: rows of odd
+// length start anywhere); a row's last elements one by one.
+typedef u32x4_t u32x4_near_t __attribute__((aligned(2)));
+template <int DT, int N = DT == ML_F32 ? 4 : 8>  // (or single elements: N = 1)
+struct RowChunk {
+  static constexpr int V = N;
+  typename Elem<DT>::raw e[V];
+
+  // zeros where n, the elements left, runs out; WHOLE: all or none of the chunk is left
+  template <bool WHOLE = false>
+  __device__ __forceinline__ void load(const typename Elem<DT>::raw* p, int64_t n) {
+    if constexpr (V == 1) {
+      e[0] = n > 0 ? *p : typename Elem<DT>::raw(0);
+    } else if (n >= V) {
+      const u32x4_t v = *(const u32x4_near_t*)p;
+      __builtin_memcpy(e, &v, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = !WHOLE && j < n ? p[j] : typename Elem<DT>::raw(0);
+    }
+  }
+  template <bool WHOLE = false>
+  __device__ __forceinline__ void store(typename Elem<DT>::raw* p, int64_t n) const {
+    if constexpr (V == 1) {
+      if (n > 0) *p = e[0];
+    } else if (n >= V) {
+      u32x4_t v;
+      __builtin_memcpy(&v, e, 16);
+      *(u32x4_near_t*)p = v;
+    } else if constexpr (!WHOLE) {
+#pragma unroll
+      for (int j = 0; j < V - 1; ++j)
+        if (j < n) p[j] = e[j];
+    }
+  }
+};
+
 // v plus the value of another lane, in the vector ALU: quad neighbours (xor 1, xor 2), the mirrored
 // lane of 8 and of 16 (whose fours and eights hold one value by then), the other 16 and the
 // other 32.  About 10 cycles a step where a shuffle through LDS takes 60.
