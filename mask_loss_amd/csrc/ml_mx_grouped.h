@@ -275,42 +275,6 @@ __global__ __launch_bounds__(64 * WM * WN) void mx_kernel(MxArgs x) {
   }
 }
 
-// ---- scales in whole fours: stages filled by direct loads into LDS ---------------------
-// Where K is a multiple of 128 (and the scales start on 4-byte boundaries), a row's four scales of a fragment are one
-// dword, and everything of a stage comes by direct loads: grouped_ring_kernel's ring (there: stages, persistent workgroups, turns,
-// waits), with the dwords of the stage's scales behind its codes, [128 of the reduced index][rows of both operands].
-
-// Four bytes from base + off, or from p, of each lane to LDS at `lds` + 4 lane; base as ring_loads'.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void ring_dwords(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
-               :
-               : "s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
-}
-__device__ __forceinline__ void ring_dwords(const char* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-               :
-               : "s"(lds), "v"(p)
-               : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
-// One operand of a stage, filled by NW waves.
-template <int F, int R, int NW, int BK>
-struct MxRing : RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)> {
-  using O = typename RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)>::O;
-  // 128 values from 128 s on, of rows row0 .. (the scale is elsewhere)
-  static __device__ __forceinline__ MxFrag<F> frag(const unsigned char* lds, int row0, int s) {
-    MxFrag<F> f;
-    f.v[0] = O::frag(lds, row0, F == ML_MX_E4M3 ? 0 : s);
-    if constexpr (F == ML_MX_E4M3) f.v[1] = O::frag(lds, row0, 1);
-    f.scale = 0;
-    return f;
-  }
-};
-
 // The scales of 64 rows: from lane l's dword of row l (its blocks 0 .. 3) to lane l's four bytes of block l / 16 in rows
 // l % 16 + 16 j, of which the instruction is told byte j.  A transpose among the lanes l % 16 + 16 g: neighbours g, g ^ 1
 // exchange their dwords, each keeps the bytes of blocks g and g ^ 2 of the two, and hands the latter to g ^ 2.
@@ -346,6 +310,179 @@ __device__ __forceinline__ f32x4_t mx_mma_at(int ba, int bb, const MxFrag<FA>& a
     default: return mx_mma_at<FA, FB, 3, 3>(a, b, sa, sb, c);
   }
 }
+
+// ---- few rows to a group ------------------------------------------------------------
+// The matrices are read once and nothing is reused but a few rows, so the operands go from memory into the registers
+// that the matrix instruction takes: a workgroup has 16 MT rows by 32 columns, its four waves take turns over the reduced
+// index, 512 of it at a time (so all of a lane's loads are in flight together), and add up through LDS.
+constexpr int kFewColumns = 32, kFewStep = 512;
+
+// 512 values of a row from `codes` and `scales` on, for the lanes l of the row l % 16; left: values of the row from there on.
+template <int F>
+struct MxRows {
+  static constexpr int N = F == ML_MX_E4M3 ? 2 : 1;  // 16-byte chunks of 128 values that a lane has
+  u32x4_t v[4][N];
+  uint32_t scale;
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales, int left) {
+    const int g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        // e4m3: values 16 g .. of the first 64 and of the last; e2m1: 32 g ..
+        const int at = 128 * s + (F == ML_MX_E4M3 ? 64 * i + 16 * g : 32 * g);
+        v[s][i] = u32x4_t{0u, 0u, 0u, 0u};
+        if (at < left) v[s][i] = *(const u32x4_t*)(codes + mx_bytes(F, at));
+      }
+    // lane group g: the four scales of 128 values from 128 g on
+    scale = 0x7F7F7F7Fu;  // 1, for the zeros past the end
+    const int n = left / kMxBlock - 4 * g;
+    if (n >= 4) {
+      scale = *(const u32_byte_t*)(scales + 4 * g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < n) scale = (scale & ~(0xFFu << (8 * j))) | (uint32_t)scales[4 * g + j] << (8 * j);
+    }
+  }
+  __device__ __forceinline__ MxFrag<F> frag(int s) const {
+    MxFrag<F> f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.v[i] = v[s][i];
+    f.scale = 0;
+    return f;
+  }
+};
+
+template <int FA, int FB, int OUT, int MT>
+__global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
+  constexpr int BM = 16 * MT, NT = kFewColumns / 16;
+  __shared__ f32x4_t part[3][MT * NT][64];
+  extern __shared__ int e[];
+  const GroupedArgs& a = x.g;
+  group_edges(a, e);
+  int* t = e + a.groups + 1;
+  const int tiles = segment_tiles(a, e, t, BM), id = xcd_item(tiles * a.cols.d);
+  if (id < 0) return;
+  const Work it = rows_work(a, e, t, tiles, id, 0, 1, BM, kFewColumns, kFewStep);
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int m0 = uniform(it.m0), n0 = uniform(it.n0), mlim = uniform(it.mlim), w = uniform(it.w), K = uniform(it.kend);
+  const int nlim = a.N - n0;
+  const bool mapped = uniform(it.mapped) != 0;
+
+  const uint8_t *pa[MT], *sa[MT], *pb[NT], *sb[NT];
+  int64_t row[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {  // rows past the last read the last one (their outputs are not stored)
+    const int r = min(16 * i + (lane & 15), mlim - 1);
+    row[i] = mapped ? merged_row(a, e, w, m0 + r) : m0 + r;
+    pa[i] = (const uint8_t*)a.a + row[i] * (a.lda * 2);
+    sa[i] = x.sa + row[i] * x.sld;
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int64_t r = (int64_t)w * a.N + n0 + min(16 * i + (lane & 15), nlim - 1);
+    pb[i] = (const uint8_t*)a.b + r * (a.ldb * 2);
+    sb[i] = x.sb + r * x.sld;
+  }
+  f32x4_t acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const MxTurn turn;
+  for (int k = wave * kFewStep; k < K; k += 4 * kFewStep) {
+    MxRows<FA> ra[MT];
+    MxRows<FB> rb[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) rb[i].load(pb[i] + mx_bytes(FB, k), sb[i] + k / kMxBlock, K - k);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) ra[j].load(pa[j] + mx_bytes(FA, k), sa[j] + k / kMxBlock, K - k);
+    uint32_t ta[MT], tb[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) tb[i] = turn(rb[i].scale);  // byte s: of the 128 values from 128 s on
+#pragma unroll
+    for (int j = 0; j < MT; ++j) ta[j] = turn(ra[j].scale);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mx_mma_at(s, s, rb[i].frag(s), ra[j].frag(s), tb[i], ta[j], acc[i][j]);
+  }
+  if (wave)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) part[wave - 1][i * MT + j][lane] = acc[i][j];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    if (16 * j + (lane & 15) >= mlim) continue;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      f32x4_t v = acc[i][j];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) v += part[q][i * MT + j][lane];
+      const int n = 16 * i + 4 * (lane >> 4), room = nlim - n;
+      if (room <= 0) continue;
+      const int64_t at = row[j] * a.ldc + n0 + n;
+      if constexpr (OUT == ML_F32) {
+        float* c = (float*)a.c + at;
+        if (room >= 4) *(f32x4_loose*)c = v;
+        else
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            if (q < room) c[q] = v[q];
+      } else {
+        const u32x2_t p = {GMma<OUT>::pack(v[0], v[1]), GMma<OUT>::pack(v[2], v[3])};
+        uint16_t* c = (uint16_t*)a.c + at;
+        if (room >= 4) *(u32x2_loose*)c = p;
+        else
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            if (q < room) c[q] = (uint16_t)(p[q / 2] >> (16 * (q & 1)));
+      }
+    }
+  }
+}
+
+// ---- scales in whole fours: stages filled by direct loads into LDS ---------------------
+// Where K is a multiple of 128 (and the scales start on 4-byte boundaries), a row's four scales of a fragment are one
+// dword, and everything of a stage comes by direct loads: grouped_ring_kernel's ring (there: stages, persistent workgroups, turns,
+// waits), with the dwords of the stage's scales behind its codes, [128 of the reduced index][rows of both operands].
+
+// Four bytes from base + off, or from p, of each lane to LDS at `lds` + 4 lane; base as ring_loads'.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void ring_dwords(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void ring_dwords(const char* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds), "v"(p)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// One operand of a stage, filled by NW waves.
+template <int F, int R, int NW, int BK>
+struct MxRing : RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)> {
+  using O = typename RingOperand<ML_BF16, true, R, NW, mx_bytes(F, BK)>::O;
+  // 128 values from 128 s on, of rows row0 .. (the scale is elsewhere)
+  static __device__ __forceinline__ MxFrag<F> frag(const unsigned char* lds, int row0, int s) {
+    MxFrag<F> f;
+    f.v[0] = O::frag(lds, row0, F == ML_MX_E4M3 ? 0 : s);
+    if constexpr (F == ML_MX_E4M3) f.v[1] = O::frag(lds, row0, 1);
+    f.scale = 0;
+    return f;
+  }
+};
 
 // Order of a sub-step's LDS reads (the scales' first, RB and RA for a fragment of either operand) and products (N for each
 // of M fragments).

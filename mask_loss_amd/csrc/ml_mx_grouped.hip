@@ -25,7 +25,7 @@ constexpr size_t kRingParts = (size_t)kRingSlots * kManyRows * kColumns * sizeof
 struct MxPlan {
   bool few, merged;
   int ring;  // 0, or the bytes of a scale load: 4, 16
-  int bm, splits;
+  int bm, bn, splits;
   int64_t bound, plane;
   size_t bytes;
 };
@@ -49,10 +49,12 @@ int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, int aligned, boo
   const int64_t segments = p.merged ? s->matrices : groups;
   const int64_t used = std::min(segments, std::max<int64_t>(s->rows, 1));  // those that can hold rows
   const double each = (double)s->rows / used;
+  const bool exact = mx_exact(fa, fb, out);
   p.few = each <= 32.0;
-  p.bm = p.few ? few_rows(fa, fb) : kManyRows;
-  p.ring = p.few || mx_exact(fa, fb, out) ? 0 : s->K % 512 == 0 && aligned >= 16 ? 16 : s->K % 128 == 0 && aligned >= 4 ? 4 : 0;
-  const int64_t columns = ceil_div(s->N, kColumns);
+  p.bm = !p.few ? kManyRows : exact ? few_rows(fa, fb) : each <= 16.0 ? 16 : 32;
+  p.bn = p.few && !exact ? kFewColumns : kColumns;
+  p.ring = p.few || exact ? 0 : s->K % 512 == 0 && aligned >= 16 ? 16 : s->K % 128 == 0 && aligned >= 4 ? 4 : 0;
+  const int64_t columns = ceil_div(s->N, p.bn);
   // values of a part of a reduction, at least one turn of the kernel's loop
   const int64_t step = p.ring == 16 ? 512 : mx_step(fa, fb), steps = std::max<int64_t>(1, ceil_div(s->K, step));
   const double x = each / p.bm, rows = used * (equal || segments == 1 ? std::ceil(x) : std::max(1.05, x + 0.5));
@@ -65,6 +67,8 @@ int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, int aligned, boo
     const double whole = 2.0 * s->K / 512, move = 0.026 * all;
     const int64_t parts = std::min({fit, (int64_t)std::lround(std::sqrt(whole / move)), steps, (int64_t)64});
     p.splits = parts > 1 && s->N % 4 == 0 && whole / parts + 4.0 + move * parts < whole ? (int)parts : 1;  // (joined by whole fours)
+  } else if (p.few && !exact) {
+    p.splits = 1;  // (the waves of a workgroup have parts already)
   } else {
     p.splits = (int)std::max<int64_t>(1, std::min({fit, steps / 4, (int64_t)64}));
   }
@@ -105,6 +109,13 @@ int mx_launch(const ml_grouped_shape* s, const MxPlan& p, MxArgs& x, hipStream_t
     }
   }
   const dim3 grid((unsigned)(ceil_div(p.bound, kXcds) * kXcds));
+  if constexpr (!mx_exact(FA, FB, OUT)) {
+    if (p.few) {
+      if (p.bm == 16) hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 1>), grid, blk, lds, st, x);
+      else hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 2>), grid, blk, lds, st, x);
+      return check_launch("grouped_matmul_mx");
+    }
+  }
   if (p.few)
     hipLaunchKernelGGL((mx_kernel<FA, FB, OUT, few_rows(FA, FB), kColumns, 1, 4>), grid, blk, lds, st, x);
   else
@@ -180,7 +191,7 @@ extern "C" int ml_grouped_matmul_mx(const ml_grouped_shape* s, int x_format, con
   a.plane = p.plane;
   a.c = y;
   a.parts = (float*)workspace;
-  a.cols = fast_div(ceil_div(s->N, kColumns));
+  a.cols = fast_div(ceil_div(s->N, p.bn));
   a.layers = fast_div(a.groups / a.matrices);
   a.mtiles = fast_div(1);
   m.sa = x_scales;
