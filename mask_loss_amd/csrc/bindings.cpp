@@ -1375,6 +1375,20 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
   }
 };
 
+// One call for a program that may or may not want gradients: y, and the sum with a residual.
+bool wants_grad(const torch::Tensor& t) { return t.requires_grad(); }
+bool wants_grad(const c10::optional<torch::Tensor>& t) { return t.has_value() && t->requires_grad(); }
+
+std::vector<torch::Tensor> rms_norm(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
+                                    const c10::optional<torch::Tensor>& residual, double eps) {
+  if (torch::GradMode::is_enabled() && (wants_grad(input) || wants_grad(weight) || wants_grad(residual)))
+    return RmsNormNode::apply(input, weight, residual, eps);
+  no_tangent("rms_norm", input, weight, residual);  // (copying drops it)
+  auto r = rms_norm_forward(input.contiguous(), contiguous_or_none(weight), contiguous_or_none(residual), eps, false);
+  r.resize(residual.has_value() ? 2 : 1);
+  return r;
+}
+
 std::vector<torch::Tensor> rms_norm_autograd(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
                                              const c10::optional<torch::Tensor>& residual, double eps) {
   return RmsNormNode::apply(input, weight, residual, eps);
@@ -1405,11 +1419,11 @@ std::vector<torch::Tensor> mx_quantize(const torch::Tensor& input, const std::st
   no_tangent("mx_quantize", input);
   const int f = mx_format_code(format);
   no_gradient("mx_quantize", {&input});
-  ML_CHECK_INPUT(input);
+  TORCH_CHECK(input.is_cuda(), "input must be a CUDA tensor");
   TORCH_CHECK(input.dim() >= 1 && input.size(-1) % 32 == 0, "mx_quantize: the last dimension must be a multiple of 32");
   const int dt = dtype_code(input, "input");
   const c10::DeviceGuard guard(input.device());
-  const auto x = on_16_bytes(input);
+  const auto x = on_16_bytes(input.contiguous());
   const auto out = mx_empty(x, f);
   const int64_t width = x.size(-1), rows = width ? x.numel() / width : 0;
   ml_ok(ml_mx_quantize(dt, x.data_ptr(), rows, width, f, out.first.data_ptr(), (uint8_t*)out.second.data_ptr(), cur_stream()));
@@ -1417,10 +1431,12 @@ std::vector<torch::Tensor> mx_quantize(const torch::Tensor& input, const std::st
 }
 
 // codes, scales, the sum (undefined without a residual)
-std::vector<torch::Tensor> rms_norm_mx_forward(const torch::Tensor& input, const c10::optional<torch::Tensor>& weight,
-                                               const c10::optional<torch::Tensor>& residual, double eps,
+std::vector<torch::Tensor> rms_norm_mx_forward(const torch::Tensor& given, const c10::optional<torch::Tensor>& given_weight,
+                                               const c10::optional<torch::Tensor>& given_residual, double eps,
                                                const std::string& format) {
-  no_tangent("rms_norm_mx", input, weight, residual);
+  no_tangent("rms_norm_mx", given, given_weight, given_residual);  // (copying drops it)
+  const auto input = given.contiguous();
+  const auto weight = contiguous_or_none(given_weight), residual = contiguous_or_none(given_residual);
   const int f = mx_format_code(format);
   const torch::Tensor none;
   no_gradient("rms_norm_mx", {&input, weight.has_value() ? &*weight : &none, residual.has_value() ? &*residual : &none});
@@ -1460,10 +1476,13 @@ int mx_operand(const char* what, const torch::Tensor& codes, const torch::Tensor
   return e2m1 ? ML_MX_E2M1 : ML_MX_E4M3;
 }
 
-torch::Tensor grouped_matmul_mx(const torch::Tensor& input, const torch::Tensor& scales, const torch::Tensor& weight,
-                                const torch::Tensor& weight_scales, const c10::optional<torch::Tensor>& offsets,
+torch::Tensor grouped_matmul_mx(const torch::Tensor& given, const torch::Tensor& given_scales, const torch::Tensor& given_weight,
+                                const torch::Tensor& given_weight_scales, const c10::optional<torch::Tensor>& given_offsets,
                                 torch::ScalarType dtype) {
-  no_tangent("grouped_matmul_mx", input, scales, weight, weight_scales);
+  no_tangent("grouped_matmul_mx", given, given_scales, given_weight, given_weight_scales);
+  const auto input = given.contiguous(), scales = given_scales.contiguous(), weight = given_weight.contiguous(),
+             weight_scales = given_weight_scales.contiguous();
+  const auto offsets = contiguous_or_none(given_offsets);
   no_gradient("grouped_matmul_mx", {&input, &scales, &weight, &weight_scales});
   int64_t K, Kw;
   const int fx = mx_operand("input", input, scales, K), fw = mx_operand("weight", weight, weight_scales, Kw);
@@ -1508,7 +1527,8 @@ torch::Tensor grouped_matmul_mx(const torch::Tensor& input, const torch::Tensor&
 // --------------------------------------------------------------------------
 // rows by expert (no counterpart in the reference)
 // --------------------------------------------------------------------------
-std::vector<torch::Tensor> sort_by_expert(const torch::Tensor& ids, int64_t experts) {
+std::vector<torch::Tensor> sort_by_expert(const torch::Tensor& given, int64_t experts) {
+  const auto ids = given.contiguous();
   ML_CHECK_INPUT(ids);
   TORCH_CHECK(ids.scalar_type() == torch::kLong, "sort_by_expert: expert numbers must be int64");
   TORCH_CHECK(ids.dim() == 2, "sort_by_expert: expert numbers must be (tokens, k)");
@@ -1620,6 +1640,12 @@ struct ToExpertsNode : public torch::autograd::Function<ToExpertsNode> {
   }
 };
 
+torch::Tensor to_experts(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets) {
+  if (torch::GradMode::is_enabled() && wants_grad(input)) return ToExpertsNode::apply(input, slots, offsets);
+  no_tangent("to_experts", input);  // (copying drops it)
+  return to_experts_forward(input.contiguous(), slots.contiguous(), offsets.contiguous());
+}
+
 torch::Tensor to_experts_autograd(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets) {
   return ToExpertsNode::apply(input, slots, offsets);
 }
@@ -1650,6 +1676,14 @@ struct FromExpertsNode : public torch::autograd::Function<FromExpertsNode> {
     return once({r[0], torch::Tensor(), torch::Tensor(), r[1]}, "the backward of from_experts cannot be differentiated");
   }
 };
+
+torch::Tensor from_experts(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets,
+                           const c10::optional<torch::Tensor>& weights) {
+  if (torch::GradMode::is_enabled() && (wants_grad(input) || wants_grad(weights)))
+    return FromExpertsNode::apply(input, slots, offsets, weights);
+  no_tangent("from_experts", input, weights);  // (copying drops it)
+  return from_experts_forward(input.contiguous(), slots.contiguous(), offsets.contiguous(), contiguous_or_none(weights));
+}
 
 torch::Tensor from_experts_autograd(const torch::Tensor& input, const torch::Tensor& slots, const torch::Tensor& offsets,
                                     const c10::optional<torch::Tensor>& weights) {
@@ -1761,6 +1795,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_matmul_autograd", &grouped_matmul_autograd,
         "Grouped product as a C++ autograd node, differentiable in input and weight (HIP)", py::arg("input"),
         py::arg("weight"), py::arg("offsets"), py::arg("transposed") = false);
+  m.def("rms_norm", &rms_norm, "Root-mean-square norm, with a node where a gradient is wanted: output, and the sum (HIP)",
+        py::arg("input"), py::arg("weight"), py::arg("residual"), py::arg("eps"));
+  m.def("to_experts", &to_experts, "Tokens' rows at their experts' places, with a node where a gradient is wanted (HIP)",
+        py::arg("input"), py::arg("slots"), py::arg("offsets"));
+  m.def("from_experts", &from_experts, "Experts' rows summed back, with a node where a gradient is wanted (HIP)",
+        py::arg("input"), py::arg("slots"), py::arg("offsets"), py::arg("weights") = py::none());
   m.def("rms_norm_forward", &rms_norm_forward,
         "Root-mean-square norm: output, the sum with a residual, and per row 1/rms if asked for (HIP)", py::arg("input"),
         py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("want_stats") = false);

@@ -49,22 +49,17 @@ class FromExpertsFunction:
 
 def sort_by_expert(ids, experts):
     """The order of (T, k) int64 expert numbers by expert (at most 4,000 experts)."""
-    return ExpertOrder(*mask_loss.sort_by_expert(ids.contiguous(), int(experts)))
+    return ExpertOrder(*mask_loss.sort_by_expert(ids, experts))
 
 
 def to_experts(input, order):
     """Row ``order.slots[t, j]`` of the result (T * k, D) is ``input[t]``, for input (T, D) of
     any dtype (gradients: float32, bfloat16 or float16); zeros in the dropped places."""
-    if torch.is_grad_enabled() and input.requires_grad:
-        return ToExpertsFunction.apply(input, order.slots, order.offsets)
-    return mask_loss.to_experts_forward(input.contiguous(), order.slots.contiguous(), order.offsets.contiguous())
+    return mask_loss.to_experts(input, order.slots, order.offsets)
 
 
 def from_experts(input, order, weights=None):
     """``sum_j weights[t, j] * input[order.slots[t, j]]`` for every token t, in float32 and
     rounded once; input (T * k, D), weights (T, k) in its dtype or float32, or None for
     ones."""
-    if torch.is_grad_enabled() and (input.requires_grad or (weights is not None and weights.requires_grad)):
-        return FromExpertsFunction.apply(input, order.slots, order.offsets, weights)
-    return mask_loss.from_experts_forward(input.contiguous(), order.slots.contiguous(), order.offsets.contiguous(),
-                                          None if weights is None else weights.contiguous())
+    return mask_loss.from_experts(input, order.slots, order.offsets, weights)

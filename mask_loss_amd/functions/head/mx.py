@@ -20,7 +20,7 @@ def mx_quantize(input, format="e4m3"):
     (2^(floor(log2 max) - 2) for e2m1, - 8 for e4m3); values are divided by it, rounded to
     nearest, ties to even, and held to the format's largest.  A block with a NaN or an infinity has the
     scale NaN and reads as NaN.  No gradient is provided."""
-    return tuple(mask_loss.mx_quantize(input.contiguous(), format))
+    return tuple(mask_loss.mx_quantize(input, format))
 
 
 def grouped_matmul_mx(input, scales, weight, weight_scales, offsets=None, dtype=torch.bfloat16):
@@ -32,5 +32,4 @@ def grouped_matmul_mx(input, scales, weight, weight_scales, offsets=None, dtype=
     With an e4m3 operand and a 16-bit ``dtype`` the matrix instruction drops, among eight neighbours of the reduced index,
     what lies over 13 bits below their largest product (1.5e-5 of a result's size with normal operands); with
     float32 nothing is dropped, at half the rate, and values of 2^128 and more count as infinite.  No gradient is provided."""
-    return mask_loss.grouped_matmul_mx(input.contiguous(), scales.contiguous(), weight.contiguous(),
-                                       weight_scales.contiguous(), None if offsets is None else offsets.contiguous(), dtype)
+    return mask_loss.grouped_matmul_mx(input, scales, weight, weight_scales, offsets, dtype)

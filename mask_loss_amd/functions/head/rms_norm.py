@@ -8,8 +8,6 @@ float32, and its gradient its own.  The statistics are float32.  Gradients are n
 differentiated a second time, and forward-mode derivatives raise."""
 from __future__ import annotations
 
-import torch
-
 import mask_loss_amd  # noqa: F401  (registers the `mask_loss` extension)
 import mask_loss
 
@@ -20,7 +18,7 @@ class RMSNormFunction:
 
     @staticmethod
     def apply(input, weight=None, eps=1e-6, residual=None):
-        out = mask_loss.rms_norm_autograd(input, weight, residual, float(eps))
+        out = mask_loss.rms_norm_autograd(input, weight, residual, eps)
         return out[0] if residual is None else tuple(out)
 
 
@@ -32,18 +30,13 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None):
     input's shape and dtype s is their sum, rounded to that dtype, and the result is
     (norm, s): s is the residual of the next layer, and its gradient comes back
     through both."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, residual)):
-        return RMSNormFunction.apply(input, weight, eps, residual)
-    y, s, _ = mask_loss.rms_norm_forward(input.contiguous(), None if weight is None else weight.contiguous(),
-                                         None if residual is None else residual.contiguous(), float(eps))
-    return y if residual is None else (y, s)
+    out = mask_loss.rms_norm(input, weight, residual, eps)
+    return out[0] if residual is None else (out[0], out[1])
 
 
 def rms_norm_mx(input, weight=None, eps=1e-6, residual=None, format="e4m3"):
     """``rms_norm`` whose norm comes out quantised from float32, as ``mx_quantize``
     does it: (codes, scales), or (codes, scales, s) with a residual.  D is a multiple of 32.
     For inference: no gradient is provided."""
-    codes, scales, s = mask_loss.rms_norm_mx_forward(input.contiguous(), None if weight is None else weight.contiguous(),
-                                                     None if residual is None else residual.contiguous(), float(eps),
-                                                     format)
+    codes, scales, s = mask_loss.rms_norm_mx_forward(input, weight, residual, eps, format)
     return (codes, scales) if residual is None else (codes, scales, s)

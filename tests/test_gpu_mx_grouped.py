@@ -94,7 +94,7 @@ def compare(x, w, offsets, dtype, drops):
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("fx,fw", PAIRS)
 @pytest.mark.parametrize("K", [32, 64, 96, 128, 160, 224, 256, 288, 512, 1056, 2048])
-@pytest.mark.parametrize("rows,N,offsets", [(20, 40, [0, 7, 7, 20]), (300, 129, [0, 131, 150, 300])])
+@pytest.mark.parametrize("rows,N,offsets", [(20, 40, [0, 7, 7, 20]), (75, 70, [0, 30, 33, 75]), (300, 129, [0, 131, 150, 300])])
 def test_exact_products(dt, fx, fw, K, rows, N, offsets):
     """Products that no format drops bits of: few rows to a group, and many."""
     x, w = operand((rows, K), fx, K, True, (125, 130)), operand((3, N, K), fw, K + 1, True, (125, 130))
