@@ -256,8 +256,10 @@ __global__ __launch_bounds__(kRowThreads) void to_experts_kernel(const uint8_t* 
   }
 }
 
-// out[t] = sum_j w[t, j] rows[slot(t, j)] (w null: ones), T lanes to a token.
-template <int DT, int T>
+// out[t] = sum_j w[t, j] rows[slot(t, j)] (w null: ones), T lanes to a token.  ONCE: more rows than the caches keep for the
+// gradient pass, read past them: what other kernels wrote is not driven out in between (8,192 tokens x 8 x 1,024 bf16, all
+// kernels of a training pass 172 -> 155 us, 16,384 x 2 x 2,048 201 -> 198; rows that fit, 20,011 x 257 f32, 57 -> 62).
+template <int DT, int T, bool ONCE>
 __global__ __launch_bounds__(kRowThreads) void from_experts_kernel(const void* rowsv, const void* w, int wf32, int64_t tokens,
                                                                    int64_t k, int64_t D, const int64_t* slots,
                                                                    const int64_t* offsets, int64_t experts, void* outv) {
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kRowThreads) void from_experts_kernel(const void* r
 #pragma unroll
         for (int q = 0; q < kFlight; ++q) {
           v[q] = C{};
-          if (from[q]) v[q].load(from[q] + c, D - c);
+          if (from[q]) v[q].template load<false, ONCE>(from[q] + c, D - c);
         }
 #pragma unroll
         for (int q = 0; q < kFlight; ++q)
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(kRowThreads) void from_experts_kernel(const void* r
 }
 
 // drows[slot] = w dout[t] and dw = <dout[t], rows[slot]> of an assignment, T lanes to it; either may be null.
-template <int DT, int T>
+template <int DT, int T, bool ONCE>
 __global__ __launch_bounds__(kRowThreads) void from_experts_backward_kernel(const void* gv, const void* rowsv, const void* w,
                                                                             int wf32, int64_t n, int64_t k, int64_t D,
                                                                             const int64_t* slots, const int64_t* offsets,
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(kRowThreads) void from_experts_backward_kernel(cons
         C g, v;
         g.load(dout + t * D + c, D - c);
         if (dw) {
-          v.load(rows + p * D + c, D - c);
+          v.template load<false, ONCE>(rows + p * D + c, D - c);
 #pragma unroll
           for (int i = 0; i < V; ++i) s[0] = fmaf(to_f32<DT>(g.e[i]), to_f32<DT>(v.e[i]), s[0]);
         }
@@ -360,6 +362,9 @@ int by_lanes(int64_t chunks, int64_t rows, F&& f) {
   if (chunks > 64 && rows <= 2048) return f(std::integral_constant<int, 256>());
   return f(std::integral_constant<int, 64>());
 }
+constexpr int64_t kOnceBytes = (int64_t)64 << 20;
+template <int DT>
+bool read_once(int64_t n, int64_t D) { return n * D * (int64_t)sizeof(typename Elem<DT>::raw) >= kOnceBytes; }
 dim3 row_grid(int64_t rows, int T) { return dim3((unsigned)std::min<int64_t>(ceil_div(rows * T, kRowThreads), 1 << 20)); }
 
 int experts_check(const char* who, int64_t tokens, int64_t k, int64_t experts) {
@@ -399,8 +404,13 @@ int from_experts(const void* rows, const void* w, int wf32, int64_t tokens, int6
                  const int64_t* offsets, int64_t experts, void* out, hipStream_t st) {
   return by_lanes(ceil_div(D, RowChunk<DT>::V), tokens, [&](auto tc) {
     constexpr int T = decltype(tc)::value;
-    hipLaunchKernelGGL((from_experts_kernel<DT, T>), row_grid(tokens, T), dim3(kRowThreads), 0, st, rows, w, wf32, tokens, k, D,
-                       slots, offsets, experts, out);
+    const dim3 grid = row_grid(tokens, T), blk(kRowThreads);
+    if (read_once<DT>(tokens * k, D))
+      hipLaunchKernelGGL((from_experts_kernel<DT, T, true>), grid, blk, 0, st, rows, w, wf32, tokens, k, D, slots, offsets,
+                         experts, out);
+    else
+      hipLaunchKernelGGL((from_experts_kernel<DT, T, false>), grid, blk, 0, st, rows, w, wf32, tokens, k, D, slots, offsets,
+                         experts, out);
     return check_launch("from_experts");
   });
 }
@@ -411,8 +421,13 @@ int from_experts_backward(const void* g, const void* rows, const void* w, int wf
                           hipStream_t st) {
   return by_lanes(ceil_div(D, RowChunk<DT>::V), n, [&](auto tc) {
     constexpr int T = decltype(tc)::value;
-    hipLaunchKernelGGL((from_experts_backward_kernel<DT, T>), row_grid(n, T), dim3(kRowThreads), 0, st, g, rows, w, wf32, n, k,
-                       D, slots, offsets, experts, drows, dw);
+    const dim3 grid = row_grid(n, T), blk(kRowThreads);
+    if (read_once<DT>(n, D))
+      hipLaunchKernelGGL((from_experts_backward_kernel<DT, T, true>), grid, blk, 0, st, g, rows, w, wf32, n, k, D, slots,
+                         offsets, experts, drows, dw);
+    else
+      hipLaunchKernelGGL((from_experts_backward_kernel<DT, T, false>), grid, blk, 0, st, g, rows, w, wf32, n, k, D, slots,
+                         offsets, experts, drows, dw);
     return check_launch("from_experts_backward");
   });
 }

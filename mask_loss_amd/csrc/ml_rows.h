@@ -55,27 +55,29 @@ struct RowChunk {
   static constexpr int V = N;
   typename Elem<DT>::raw e[V];
 
-  // zeros where n, the elements left, runs out; WHOLE: all or none of the chunk is left
-  template <bool WHOLE = false>
+  // zeros where n, the elements left, runs out; WHOLE: all or none of the chunk is left; ONCE: past the caches, which keep what is
+  // read again and what waits to be written
+  template <bool WHOLE = false, bool ONCE = false>
   __device__ __forceinline__ void load(const typename Elem<DT>::raw* p, int64_t n) {
     if constexpr (V == 1) {
       e[0] = n > 0 ? *p : typename Elem<DT>::raw(0);
     } else if (n >= V) {
-      const u32x4_t v = *(const u32x4_near_t*)p;
+      const u32x4_t v = ONCE ? __builtin_nontemporal_load((const u32x4_near_t*)p) : *(const u32x4_near_t*)p;
       __builtin_memcpy(e, &v, 16);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) e[j] = !WHOLE && j < n ? p[j] : typename Elem<DT>::raw(0);
     }
   }
-  template <bool WHOLE = false>
+  template <bool WHOLE = false, bool ONCE = false>
   __device__ __forceinline__ void store(typename Elem<DT>::raw* p, int64_t n) const {
     if constexpr (V == 1) {
       if (n > 0) *p = e[0];
     } else if (n >= V) {
       u32x4_t v;
       __builtin_memcpy(&v, e, 16);
-      *(u32x4_near_t*)p = v;
+      if constexpr (ONCE) __builtin_nontemporal_store(v, (u32x4_near_t*)p);
+      else *(u32x4_near_t*)p = v;
     } else if constexpr (!WHOLE) {
 #pragma unroll
       for (int j = 0; j < V - 1; ++j)
