@@ -453,7 +453,8 @@ int ml_mx_quantize(int dtype, const void* x, int64_t rows, int64_t width, int fo
                    ml_stream_t stream);
 
 /* Products of ragged groups of microscaled rows with one microscaled matrix per group: ml_grouped_matmul_forward's groups,
- * matrices (matrices, N, K) and limits, for inference.  x: codes (rows, K) in x_format on 16-byte boundaries and x_scales
+ * matrices (matrices, N, K) and limits, for inference; with few rows to a group the parts of the output that may not be 2^24
+ * or more have 16 rows by 32 columns.  x: codes (rows, K) in x_format on 16-byte boundaries and x_scales
  * (rows, K / 32); weight: codes (matrices, N, K) in weight_format on 16-byte boundaries and weight_scales (matrices, N, K / 32);
  * K a multiple of 32; y (rows, N) in `dtype`.
  * Sums are float32 in an order that the shape, the formats, the groups' sizes and whether offsets are given fix, rounded

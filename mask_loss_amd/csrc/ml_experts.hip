@@ -17,7 +17,9 @@
 //
 // Everything else is bound by HBM: there reads each row once and writes it k times, back and the gradients
 // read or write each assignment's row once.  A token (back's gradient: an assignment) is a wave's or 16 lanes', which
-// pass over the row in 16-byte chunks, at any alignment; sums are float32 in the order of j, rounded once.
+// pass over the row in 16-byte chunks, at any alignment; sums are float32 in the order of j, rounded once.  8,192 tokens x 8 of 64
+// experts, 1,024 wide, bf16 (17 and 134 MB): order 12 us, there 29 (5.2 TB/s), back 32, gradient of back 58 (4.9 TB/s), of there 32;
+// single elements at odd widths cost more (8,192 x 4 x 1,025 bf16 back 29 / 48 us, its gradient 36 / 69; 513 f32 27 / 29, 33 / 40).
 #include <algorithm>
 
 #include "ml_rows.h"

@@ -221,6 +221,26 @@ def test_no_size():
     x, w = operand((4, 0), "e4m3", 1), operand((2, 5, 0), "e2m1", 1)
     y = call(x, w, [0, 2, 4], torch.bfloat16)
     assert y.shape == (4, 5) and not y.any()
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w = operand((300, 0), "e4m3", 1), operand((2, 5, 0), "e2m1", 1)
+        y = call(x, w, [0, 100, 290], dtype)
+        assert y.shape == (300, 5) and not y.any()
+
+
+@pytest.mark.parametrize("each", [1, 40])
+@pytest.mark.parametrize("matrices", [4000, 40])
+def test_most_groups(each, matrices):
+    """4,000 groups, the most: their borders fill much of the LDS."""
+    rows, K, N = 4000 * each, 128, 24
+    x, w = operand((rows, K), "e4m3", 3, True, (127, 128)), operand((matrices, N, K), "e2m1", 4, True, (127, 128))
+    gen = torch.Generator().manual_seed(5)
+    offsets = [0, *torch.randint(0, rows + 1, (3999,), generator=gen).sort().values.tolist(), rows]
+    y = call(x, w, offsets, torch.float32)
+    group = torch.searchsorted(torch.tensor(offsets[1:]), torch.arange(rows), right=True) % matrices
+    xv, wv = mx.values(x[0]).float().cuda(), mx.values(w[0]).float().cuda()
+    for lo in range(0, rows, 20000):  # every partial sum is a float32: any order
+        part = group[lo:lo + 20000].cuda()
+        assert torch.equal(y[lo:lo + 20000], (xv[lo:lo + 20000, None, :] * wv[part]).sum(-1))
 
 
 def test_layouts():
