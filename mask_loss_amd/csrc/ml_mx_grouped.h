@@ -59,6 +59,45 @@ __device__ __forceinline__ f32x4_t mx_mma(const MxFrag<FA>& a, const MxFrag<FB>&
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.wide(), b.wide(), c, ca, cb, 0, (int)a.scale, 0, (int)b.scale);
 }
 
+// Eight values in bfloat16 with their scale (of e2m1: the low word).  The conversion takes the exponent field alone of
+// its scale, with 0 for 2^-127 and 255 for NaN whatever the value (all 256 codes of both formats checked).
+template <int F>
+__device__ __forceinline__ bf16x8_t mx_bf16(uint32_t p0, uint32_t p1, uint32_t code) {
+  const float scale = __uint_as_float(code << 23);
+  bf16x2_t v[4];
+  if constexpr (F == ML_MX_E4M3) {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p0, scale, false);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p0, scale, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p1, scale, false);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p1, scale, true);
+  } else {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, scale, 0);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, scale, 1);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, scale, 2);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, scale, 3);
+  }
+  bf16x8_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = v[i][0];
+    o[2 * i + 1] = v[i][1];
+  }
+  return o;
+}
+
+// Block b (32 values) of rows row0 .. of an operand's LDS image: lane l holds values 8 (l / 16) .. of row l % 16, whose
+// scale is `code`.
+template <int F, class O>
+__device__ __forceinline__ bf16x8_t mx_block(const unsigned char* lds, int row0, int b, uint32_t code) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  if constexpr (F == ML_MX_E4M3) {
+    const u32x2_t p = *(const u32x2_t*)(lds + (row0 + r) * O::ROWB + (O::swizzled(r, 2 * b + (g >> 1)) << 4) + 8 * (g & 1));
+    return mx_bf16<F>(p[0], p[1], code);
+  } else {
+    return mx_bf16<F>(*(const uint32_t*)(lds + (row0 + r) * O::ROWB + (O::swizzled(r, b) << 4) + 4 * g), 0u, code);
+  }
+}
+
 // One operand of a tile: R rows by a step of BK values, and their scales.
 template <int F, int R, int NT, int BK>
 struct MxOperand : Operand<ML_BF16, true, R, NT, mx_bytes(F, BK)> {
@@ -78,32 +117,7 @@ struct MxOperand : Operand<ML_BF16, true, R, NT, mx_bytes(F, BK)> {
 
   // Block b (32 values) of rows row0 .., in bfloat16 with its scale: lane l holds values 8 (l / 16) .. of row l % 16.
   static __device__ __forceinline__ bf16x8_t block(const unsigned char* lds, int row0, int b) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t code = lds[O::BYTES + (row0 + r) * 4 + b];
-    const float scale = __uint_as_float(max(code << 23, 0x00400000u));  // 2^-127 is below the normal range
-    bf16x2_t v[4];
-    if constexpr (F == ML_MX_E4M3) {
-      const u32x2_t p = *(const u32x2_t*)(lds + (row0 + r) * O::ROWB + (O::swizzled(r, 2 * b + (g >> 1)) << 4) + 8 * (g & 1));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        v[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p[i], scale, false);
-        v[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(p[i], scale, true);
-      }
-    } else {
-      const uint32_t p = *(const uint32_t*)(lds + (row0 + r) * O::ROWB + (O::swizzled(r, b) << 4) + 4 * g);
-      v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p, scale, 0);
-      v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p, scale, 1);
-      v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p, scale, 2);
-      v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p, scale, 3);
-    }
-    bf16x8_t o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (code == 255u) v[i] = __builtin_bit_cast(bf16x2_t, 0x7FC07FC0u);  // NaN
-      o[2 * i] = v[i][0];
-      o[2 * i + 1] = v[i][1];
-    }
-    return o;
+    return mx_block<F, O>(lds, row0, b, lds[O::BYTES + (row0 + (threadIdx.x & 15)) * 4 + b]);
   }
 };
 
@@ -129,7 +143,7 @@ struct MxScales {
   }
 };
 
-// WM x WN waves make BM x BN outputs in OUT.  Work items and dynamic LDS as grouped_kernel's.
+// Any K, scales on any byte.  WM x WN waves make BM x BN outputs in OUT.  Work items and dynamic LDS as grouped_kernel's.
 template <int FA, int FB, int OUT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void mx_kernel(MxArgs x) {
   constexpr int NT = 64 * WM * WN, BK = mx_step(FA, FB), TM = BM / WM / 16, TN = BN / WN / 16;
@@ -355,8 +369,41 @@ struct MxRows {
   }
 };
 
+// The same for products in bfloat16: lane group g has, of each 128 values, those 16 g .. of the first 64 and of the last, in
+// either format, and their row's 16 scales.
+template <int F>
+struct MxExactRows {
+  using P = std::conditional_t<F == ML_MX_E4M3, u32x4_t, u32x2_t>;
+  P v[4][2];
+  uint32_t scale[4];
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales, int left) {
+    const int g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = 128 * s + 64 * i + 16 * g;
+        v[s][i] = P{};
+        if (at < left) v[s][i] = *(const P*)(codes + mx_bytes(F, at));
+      }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      MxScales<128> c;
+      c.load(scales + 4 * s, left / kMxBlock - 4 * s);
+      scale[s] = c.v[0];
+    }
+  }
+  // eight of them, h: the first or the last of the 16
+  __device__ __forceinline__ bf16x8_t eight(int s, int i, int h) const {
+    const uint32_t code = scale[s] >> (16 * i + 8 * (threadIdx.x >> 5 & 1)) & 255u;
+    if constexpr (F == ML_MX_E4M3) return mx_bf16<F>(v[s][i][2 * h], v[s][i][2 * h + 1], code);
+    else return mx_bf16<F>(v[s][i][h], 0u, code);
+  }
+};
+
 template <int FA, int FB, int OUT, int MT>
 __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
+  constexpr bool EXACT = mx_exact(FA, FB, OUT);
   constexpr int BM = 16 * MT, NT = kFewColumns / 16;
   __shared__ f32x4_t part[3][MT * NT][64];
   extern __shared__ int e[];
@@ -393,23 +440,38 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const MxTurn turn;
   for (int k = wave * kFewStep; k < K; k += 4 * kFewStep) {
-    MxRows<FA> ra[MT];
-    MxRows<FB> rb[NT];
+    std::conditional_t<EXACT, MxExactRows<FA>, MxRows<FA>> ra[MT];
+    std::conditional_t<EXACT, MxExactRows<FB>, MxRows<FB>> rb[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) rb[i].load(pb[i] + mx_bytes(FB, k), sb[i] + k / kMxBlock, K - k);
 #pragma unroll
     for (int j = 0; j < MT; ++j) ra[j].load(pa[j] + mx_bytes(FA, k), sa[j] + k / kMxBlock, K - k);
-    uint32_t ta[MT], tb[NT];
+    if constexpr (EXACT) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) tb[i] = turn(rb[i].scale);  // byte s: of the 128 values from 128 s on
+      for (int q = 0; q < 16; ++q) {
+        bf16x8_t xa[MT], xb[NT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) ta[j] = turn(ra[j].scale);
+        for (int i = 0; i < NT; ++i) xb[i] = rb[i].eight(q >> 2, q >> 1 & 1, q & 1);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+        for (int j = 0; j < MT; ++j) xa[j] = ra[j].eight(q >> 2, q >> 1 & 1, q & 1);
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = mx_mma_at(s, s, rb[i].frag(s), ra[j].frag(s), tb[i], ta[j], acc[i][j]);
+          for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[i], xa[j], acc[i][j], 0, 0, 0);
+      }
+    } else {
+      uint32_t ta[MT], tb[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) tb[i] = turn(rb[i].scale);  // byte s: of the 128 values from 128 s on
+#pragma unroll
+      for (int j = 0; j < MT; ++j) ta[j] = turn(ra[j].scale);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[i][j] = mx_mma_at(s, s, rb[i].frag(s), ra[j].frag(s), tb[i], ta[j], acc[i][j]);
+    }
   }
   if (wave)
 #pragma unroll
@@ -549,9 +611,15 @@ __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, co
 // What bounds it (16,384 rows in 16 groups, K = 1,024, N = 4,096, e2m1: 62 us, 76 to 78 where the operands come from memory; the
 // matrix instructions alone run at 7,400 TFLOP/s on random values and are busy for 2.3 of the 7 us of a compute unit's
 // two tiles): the latency of the loads behind two stages, and the stores.  An earlier form that took 72 us took 54 without its
-// stores, 46 without loads and LDS reads, 44 without either.
+// stores, 46 without loads and LDS reads, 44 without either.  Non-temporal stores take 65 for the 76, but what reads the result next
+// then waits for memory (with a product by 2 behind it 133 to 148 us, 129 as it is); half of the workgroups starting
+// a half tile later, to store while the others multiply, changes nothing.
+//
+// Products in bfloat16 (mx_exact) read a block of 32 of both operands at once and convert it, the next one's conversions
+// between the products (without: 1 to 3% more): 32 of 4 cycles for 16 products of 16, 1,100 TFLOP/s at 8,192 x 8,192 x 4,096.
 template <int FA, int FB, int OUT, int BM, int BN, int WM, int WN, int BK, int OCC, int SW>
 __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void mx_ring_kernel(MxArgs x) {
+  constexpr bool EXACT = mx_exact(FA, FB, OUT);
   constexpr int NS = 2, NW = WM * WN, H = BK / 128, TM = BM / WM / 16, TN = BN / WN / 16;
   using OA = MxRing<FA, BM, NW, BK>;
   using OB = MxRing<FB, BN, NW, BK>;
@@ -687,18 +755,25 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void mx_ring_kerne
                                       : slots + stage * SLOT + (h * ROWS + row0 + lane) * 4;
     return *(const uint32_t*)p;
   };
+  auto scales_of = [&](int stage, int part, int row0) {  // lane l's: row row0 + l % 16, its four of the stage
+    const int row = row0 + (lane & 15);
+    return *(const uint32_t*)(SW == 16 ? slots + at * SLOT + row * 16 + part * 4 : slots + stage * SLOT + row * 4);
+  };
   MxFrag<FA> fa[TM];
   MxFrag<FB> fb[TN], fn[TN];
   uint32_t sa[TM / 4], sb[TN / 4];
-  ring_wait<OA::PER + OB::PER>();
+  constexpr int P = OA::PER + OB::PER;  // loads of a stage's codes
+  if constexpr (!EXACT) {
+    ring_wait<P>();
 #pragma unroll
-  for (int i = 0; i < TN; ++i) fb[i] = frag_b(0, i, 0);
+    for (int i = 0; i < TN; ++i) fb[i] = frag_b(0, i, 0);
 #pragma unroll
-  for (int i = 0; i < TM; ++i) fa[i] = frag_a(0, i, 0);
+    for (int i = 0; i < TM; ++i) fa[i] = frag_a(0, i, 0);
 #pragma unroll
-  for (int i = 0; i < TM / 4; ++i) sa[i] = turn(scale(0, 0, wm + 64 * i, 0));
+    for (int i = 0; i < TM / 4; ++i) sa[i] = turn(scale(0, 0, wm + 64 * i, 0));
 #pragma unroll
-  for (int i = 0; i < TN / 4; ++i) sb[i] = turn(scale(0, 0, BM + wn + 64 * i, 0));
+    for (int i = 0; i < TN / 4; ++i) sb[i] = turn(scale(0, 0, BM + wn + 64 * i, 0));
+  }
   int cur = 0;     // the stage in turn (SW = 4)
   bool credit = false;  // a stage's loads were issued before the last tile's stores
   for (int n = 0; n < count; ++n) {
@@ -734,6 +809,52 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void mx_ring_kerne
 #pragma unroll
       for (int part = 0; part < SUPER; ++part) {
         const int stage = SW == 16 ? part % NS : cur, next = SW == 16 ? (part + 1) % NS : cur ^ 1;
+        if constexpr (EXACT) {
+          // the next stage's loads (and the last tile's stores) may be under way
+          if (part == 0 && credit) ring_wait<(P + ST < 63 ? P + ST : 63)>();
+          else ring_wait<P>();
+          credit = credit && part != 0;
+          uint32_t ra[TM], rb[TN];  // lane l's: the four scales of row l % 16
+#pragma unroll
+          for (int j = 0; j < TM; ++j) ra[j] = scales_of(stage, part, wm + 16 * j);
+#pragma unroll
+          for (int i = 0; i < TN; ++i) rb[i] = scales_of(stage, part, BM + wn + 16 * i);
+          const unsigned char* ca = lds + stage * CODES;
+          bf16x8_t xa[2][TM], xb[2][TN];
+          auto blocks = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+              xb[b & 1][i] = mx_block<FB, typename OB::O>(ca + OA::BYTES, wn + 16 * i, b, rb[i] >> (8 * b) & 255u);
+#pragma unroll
+            for (int j = 0; j < TM; ++j)
+              xa[b & 1][j] = mx_block<FA, typename OA::O>(ca, wm + 16 * j, b, ra[j] >> (8 * b) & 255u);
+          };
+          blocks(0);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if (b < 3) blocks(b + 1);
+#pragma unroll
+            for (int j = 0; j < TM; ++j)
+#pragma unroll
+              for (int i = 0; i < TN; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[b & 1][i], xa[b & 1][j], acc[i][j], 0, 0, 0);
+            if (b < 3) {  // the next block's reads and conversions between the products
+              __builtin_amdgcn_sched_group_barrier(0x100, TM + TN, 0);
+#pragma unroll
+              for (int q = 0; q < TM * TN; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          ring_wait<63>();  // (no load is waited for: every wave has read the stage)
+          load(stage, (part + NS) % SUPER == 0);
+          if (part + 1 == SUPER) at ^= 1;
+          cur ^= 1;
+          continue;
+        }
         if constexpr (H == 2) sub_step(fb, fn, stage, part, 1);
         // the products so far stay on this side of the wait: sunk to the next, they would keep both fragments (nothing is
         // read here: the compiler puts the wait states of a matrix instruction in front of the result's first reader)

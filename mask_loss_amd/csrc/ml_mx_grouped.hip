@@ -10,15 +10,13 @@ namespace {
 constexpr int64_t kMaxGroups = 4000;   // their edges and tile counts fit the LDS beside the tiles
 constexpr int64_t kMaxRows = ((int64_t)1 << 31) - 4096;  // positions a step or a tile on stay 32-bit
 constexpr int64_t kMaxLength = 1 << 22;  // rows of a tile stay within 2^32 bytes of its first
-constexpr int64_t kUnits = 256;
 
-// Tiles: few rows to a group (64 where the rows are e2m1 and the matrix e4m3: a chunk for every thread), or many.
-// Many rows take the ring where K and the scales' alignment let them (us, the ring / mx_kernel; e2m1 by e2m1 unless named):
-// 16,384 rows in 16 groups, K = 1,024, N = 4,096 62 / 102, e4m3 by e2m1 83 / 128, e4m3 by e4m3 108 / 159; 4,096 rows in 8 groups, K =
-// 1,024, N = 2,736, e4m3 by e2m1 24 / 31; one matrix 8,192 x 8,192 x 8,192 359 / 446.  Larger tiles of the ring move fewer
+// Few rows to a group take mx_few_kernel's tiles, many 128 x 128: the ring where K and the scales' alignment let it, mx_kernel
+// otherwise (us, the ring / mx_kernel; e2m1 by e2m1 in bfloat16 unless named): 16,384 rows in 16 groups, K = 1,024, N = 4,096
+// 62 / 102, e4m3 by e2m1 83 / 128, in float32 174 / 228, e4m3 by e4m3 108 / 159, in float32 184 / 251; 4,096 rows in 8 groups, K = 1,024,
+// N = 2,736, e4m3 by e2m1 24 / 31, in float32 43 / 58; one matrix 8,192 x 8,192 x 8,192 359 / 446.  Larger tiles of the ring move fewer
 // bytes through LDS, but a tile's stores wait for less beside them: 128 x 256 and 256 x 256 on 8 waves take 68 and 80 for the
 // first of these (and 325 and 283 for the last, alone).
-constexpr int few_rows(int fa, int fb) { return fa == ML_MX_E2M1 && fb == ML_MX_E4M3 ? 64 : 32; }
 constexpr int kColumns = 128, kManyRows = 128, kRingSlots = 512;
 constexpr size_t kRingParts = (size_t)kRingSlots * kManyRows * kColumns * sizeof(float);
 
@@ -51,23 +49,23 @@ int mx_plan(const ml_grouped_shape* s, int fa, int fb, int out, int aligned, boo
   const double each = (double)s->rows / used;
   const bool exact = mx_exact(fa, fb, out);
   p.few = each <= 32.0;
-  p.bm = !p.few ? kManyRows : exact ? few_rows(fa, fb) : each <= 16.0 ? 16 : 32;
-  p.bn = p.few && !exact ? kFewColumns : kColumns;
-  p.ring = p.few || exact ? 0 : s->K % 512 == 0 && aligned >= 16 ? 16 : s->K % 128 == 0 && aligned >= 4 ? 4 : 0;
+  p.bm = !p.few ? kManyRows : each <= 16.0 ? 16 : 32;
+  p.bn = p.few ? kFewColumns : kColumns;
+  p.ring = p.few ? 0 : s->K % 512 == 0 && aligned >= 16 ? 16 : s->K % 128 == 0 && aligned >= 4 ? 4 : 0;
   const int64_t columns = ceil_div(s->N, p.bn);
   // values of a part of a reduction, at least one turn of the kernel's loop
   const int64_t step = p.ring == 16 ? 512 : mx_step(fa, fb), steps = std::max<int64_t>(1, ceil_div(s->K, step));
   const double x = each / p.bm, rows = used * (equal || segments == 1 ? std::ceil(x) : std::max(1.05, x + 0.5));
-  // Parts of each tile's reduction where the tiles leave slots without work.  The ring takes 2 us for 512 values of a tile, and
-  // a join 4 us and what its parts' 64 KiB take to memory and back: as many parts as cost the least, if they cost less
+  // Parts of each tile's reduction where the tiles leave slots without work.  The ring takes 2 us for 512 values of a tile, 4 in bfloat16,
+  // and a join 4 us and what its parts' 64 KiB take to memory and back: as many parts as cost the least, if they cost less
   // than none (512 x 8,192 x 1,024 25 us in parts, 43 whole; 512 x 4,096 x 4,096 29 in as many as fit, 25 whole).
   const double all = std::max(1.0, rows * columns);
-  const int64_t fit = (int64_t)((p.ring ? kRingSlots : kUnits * (p.few ? 4 : 2)) / all);
+  const int64_t fit = (int64_t)(kRingSlots / all);
   if (p.ring) {
-    const double whole = 2.0 * s->K / 512, move = 0.026 * all;
+    const double whole = (exact ? 4.0 : 2.0) * s->K / 512, move = 0.026 * all;
     const int64_t parts = std::min({fit, (int64_t)std::lround(std::sqrt(whole / move)), steps, (int64_t)64});
     p.splits = parts > 1 && s->N % 4 == 0 && whole / parts + 4.0 + move * parts < whole ? (int)parts : 1;  // (joined by whole fours)
-  } else if (p.few && !exact) {
+  } else if (p.few) {
     p.splits = 1;  // (the waves of a workgroup have parts already)
   } else {
     p.splits = (int)std::max<int64_t>(1, std::min({fit, steps / 4, (int64_t)64}));
@@ -92,34 +90,27 @@ int mx_launch(const ml_grouped_shape* s, const MxPlan& p, MxArgs& x, hipStream_t
   ProfScope ps("grouped_matmul_mx", st);
   const size_t lds = (2 * (size_t)x.g.groups + 3) * sizeof(int);  // edges, tiles of the segments
   const dim3 blk(256);
-  if constexpr (!mx_exact(FA, FB, OUT)) {
-    if (p.ring) {
-      // persistent workgroups, all that fit where tiles may be split
-      const int64_t items = ceil_div(p.bound, kXcds) * kXcds;
-      const dim3 grid((unsigned)(p.splits > 1 ? kRingSlots : std::min<int64_t>(items, kRingSlots)));
-      constexpr int BK = mx_step(FA, FB);
-      if (p.ring == 16)
-        hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 16>), grid, blk, lds, st, x);
-      else
-        hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 4>), grid, blk, lds, st, x);
-      const int rc = check_launch("grouped_matmul_mx");
-      if (rc || p.splits == 1) return rc;
-      hipLaunchKernelGGL(grouped_tail_kernel<OUT>, grid, blk, lds, st, x.g, 0, kManyRows, kColumns, 2, (int)grid.x / kXcds);
-      return check_launch("grouped_matmul_mx");
-    }
+  if (p.ring) {
+    // persistent workgroups, all that fit where tiles may be split
+    const int64_t items = ceil_div(p.bound, kXcds) * kXcds;
+    const dim3 grid((unsigned)(p.splits > 1 ? kRingSlots : std::min<int64_t>(items, kRingSlots)));
+    constexpr int BK = mx_step(FA, FB);
+    if (p.ring == 16)
+      hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 16>), grid, blk, lds, st, x);
+    else
+      hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 4>), grid, blk, lds, st, x);
+    const int rc = check_launch("grouped_matmul_mx");
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL(grouped_tail_kernel<OUT>, grid, blk, lds, st, x.g, 0, kManyRows, kColumns, 2, (int)grid.x / kXcds);
+    return check_launch("grouped_matmul_mx");
   }
   const dim3 grid((unsigned)(ceil_div(p.bound, kXcds) * kXcds));
-  if constexpr (!mx_exact(FA, FB, OUT)) {
-    if (p.few) {
-      if (p.bm == 16) hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 1>), grid, blk, lds, st, x);
-      else hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 2>), grid, blk, lds, st, x);
-      return check_launch("grouped_matmul_mx");
-    }
+  if (p.few) {
+    if (p.bm == 16) hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 1>), grid, blk, lds, st, x);
+    else hipLaunchKernelGGL((mx_few_kernel<FA, FB, OUT, 2>), grid, blk, lds, st, x);
+    return check_launch("grouped_matmul_mx");
   }
-  if (p.few)
-    hipLaunchKernelGGL((mx_kernel<FA, FB, OUT, few_rows(FA, FB), kColumns, 1, 4>), grid, blk, lds, st, x);
-  else
-    hipLaunchKernelGGL((mx_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2>), grid, blk, lds, st, x);
+  hipLaunchKernelGGL((mx_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2>), grid, blk, lds, st, x);
   const int rc = check_launch("grouped_matmul_mx");
   if (rc || p.splits == 1) return rc;
   const int64_t n = s->rows * s->N;

@@ -414,7 +414,7 @@ int rms_backward(const RmsBackward& a, hipStream_t st) {
   ProfScope ps("rms_norm_backward", st);
   int rc = ML_OK;
   if (a.rows > 0) {
-  constexpr int V16 = RowChunk<DT>::V;
+    constexpr int V16 = RowChunk<DT>::V;
     if (a.D % V16 == 0) rc = a.du ? rms_backward_launch<DT, V16, true>(a, st) : rms_backward_launch<DT, V16, false>(a, st);
     else rc = a.du ? rms_backward_launch<DT, 1, true>(a, st) : rms_backward_launch<DT, 1, false>(a, st);
   }
