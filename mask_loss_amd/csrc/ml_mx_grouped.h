@@ -330,7 +330,9 @@ __device__ __forceinline__ f32x4_t mx_mma_at(int ba, int bb, const MxFrag<FA>& a
 // that the matrix instruction takes: a workgroup has 16 MT rows by 32 columns, its four waves take turns over the reduced
 // index, 512 of it at a time (so all of a lane's loads are in flight together), and add up through LDS.  32 rows in 32
 // groups, K = 2,048, N = 1,024, e4m3 by e2m1: 9.0 us; with tiles through LDS and a join of their parts 9.3 + 2.6.
-constexpr int kFewColumns = 32, kFewStep = 512;
+// Where there are few tiles, their reductions go to several workgroups in whole turns and are joined (calls, 8 rows by e2m1: K =
+// 65,536, N = 256 59 -> 11 us, K = 16,384, N = 4,096 20 -> 15).
+constexpr int kFewColumns = 32, kFewStep = 512, kFewTurn = 4 * kFewStep;
 
 // 512 values of a row from `codes` and `scales` on, for the lanes l of the row l % 16; left: values of the row from there on.
 template <int F>
@@ -410,12 +412,13 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
   const GroupedArgs& a = x.g;
   group_edges(a, e);
   int* t = e + a.groups + 1;
-  const int tiles = segment_tiles(a, e, t, BM), id = xcd_item(tiles * a.cols.d);
+  const int tiles = segment_tiles(a, e, t, BM), count = tiles * a.cols.d, id = xcd_item(count * a.splits);
   if (id < 0) return;
-  const Work it = rows_work(a, e, t, tiles, id, 0, 1, BM, kFewColumns, kFewStep);
+  const int split = id / count;
+  const Work it = rows_work(a, e, t, tiles, id - split * count, split, a.splits, BM, kFewColumns, kFewTurn);
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
-  const int m0 = uniform(it.m0), n0 = uniform(it.n0), mlim = uniform(it.mlim), w = uniform(it.w), K = uniform(it.kend);
-  const int nlim = a.N - n0;
+  const int m0 = uniform(it.m0), n0 = uniform(it.n0), mlim = uniform(it.mlim), w = uniform(it.w);
+  const int nlim = a.N - n0, k0 = uniform(it.k), K = uniform(min(it.kend, it.k + it.steps * kFewTurn));  // the part's
   const bool mapped = uniform(it.mapped) != 0;
 
   const uint8_t *pa[MT], *sa[MT], *pb[NT], *sb[NT];
@@ -439,7 +442,7 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const MxTurn turn;
-  for (int k = wave * kFewStep; k < K; k += 4 * kFewStep) {
+  for (int k = k0 + wave * kFewStep; k < K; k += kFewTurn) {
     std::conditional_t<EXACT, MxExactRows<FA>, MxRows<FA>> ra[MT];
     std::conditional_t<EXACT, MxExactRows<FB>, MxRows<FB>> rb[NT];
 #pragma unroll
@@ -480,6 +483,7 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
       for (int j = 0; j < MT; ++j) part[wave - 1][i * MT + j][lane] = acc[i][j];
   __syncthreads();
   if (wave) return;
+  const bool planes = a.splits > 1;
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     if (16 * j + (lane & 15) >= mlim) continue;
@@ -491,14 +495,14 @@ __global__ __launch_bounds__(256) void mx_few_kernel(MxArgs x) {
       const int n = 16 * i + 4 * (lane >> 4), room = nlim - n;
       if (room <= 0) continue;
       const int64_t at = row[j] * a.ldc + n0 + n;
-      if constexpr (OUT == ML_F32) {
-        float* c = (float*)a.c + at;
+      if (planes || OUT == ML_F32) {
+        float* c = (planes ? a.parts + (int64_t)split * a.plane : (float*)a.c) + at;
         if (room >= 4) *(f32x4_loose*)c = v;
         else
 #pragma unroll
           for (int q = 0; q < 3; ++q)
             if (q < room) c[q] = v[q];
-      } else {
+      } else if constexpr (OUT != ML_F32) {
         const u32x2_t p = {GMma<OUT>::pack(v[0], v[1]), GMma<OUT>::pack(v[2], v[3])};
         uint16_t* c = (uint16_t*)a.c + at;
         if (room >= 4) *(u32x2_loose*)c = p;
