@@ -342,18 +342,19 @@ __device__ __forceinline__ int part_start(int n, int part, int parts) {
 constexpr int kBand = 4;
 // Rows kernels, tile id of tiles * column tiles.  Bands of kBand row tiles pass over the columns
 // together: their rows and the matrix's columns are both met again while they are in the L2.
+template <int BAND = kBand>
 __device__ __forceinline__ Work rows_work(const GroupedArgs& a, const int* e, const int* t, int tiles, int id, int part,
                                           int parts, int bm, int bn, int bk) {
   const int lane = threadIdx.x & 63;
   Work it;
   it.seg = 0;
-  const int band = div_by(id >> 2, a.cols);  // kBand = 4
-  const int height = min(kBand, tiles - band * kBand);
-  const int rest = id - band * kBand * a.cols.d;
+  const int band = div_by(id / BAND, a.cols);
+  const int height = min(BAND, tiles - band * BAND);
+  const int rest = id - band * BAND * a.cols.d;
   const int y = height == 4 ? rest >> 2 : height == 3 ? (int)(__umulhi((uint32_t)rest, 0xAAAAAAABu) >> 1)
                                                       : rest >> (height - 1);
   it.n0 = y * bn;
-  const int tile = band * kBand + rest - y * height;
+  const int tile = band * BAND + rest - y * height;
   int q = 0;
   for (int base = 0; base < a.segments + 2; base += 64)
     q += __popcll(__ballot(base + lane < a.segments + 2 && t[base + lane] <= tile));
@@ -925,7 +926,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC * WM * WN / 4) void grouped_ring_
 // The last round's tiles of a grouped_ring_kernel launch of `turns` workgroups an XCD (same arguments):
 // sums of their parts in order, by all workgroups of the XCD, turns / rest of them to a tile.  A part is
 // bm * bn floats as the waves' registers hold them.
-template <int DT>
+template <int DT, int BAND = kBand>
 __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg, int bm, int bn, int wn, int turns) {
   extern __shared__ int e[];
   group_edges(a, e);
@@ -937,7 +938,7 @@ __global__ __launch_bounds__(256) void grouped_tail_kernel(GroupedArgs a, int wg
   if (share.rest == 0) return;
   const int pieces = turns / share.rest, r = i / pieces, piece = i - r * pieces, tile = share.start + share.whole + r;
   if (r >= share.rest) return;
-  const Work it = wg ? weight_work(a, e, tile, 0, 1, bm, bn, 1) : rows_work(a, e, t, tiles, tile, 0, 1, bm, bn, 1);
+  const Work it = wg ? weight_work(a, e, tile, 0, 1, bm, bn, 1) : rows_work<BAND>(a, e, t, tiles, tile, 0, 1, bm, bn, 1);
   const int tm = bm / 32, tn = bn / wn / 16, chunks = 2 * wn * tm * tn;  // 2 x wn waves; 64 x 4 values to a chunk
   const f32x4_t* p = (const f32x4_t*)a.parts + (int64_t)(xcd * turns + r * share.parts) * chunks * 64 + lane;
   const int c1 = (piece + 1) * chunks / pieces;

@@ -569,6 +569,9 @@ struct alignas(16) MxItem {
   int kind;        // 1: rows of several groups (merged_row); 2: rows in no group, zeros
 };
 constexpr int kMxItems = 32;
+// (1, 2, 3, 4 row tiles to a band: 16,384 rows in 16 groups, K = 1,024, N = 4,096, e2m1 69, 71, 70, 77 us with operands from memory,
+// e4m3 by e4m3 102, 105, 103, 111; one matrix 8,192 x 8,192 x 8,192, e2m1 399, 363, 350, 352, e4m3 by e2m1 563, 492, 489, 486.)
+constexpr int kMxBand = 3;
 
 __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, const int* t, int tiles, const RingShare& share,
                                           int next, int bm, int bn, int bk) {
@@ -582,11 +585,11 @@ __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, co
     part = p - r * parts;
     if (parts > 1) it.block = p;
   }
-  const int band = div_by(id >> 2, a.cols);  // kBand = 4
-  const int height = min(kBand, tiles - band * kBand);
-  const int rest = id - band * kBand * a.cols.d, y = rest / height;
+  const int band = div_by(id / kMxBand, a.cols);
+  const int height = min(kMxBand, tiles - band * kMxBand);
+  const int rest = id - band * kMxBand * a.cols.d, y = rest / height;
   it.n0 = y * bn;
-  const int tile = band * kBand + rest - y * height;
+  const int tile = band * kMxBand + rest - y * height;
   int q = 0, end = a.segments + 1;  // the first segment whose tiles end behind this one
   while (q < end) {
     const int mid = (q + end) >> 1;
@@ -612,11 +615,11 @@ __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, co
 // index][row][4].  A row's scales are far from the next one's, so a load of 64 rows takes 64 cache lines however few bytes of
 // each: 8,192 x 8,192 x 8,192 in e2m1 took 396 us with a stage's dwords, 303 with no scale loads, 359 with these.
 //
-// What bounds it (16,384 rows in 16 groups, K = 1,024, N = 4,096, e2m1: 62 us, 76 to 78 where the operands come from memory; the
+// What bounds it (16,384 rows in 16 groups, K = 1,024, N = 4,096, e2m1: 62 us, 70 where the operands come from memory; the
 // matrix instructions alone run at 7,400 TFLOP/s on random values and are busy for 2.3 of the 7 us of a compute unit's
 // two tiles): the latency of the loads behind two stages, and the stores.  An earlier form that took 72 us took 54 without its
-// stores, 46 without loads and LDS reads, 44 without either.  Non-temporal stores take 65 for the 76, but what reads the result next
-// then waits for memory (with a product by 2 behind it 133 to 148 us, 129 as it is); half of the workgroups starting
+// stores, 46 without loads and LDS reads, 44 without either.  Non-temporal stores took 65 for 76, but what reads the result next
+// then waits for memory (with a product by 2 behind it 133 to 148 us, without them 129); half of the workgroups starting
 // a half tile later, to store while the others multiply, changes nothing.
 //
 // Products in bfloat16 (mx_exact) read a block of 32 of both operands at once and convert it, the next one's conversions

@@ -103,7 +103,7 @@ int mx_launch(const ml_grouped_shape* s, const MxPlan& p, MxArgs& x, hipStream_t
       hipLaunchKernelGGL((mx_ring_kernel<FA, FB, OUT, kManyRows, kColumns, 2, 2, BK, 2, 4>), grid, blk, lds, st, x);
     const int rc = check_launch("grouped_matmul_mx");
     if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL(grouped_tail_kernel<OUT>, grid, blk, lds, st, x.g, 0, kManyRows, kColumns, 2, (int)grid.x / kXcds);
+    hipLaunchKernelGGL((grouped_tail_kernel<OUT, kMxBand>), grid, blk, lds, st, x.g, 0, kManyRows, kColumns, 2, (int)grid.x / kXcds);
     return check_launch("grouped_matmul_mx");
   }
   const dim3 grid((unsigned)(ceil_div(p.bound, kXcds) * kXcds));
