@@ -617,8 +617,8 @@ __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, co
 //
 // What bounds it (16,384 rows in 16 groups, K = 1,024, N = 4,096, e2m1: 62 us, 70 where the operands come from memory; the
 // matrix instructions alone run at 7,400 TFLOP/s on random values and are busy for 2.3 of the 7 us of a compute unit's
-// two tiles): the latency of the loads behind two stages, and the stores.  An earlier form that took 72 us took 54 without its
-// stores, 46 without loads and LDS reads, 44 without either.  Non-temporal stores took 65 for 76, but what reads the result next
+// two tiles): the waits and other instructions around each stage's products, then the stores.  An earlier form that took 72 us took 54
+// without its stores, 46 without loads and LDS reads, 44 without either; four stages of half the length took 71 for 66.  Non-temporal stores took 65 for 76, but what reads the result next
 // then waits for memory (with a product by 2 behind it 133 to 148 us, without them 129); half of the workgroups starting
 // a half tile later, to store while the others multiply, changes nothing.
 //
