@@ -166,6 +166,17 @@ def test_split_reductions(fx, fw, rows, K, N):
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("fx,fw", PAIRS)
+@pytest.mark.parametrize("rows,M,offsets", [(50, 3, [2, 20, 31, 47]), (29, 2, [1, 9, 9, 20, 27]), (90, 3, [0, 31, 62, 90])])
+@pytest.mark.parametrize("K", [16384 + 32, 8192])
+def test_split_reductions_of_groups(dt, fx, fw, rows, M, offsets, K):
+    """The same with few rows to a group: 16 and 32 rows to a tile, rows outside, groups that share a matrix, and
+    columns and a last part of no round number."""
+    x, w = operand((rows, K), fx, 7, True, (125, 130)), operand((M, 21, K), fw, 8, True, (125, 130))
+    compare(x, w, offsets, TDT[dt], False)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("fx,fw", PAIRS)
 @pytest.mark.parametrize("rows", [6, 140])
 def test_scales(fx, fw, dt, rows):
     """The smallest and largest scales where their product is not, and NaN scales: a row's and a column's alone."""
