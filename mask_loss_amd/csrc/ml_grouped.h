@@ -348,7 +348,7 @@ __device__ __forceinline__ Work rows_work(const GroupedArgs& a, const int* e, co
   const int lane = threadIdx.x & 63;
   Work it;
   it.seg = 0;
-  const int band = div_by(id / BAND, a.cols);
+  const int band = div_by((int)((uint32_t)id / BAND), a.cols);
   const int height = min(BAND, tiles - band * BAND);
   const int rest = id - band * BAND * a.cols.d;
   const int y = height == 4 ? rest >> 2 : height == 3 ? (int)(__umulhi((uint32_t)rest, 0xAAAAAAABu) >> 1)

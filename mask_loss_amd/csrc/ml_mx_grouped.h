@@ -585,7 +585,7 @@ __device__ __forceinline__ MxItem mx_item(const GroupedArgs& a, const int* e, co
     part = p - r * parts;
     if (parts > 1) it.block = p;
   }
-  const int band = div_by(id / kMxBand, a.cols);
+  const int band = div_by((int)((uint32_t)id / kMxBand), a.cols);
   const int height = min(kMxBand, tiles - band * kMxBand);
   const int rest = id - band * kMxBand * a.cols.d, y = rest / height;
   it.n0 = y * bn;
