@@ -381,6 +381,9 @@ int experts_check(const char* who, int64_t tokens, int64_t k, int64_t experts) {
 }
 
 bool one_workgroup(int64_t n, int64_t experts) { return n <= kOneWaves * kSortItems && experts <= kOneExperts; }
+// Workgroups of a sort by several, each with a row of counts in the workspace: one at least, which writes the offsets where
+// there is no assignment.
+int64_t sort_chunks(int64_t n) { return std::max<int64_t>(1, ceil_div(n, kManyWaves * kSortItems)); }
 
 template <int W>
 size_t place_lds(int64_t experts) {
@@ -443,7 +446,7 @@ extern "C" size_t ml_sort_by_expert_workspace_size(int64_t tokens, int64_t k, in
   if (experts_check("sort_by_expert", tokens, k, experts)) return 0;
   const int64_t n = tokens * k;
   if (one_workgroup(n, experts)) return 256;
-  return align256((size_t)(ceil_div(n, kManyWaves * kSortItems) + 1) * (size_t)(experts + 1) * sizeof(int));
+  return align256((size_t)(sort_chunks(n) + 1) * (size_t)(experts + 1) * sizeof(int));
 }
 
 extern "C" int ml_sort_by_expert(const int64_t* ids, int64_t tokens, int64_t k, int64_t experts, int64_t* order,
@@ -463,7 +466,7 @@ extern "C" int ml_sort_by_expert(const int64_t* ids, int64_t tokens, int64_t k, 
   if (!workspace || workspace_bytes < ml_sort_by_expert_workspace_size(tokens, k, experts))
     return fail(ML_EWORKSPACE, "sort_by_expert: workspace too small");
   const int keys = (int)experts + 1;
-  const int64_t chunks = std::max<int64_t>(1, ceil_div(n, kManyWaves * kSortItems));
+  const int64_t chunks = sort_chunks(n);
   int* totals = (int*)workspace;
   int* counts = totals + keys;
   hipLaunchKernelGGL(expert_count_kernel, dim3((unsigned)chunks), dim3(64 * kManyWaves), (size_t)keys * sizeof(int), st, ids, n,

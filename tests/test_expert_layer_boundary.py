@@ -283,3 +283,16 @@ def test_tangents_are_refused():
                         these[0].requires_grad_(True)
                     with pytest.raises(NotImplementedError, match="forward-mode|no gradient"):
                         fn(*these)
+
+
+@pytest.mark.parametrize("experts", [1, 4, 1023, 1024, 4000])
+@pytest.mark.parametrize("tokens,k", [(0, 2), (5, 0), (0, 0), (1, 1), (1024, 1), (1025, 1), (4096, 1), (4097, 1), (70001, 3)])
+def test_sort_workspace_holds_totals_and_counts(lib, tokens, k, experts):
+    """Several workgroups keep totals and a row of counts for each 1,024 assignments, one row at least, also where there is no
+    assignment: experts + 1 numbers of 4 bytes to a row.  One workgroup (4,096 assignments and 1,023 experts at most) needs none."""
+    n, size = tokens * k, lib.ml_sort_by_expert_workspace_size(tokens, k, experts)
+    if n <= 4096 and experts <= 1023:
+        assert size == 256
+    else:
+        rows = 1 + max(1, -(-n // 1024))
+        assert rows * (experts + 1) * 4 <= size <= rows * (experts + 1) * 4 + 255
