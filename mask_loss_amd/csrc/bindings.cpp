@@ -1359,14 +1359,14 @@ struct RmsNormNode : public torch::autograd::Function<RmsNormNode> {
     no_eager_edge("rms_norm", edges, 0, need_x);
     no_eager_edge("rms_norm", edges, 1, need_w);
     no_eager_edge("rms_norm", edges, 2, need_r);
-    if (residual && g[1].defined()) gs = g[1].detach().contiguous();
     torch::Tensor dx, dw, dr;
     if (g[0].defined()) {
+      if (residual && g[1].defined()) gs = g[1].detach().contiguous();
       const auto r = rms_norm_backward(g[0].detach().contiguous(), gs, sum, w, sv[2], need_x || need_r, need_w);
       dx = r[0];
       dw = r[1];
-    } else {  // the sum alone was used
-      if (gs.has_value() && (need_x || need_r)) dx = *gs;
+    } else {  // the sum alone was used: a copy, as the upstream gradient may be another tensor's, too, and leaves keep theirs
+      if (residual && g[1].defined() && (need_x || need_r)) dx = g[1].detach().clone(at::MemoryFormat::Contiguous);
       if (need_w) dw = torch::zeros_like(*w);
     }
     if (need_r) dr = dx;

@@ -373,3 +373,46 @@ def test_views():
     assert torch.equal(out, from_experts(rows, order))
     g, = torch.autograd.grad(out, one, torch.ones_like(out))
     assert g.shape == (40, 2)
+
+
+def memory(t):
+    return t.untyped_storage().data_ptr()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_gradients_have_their_own_memory(name):
+    """Gradients that accumulate in leaves share memory with no upstream gradient and with no other leaf's: a second backward
+    and zero_() change each leaf's alone."""
+    fn, leaves, dy = operator(name)
+    want = torch.autograd.grad(fn(*leaves), leaves, dy, allow_unused=True)
+    want = [None if g is None else g.clone() for g in want]
+    up = dy.clone()
+    fn(*leaves).backward(up)
+    given = [(t, g) for t, g in zip(leaves, want) if g is not None]
+    assert len({memory(up), *[memory(t.grad) for t, _ in given]}) == len(given) + 1
+    assert all(torch.equal(t.grad, g) for t, g in given)
+    fn(*leaves).backward(up)
+    assert torch.equal(up, dy) and all(torch.equal(t.grad, g + g) for t, g in given)
+    given[0][0].grad.zero_()
+    assert torch.equal(up, dy) and all(torch.equal(t.grad, g + g) for t, g in given[1:])
+
+
+@pytest.mark.parametrize("residual_wanted", [False, True])
+def test_the_sum_beside_another_user_of_its_gradient(residual_wanted):
+    """The sum alone, added to another leaf, whose gradient is the sum's upstream one: accumulated twice, clipped in
+    place, and in a broadcast form."""
+    from mask_loss_amd.functions import rms_norm
+    x, other = (torch.randn(40, 64, device="cuda").requires_grad_(True) for _ in range(2))
+    res = torch.randn(40, 64, device="cuda").requires_grad_(residual_wanted)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    leaves = [t for t in (x, other, res) if t.requires_grad]
+    for up in (torch.ones(40, 64, device="cuda"), torch.ones((), device="cuda").expand(40, 64)):
+        ((rms_norm(x, w, 1e-6, res)[1] + other) * 1.0).backward(up)
+    assert all(bool((t.grad == 2).all()) for t in leaves)
+    assert len({memory(t.grad) for t in leaves}) == len(leaves)
+    x.grad.clamp_(max=0.5)
+    assert bool((x.grad == 0.5).all()) and all(bool((t.grad == 2).all()) for t in leaves[1:])
+    assert w.grad is None or not w.grad.any()
+    up = torch.full((40, 64), 3.0, device="cuda")
+    g, = torch.autograd.grad(rms_norm(x, w, 1e-6, res)[1], x, up)
+    assert memory(g) != memory(up) and bool((g == 3).all())
