@@ -479,7 +479,9 @@ int ml_grouped_matmul_mx(const ml_grouped_shape* s, int x_format, const void* x,
  * ml_from_experts_backward: grad_rows (tokens * k, width), zeros in the dropped places, and grad_weights (tokens, k), zeros
  * for the dropped assignments; each NULL where it is not wanted.
  * experts <= 4,000, at most 2^31 - 4,096 assignments.  slots and offsets are read on the GPU alone; places outside the
- * kept ones count as dropped, so no value reads or writes outside the tensors. */
+ * kept ones (0 .. offsets[experts] - 1) count as dropped, so no value reads or writes outside the tensors.  Each kept place is
+ * to be named by one assignment, as ml_sort_by_expert's are: a place that slots leave out stays as it was in rows and in
+ * grad_rows, one that several name has a row of any of them.  An assignment is dropped by its expert's number, before the sort. */
 size_t ml_sort_by_expert_workspace_size(int64_t tokens, int64_t k, int64_t experts);
 int ml_sort_by_expert(const int64_t* ids, int64_t tokens, int64_t k, int64_t experts, int64_t* order, int64_t* slots,
                       int64_t* offsets, void* workspace, size_t workspace_bytes, ml_stream_t stream);

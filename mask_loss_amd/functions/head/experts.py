@@ -10,7 +10,11 @@ back with weights, with their gradients.  No counterpart in the reference.
 An expert number outside 0 .. experts - 1 drops its assignment (a token over an expert's
 capacity): its place, behind all experts', holds zeros, and it counts for no sum and no
 gradient.  Nothing is read back to the host.  Gradients are not differentiated a second
-time, and forward-mode derivatives raise."""
+time, and forward-mode derivatives raise.
+
+An order that does not come from ``sort_by_expert`` has to name each place below
+``offsets[experts]`` once in ``slots``: rows of places that it leaves out are uninitialised,
+in ``to_experts`` and in the row gradient of ``from_experts``."""
 from __future__ import annotations
 
 from typing import NamedTuple

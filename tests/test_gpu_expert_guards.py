@@ -26,6 +26,10 @@ def lib():
     so.ml_sort_by_expert_workspace_size.argtypes = [i64, i64, i64]
     so.ml_sort_by_expert_workspace_size.restype = sz
     so.ml_sort_by_expert.argtypes = [vp, i64, i64, i64, vp, vp, vp, vp, sz, vp]
+    i32 = ctypes.c_int
+    so.ml_to_experts.argtypes = [vp, i64, i64, i64, vp, vp, i64, vp, vp]
+    so.ml_from_experts_forward.argtypes = [i32, i32, vp, vp, i64, i64, i64, vp, vp, i64, vp, vp]
+    so.ml_from_experts_backward.argtypes = [i32, i32, vp, vp, vp, i64, i64, i64, vp, vp, i64, vp, vp, vp]
     return so
 
 
@@ -85,3 +89,46 @@ def test_no_assignments(tokens, k, experts):
     assert order.offsets.shape == (experts + 1,) and not order.offsets.any()
     rows = to_experts(torch.randn(tokens, 24, device="cuda"), order)
     assert rows.shape == (0, 24) and not from_experts(rows, order).any()
+
+
+def ptr(t):
+    return ctypes.c_void_p(t.data_ptr())
+
+
+# lanes to a row: 16, 64 and 256; whole and cut 16-byte chunks
+@pytest.mark.parametrize("D", [32, 7, 260, 257, 1031])
+@pytest.mark.parametrize("end,kept", [(6, 6), (2 ** 62, 6), (4, 4), (1, 1), (0, 0), (-5, 0)])
+def test_places_outside(lib, end, kept, D):
+    """Places outside the kept ones, and an end outside the rows: rows, sums and gradients of the kept places that slots name, zeros
+    in the dropped places and for the dropped assignments, kept places that no slot names as they were, and nothing written
+    outside (sums of one float32 product: exact)."""
+    gen = torch.Generator().manual_seed(D + kept)
+    slots = np.array([[0, 6], [-1, 2 ** 62], [1, -2 ** 63]])
+    s, offsets = torch.from_numpy(slots).cuda(), torch.tensor([0, end], device="cuda")
+    x, y, dout, w = (torch.randn(*shape, generator=gen) for shape in ((3, D), (6, D), (3, D), (3, 2)))
+    xd, yd, gd, wd = (t.cuda() for t in (x, y, dout, w))
+    rows, out, drows, dw = Room(6 * D * 4), Room(3 * D * 4), Room(6 * D * 4), Room(6 * 4)
+    before = rows.view(torch.int32, 6, D).cpu()
+    assert lib.ml_to_experts(ptr(xd), 3, 2, D * 4, ptr(s), ptr(offsets), 1, rows.ptr, stream()) == 0
+    assert lib.ml_from_experts_forward(0, 0, ptr(yd), ptr(wd), 3, 2, D, ptr(s), ptr(offsets), 1, out.ptr, stream()) == 0
+    assert lib.ml_from_experts_backward(0, 0, ptr(gd), ptr(yd), ptr(wd), 3, 2, D, ptr(s), ptr(offsets), 1, drows.ptr, dw.ptr,
+                                        stream()) == 0
+    torch.cuda.synchronize()
+    assert all(r.whole() for r in (rows, out, drows, dw))
+    want_rows, want_drows = before.clone(), before.clone()
+    want_rows[kept:], want_drows[kept:] = 0, 0
+    want_out, want_dw, bound = torch.zeros(3, D), torch.zeros(3, 2, dtype=torch.float64), torch.zeros(3, 2, dtype=torch.float64)
+    for t in range(3):
+        for j in range(2):
+            p = int(slots[t, j])
+            if not 0 <= p < kept:
+                continue
+            want_rows[p] = x[t].view(torch.int32)
+            want_drows[p] = (w[t, j] * dout[t]).view(torch.int32)
+            want_out[t] = w[t, j] * y[p]
+            want_dw[t, j] = (dout[t].double() * y[p].double()).sum()
+            bound[t, j] = (D / 16 + 8) * 2.0 ** -24 * (dout[t].double() * y[p].double()).abs().sum()
+    assert torch.equal(rows.view(torch.int32, 6, D).cpu(), want_rows)
+    assert torch.equal(drows.view(torch.int32, 6, D).cpu(), want_drows)
+    assert torch.equal(out.view(torch.float32, 3, D).cpu(), want_out)
+    assert bool(((dw.view(torch.float32, 3, 2).cpu().double() - want_dw).abs() <= bound + 2.0 ** -24 * want_dw.abs()).all())
