@@ -319,3 +319,35 @@ def test_refusals():
                         ((x, s, w, ws, o, torch.float64), "dtype must be")):
         with pytest.raises(RuntimeError, match=words):
             grouped_matmul_mx(*args)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("fx,fw", [("e4m3", "e2m1"), ("e4m3", "e4m3"), ("e2m1", "e4m3")])
+@pytest.mark.parametrize("rows,K", [(8, 512), (200, 512), (200, 128), (200, 160)])
+def test_values_outside_bfloat16(rows, K, fx, fw, dt):
+    """An e4m3 operand whose values with their scale lie outside bfloat16's normal range, and another that brings the products
+    back: right in 16 bits, where the instruction applies both scales at once; in float32 the largest values are infinite from
+    2^128 on and the smallest count as they are or as zero below 2^-126.  All values are equal: sums are exact."""
+    def full(shape, format, value, scale):
+        codes, _ = mx.kept(torch.full((*shape, K), value), format)
+        return codes, torch.full((*shape, K // 32), scale, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+
+    which = "x" if fx == "e4m3" else "w"
+    # (codes of 448, of 256 and, for a block of ones, of the format's last binade: 256 or 4)
+    for value, scale, result in ((448.0, 254, "infinite"), (256.0, 246, "exact"), (256.0, 0, "exact"), (256.0, 0, "small")):
+        other = 27 if scale > 127 else 227
+        a = full((rows,), fx, value if which == "x" else 1.0, scale if which == "x" else other)
+        b = full((1, 24), fw, value if which == "w" else 1.0, scale if which == "w" else other)
+        if result == "small":  # the format's smallest value: 2^-9 2^-127
+            t = a if which == "x" else b
+            t[0].view(torch.uint8).fill_(1)
+        y = call(a, b, [0, rows], TDT[dt]).double().cpu()
+        want = mx.decode(*a) @ mx.decode(*b)[0].t()
+        assert float(want.max()) == float(want.min()) and 2.0 ** -120 < float(want[0, 0]) < 2.0 ** 120
+        near = (y - want).abs() <= STEP[TDT[dt]] * want
+        if dt == "f32" and result == "infinite":
+            assert bool(torch.isinf(y).all())
+        elif dt == "f32" and result == "small":
+            assert bool((near | (y == 0)).all()) and float(y.max()) == float(y.min())
+        else:
+            assert bool(near.all())
