@@ -416,3 +416,28 @@ def test_the_sum_beside_another_user_of_its_gradient(residual_wanted):
     up = torch.full((40, 64), 3.0, device="cuda")
     g, = torch.autograd.grad(rms_norm(x, w, 1e-6, res)[1], x, up)
     assert memory(g) != memory(up) and bool((g == 3).all())
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_function_classes(grad):
+    """The operators' Function classes: results and gradients of the functions, with and without leaves that want them."""
+    from mask_loss_amd.functions import (FromExpertsFunction, RMSNormFunction, ToExpertsFunction, from_experts, rms_norm,
+                                         sort_by_expert, to_experts)
+    gen = torch.Generator().manual_seed(8)
+    x, res = (torch.randn(40, 64, generator=gen).cuda() for _ in range(2))
+    w, y, g = torch.randn(64, generator=gen).cuda(), torch.randn(80, 64, generator=gen).cuda(), torch.rand(40, 2, generator=gen).cuda()
+    order = sort_by_expert(torch.randint(-1, 5, (40, 2), generator=gen).cuda(), 4)
+    calls = [(lambda a: RMSNormFunction.apply(a), rms_norm, (x,)),
+             (lambda a, b: RMSNormFunction.apply(a, b, 1e-5), lambda a, b: rms_norm(a, b, 1e-5), (x, w)),
+             (lambda a, b, c: RMSNormFunction.apply(a, b, 1e-5, c), lambda a, b, c: rms_norm(a, b, 1e-5, c), (x, w, res)),
+             (lambda a: ToExpertsFunction.apply(a, order.slots, order.offsets), lambda a: to_experts(a, order), (x,)),
+             (lambda a: FromExpertsFunction.apply(a, order.slots, order.offsets), lambda a: from_experts(a, order), (y,)),
+             (lambda a, b: FromExpertsFunction.apply(a, order.slots, order.offsets, b), lambda a, b: from_experts(a, order, b), (y, g))]
+    for one, other, args in calls:
+        leaves = [t.clone().requires_grad_(grad) for t in args]
+        got, want = ([o] if isinstance(o, torch.Tensor) else list(o) for o in (one(*leaves), other(*leaves)))
+        assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(o.requires_grad == grad for o in got)
+        if grad:
+            ups = [torch.randn(o.shape, generator=gen).cuda() for o in got]
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, ups), torch.autograd.grad(want, leaves, ups)))
